@@ -135,6 +135,20 @@ __device__ __forceinline__ int xcd_remap(int bid, int nb) {
     return xcd < r ? xcd * (q + 1) + slot : r * (q + 1) + (xcd - r) * q + slot;
 }
 
+// Fast unsigned division by a runtime constant (Granlund-Montgomery round-up method).
+struct FastDiv {
+    uint32_t d, m, s;
+    __host__ __device__ FastDiv() : d(1), m(0), s(0) {}
+    __host__ explicit FastDiv(uint32_t div) : d(div) {
+        s = 0;
+        while ((1u << s) < div) ++s;
+        m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - div)) / div + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const {
+        return (uint32_t)(((uint64_t)__umulhi(n, m) + n) >> s);
+    }
+};
+
 // ---------------------------------------------------------------- buffer -> LDS transfers
 // 16 bytes per lane from a buffer straight into LDS: lane i writes LDS byte address
 // lds + 16 i (buffer_load_dwordx4 ... lds; the compiler loads M0 = lds). Out-of-range offsets write zeros and

@@ -182,6 +182,11 @@ struct fa_ctx {
     // growable scratch for the backward's partial dK, dV (fa::BackwardSplit)
     void* ws_part = nullptr;
     size_t ws_part_bytes = 0;
+    // growable scratch of the device-resident batch: reservation plans, attention partials
+    void* ws_plan = nullptr;
+    size_t ws_plan_bytes = 0;
+    void* ws_tree = nullptr;
+    size_t ws_tree_bytes = 0;
     int backward_ds_policy = -1;
     // dK/dV kernel of the backward: -1 / 1 the assembly kernel where it applies, 0 HIP only
     int backward_kernel_policy = -1;
@@ -518,6 +523,7 @@ const char* fa_status_string(int s) {
         case FA_ERR_NULL_ARGUMENT: return "NullArgument";
         case FA_ERR_HIP: return "Hip";
         case FA_ERR_SCRATCH_EXCEEDED: return "ScratchExceeded";
+        case FA_ERR_MISALIGNED: return "Misaligned";
         default: return "Unknown";
     }
 }
@@ -607,6 +613,8 @@ int fa_ctx_destroy(fa_ctx* ctx) {
     if (ctx->ws_delta) (void)hipFree(ctx->ws_delta);
     if (ctx->ws_ds) (void)hipFree(ctx->ws_ds);
     if (ctx->ws_part) (void)hipFree(ctx->ws_part);
+    if (ctx->ws_plan) (void)hipFree(ctx->ws_plan);
+    if (ctx->ws_tree) (void)hipFree(ctx->ws_tree);
     if (ctx->meta_dev) (void)hipFree(ctx->meta_dev);
     for (const auto& s : ctx->pending) {
         (void)hipEventDestroy(s.begin);
@@ -3254,6 +3262,338 @@ int fa_backward_recompute_mha(fa_ctx* ctx, const void* packed_forward, size_t fo
     const fa_grouped_shape g{sh->batch, sh->heads, sh->heads, sh->seq_len, sh->head_dim};
     return fa_backward_grouped_recompute(ctx, packed_forward, forward_bytes, packed_grads,
                                          grads_bytes, &g, cfg, dtype);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ device-resident batch
+namespace {
+
+// Sizes and index ranges of a batch; `tables`: its block tables are used. *capacity: tokens a row holds.
+int check_batch(const fa_paged_batch* b, bool tables, uint64_t* capacity) {
+    if (!b) return fail(FA_ERR_NULL_ARGUMENT, "batch is null");
+    if (!b->n_seqs || !b->max_pages)
+        return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
+    if (!b->page_size || !b->physical_pages)
+        return fail(FA_ERR_PAGED_ZERO_DIMENSION, "paged KV dimensions must be non-zero");
+    uint64_t entries, rows;
+    if (mul_ov(b->page_size, b->physical_pages, &rows) || rows > kI32 ||
+        mul_ov(b->max_pages, b->page_size, capacity) || *capacity > kI32 ||
+        mul_ov(b->n_seqs, b->max_pages, &entries) || entries > kI32)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the i32 index space");
+    if (int rc = check_buffer("context lengths", b->ctx_lens, b->ctx_lens_bytes, b->n_seqs * 4))
+        return rc;
+    if (tables)
+        if (int rc = check_buffer("block tables", b->block_tables, b->block_tables_bytes, entries * 4))
+            return rc;
+    return FA_OK;
+}
+
+int check_aligned(const char* name, const void* p) {
+    if ((uintptr_t)p % 16)
+        return fail(FA_ERR_MISALIGNED, "buffer %s does not start at a multiple of 16 bytes", name);
+    return FA_OK;
+}
+
+// Heads, storage and pools of a batch; *row: bytes of a pool row.
+int check_pools(const fa_paged_batch* b, const void* k_pool, const void* v_pool, size_t pool_bytes,
+                uint64_t kv_heads, uint64_t head_dim, int dtype, uint64_t* row) {
+    if (int rc = check_dtype(dtype)) return rc;
+    if (!kv_heads || !head_dim)
+        return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
+    const uint64_t unit = dtype == FA_DTYPE_F32 ? 4 : 8;
+    if (head_dim % unit)
+        return fail(FA_ERR_UNSUPPORTED_HEAD_DIM, "head_dim %llu is not a multiple of %llu, required for %s storage",
+                    (unsigned long long)head_dim, (unsigned long long)unit, dtype_name(dtype));
+    uint64_t need;
+    if (mul_ov(kv_heads, head_dim, row) || *row > kI32 || mul_ov(*row, elem_bytes(dtype), row) ||
+        mul_ov(b->page_size * b->physical_pages, *row, &need))
+        return fail(FA_ERR_SHAPE_OVERFLOW, "attention shape overflows the address space");
+    if (int rc = check_buffer("K pool", k_pool, pool_bytes, need)) return rc;
+    if (int rc = check_buffer("V pool", v_pool, pool_bytes, need)) return rc;
+    if (int rc = check_aligned("K pool", k_pool)) return rc;
+    return check_aligned("V pool", v_pool);
+}
+
+int check_tree_tokens(uint64_t max_tokens) {
+    if (!max_tokens) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
+    if (max_tokens > (uint64_t)fa::kTreeTokens)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "%llu drafted tokens exceed the maximum %d",
+                    (unsigned long long)max_tokens, fa::kTreeTokens);
+    return FA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa_paged_reserve_slots(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* new_lens,
+                           size_t new_lens_bytes, uint64_t max_new, const int32_t* mapped,
+                           int32_t* mapped_out, size_t mapped_bytes, int32_t* free_pages,
+                           size_t free_pages_bytes, const int32_t* free_count,
+                           int32_t* free_count_out, size_t free_count_bytes, int32_t* granted,
+                           size_t granted_bytes, int32_t* slots, size_t slots_bytes) {
+    uint64_t capacity, n_slots;
+    if (int rc = check_batch(b, true, &capacity)) return rc;
+    if (!max_new) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
+    const uint64_t n = b->n_seqs;
+    if (mul_ov(n, max_new, &n_slots) || n_slots > kI32)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "slot map exceeds the i32 index space");
+    if (int rc = check_buffer("new lengths", new_lens, new_lens_bytes, n * 4)) return rc;
+    if (int rc = check_buffer("mapped pages", mapped, mapped_bytes, n * 4)) return rc;
+    if (int rc = check_buffer("mapped pages out", mapped_out, mapped_bytes, n * 4)) return rc;
+    if (int rc = check_buffer("free pages", free_pages, free_pages_bytes, 4)) return rc;
+    if (int rc = check_buffer("free count", free_count, free_count_bytes, 4)) return rc;
+    if (int rc = check_buffer("free count out", free_count_out, free_count_bytes, 4)) return rc;
+    if (int rc = check_buffer("granted", granted, granted_bytes, n * 4)) return rc;
+    if (int rc = check_buffer("slots", slots, slots_bytes, n_slots * 4)) return rc;
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int rc = set_device(ctx)) return rc;
+    fa::ReserveArgs a{};
+    if (!fa::reserve_fused((int)n, (int)max_new))
+        if (int rc = grow(ctx, &ctx->ws_plan, &ctx->ws_plan_bytes, (n + 1) * sizeof(int4),
+                          (void**)&a.plan))
+            return rc;
+    a.block_tables = b->block_tables;
+    a.ctx_lens = b->ctx_lens;
+    a.new_lens = new_lens;
+    a.mapped = mapped;
+    a.mapped_out = mapped_out;
+    a.free_pages = free_pages;
+    a.free_count = free_count;
+    a.free_count_out = free_count_out;
+    a.granted = granted;
+    a.slots = slots;
+    a.n_seqs = (int)n;
+    a.max_pages = (int)b->max_pages;
+    a.max_new = (int)max_new;
+    a.page_size = (int)b->page_size;
+    a.physical_pages = (int)b->physical_pages;
+    a.free_capacity = (int)std::min<uint64_t>(free_pages_bytes / 4, kI32);
+    unsigned grid[3], block, dispatches;
+    begin_span(ctx);
+    fa::launch_reserve(a, ctx->stream, grid, &block, &dispatches);
+    end_span(ctx, FA_KERNEL_PAGED_RESERVE);
+    HIP_TRY(hipGetLastError());
+    record(ctx, FA_KERNEL_PAGED_RESERVE, dispatches > 1 ? "reserve_plan + reserve_fill" : "reserve_plan",
+           0, (uint32_t)b->page_size, grid, block, dispatches, 1, nullptr);
+    return ok();
+}
+
+int fa_paged_tree_masks(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* parents,
+                        size_t parents_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                        uint64_t max_tokens, uint64_t* masks, size_t masks_bytes,
+                        int32_t* positions, size_t positions_bytes) {
+    uint64_t capacity;
+    if (int rc = check_batch(b, false, &capacity)) return rc;
+    if (int rc = check_tree_tokens(max_tokens)) return rc;
+    const uint64_t n = b->n_seqs, words = (max_tokens + 63) / 64;
+    if (n * max_tokens > kI32)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "drafted tokens exceed the i32 index space");
+    if (int rc = check_buffer("parents", parents, parents_bytes, n * max_tokens * 4)) return rc;
+    if (int rc = check_buffer("tree lengths", tree_lens, tree_lens_bytes, n * 4)) return rc;
+    if (int rc = check_buffer("masks", masks, masks_bytes, n * max_tokens * words * 8)) return rc;
+    if (int rc = check_buffer("positions", positions, positions_bytes, n * max_tokens * 4)) return rc;
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int rc = set_device(ctx)) return rc;
+    fa::TreeMaskArgs a{};
+    a.parents = parents;
+    a.tree_lens = tree_lens;
+    a.ctx_lens = b->ctx_lens;
+    a.masks = masks;
+    a.positions = positions;
+    a.n_seqs = (int)n;
+    a.max_tokens = (int)max_tokens;
+    a.words = (int)words;
+    unsigned grid[3], block;
+    begin_span(ctx);
+    fa::launch_tree_masks(a, ctx->stream, grid, &block);
+    end_span(ctx, FA_KERNEL_TREE_MASKS);
+    HIP_TRY(hipGetLastError());
+    record(ctx, FA_KERNEL_TREE_MASKS, "tree_masks", (uint32_t)max_tokens, 0, grid, block, 1, 1, nullptr);
+    return ok();
+}
+
+int fa_paged_append_slots(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* slots,
+                          size_t slots_bytes, const int32_t* positions, size_t positions_bytes,
+                          uint64_t max_new, const void* k_src, const void* v_src,
+                          size_t src_bytes, void* k_pool, void* v_pool, size_t pool_bytes,
+                          uint64_t kv_heads, uint64_t head_dim, const fa_rotary* rot, int dtype) {
+    uint64_t capacity, row, rows, pieces, need;
+    if (int rc = check_batch(b, false, &capacity)) return rc;
+    if (!max_new) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
+    if (int rc = check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)) return rc;
+    if (mul_ov(b->n_seqs, max_new, &rows) || rows > kI32 || mul_ov(rows, row / 16, &pieces) ||
+        pieces > 0xffffffffull)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged append exceeds the index space");
+    need = rows * row;
+    if (int rc = check_buffer("slots", slots, slots_bytes, rows * 4)) return rc;
+    if (positions)
+        if (int rc = check_buffer("positions", positions, positions_bytes, rows * 4)) return rc;
+    if (int rc = check_buffer("K", k_src, src_bytes, need)) return rc;
+    if (int rc = check_buffer("V", v_src, src_bytes, need)) return rc;
+    if (int rc = check_aligned("K", k_src)) return rc;
+    if (int rc = check_aligned("V", v_src)) return rc;
+    if (rot) {
+        if (head_dim > kMaxHeadDim)  // (the table's frequencies travel in the kernel arguments)
+            return fail(FA_ERR_UNSUPPORTED_HEAD_DIM, "head_dim %llu exceeds maximum %llu",
+                        (unsigned long long)head_dim, (unsigned long long)kMaxHeadDim);
+        if (int rc = check_rotary(rot->theta, rot->position_offset, head_dim, capacity)) return rc;
+    }
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int rc = set_device(ctx)) return rc;
+    fa::SlotAppendArgs a{};
+    if (rot)
+        if (int rc = ensure_rope(ctx, rot->theta, head_dim, rot->position_offset + capacity,
+                                 &a.rope_table))
+            return rc;
+    a.k_src = k_src;
+    a.v_src = v_src;
+    a.k_pool = k_pool;
+    a.v_pool = v_pool;
+    a.slots = slots;
+    a.positions = positions;
+    a.ctx_lens = b->ctx_lens;
+    a.rope_positions = (int64_t)capacity;
+    a.rope_offset = rot ? (int)rot->position_offset : 0;
+    a.n_rows = (int)rows;
+    a.max_new = (int)max_new;
+    a.pool_rows = (int)(b->page_size * b->physical_pages);
+    a.kv_heads = (int)kv_heads;
+    a.head_dim = (int)head_dim;
+    unsigned grid[3];
+    begin_span(ctx);
+    fa::launch_append_slots((Dtype)dtype, a, ctx->stream, grid);
+    end_span(ctx, FA_KERNEL_PAGED_APPEND);
+    HIP_TRY(hipGetLastError());
+    record(ctx, FA_KERNEL_PAGED_APPEND, "append_slots", 0, (uint32_t)b->page_size, grid, 256, 1, 1,
+           nullptr);
+    return ok();
+}
+
+int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q, size_t q_bytes,
+                            const void* k_pool, const void* v_pool, size_t pool_bytes,
+                            void* out_lse, size_t out_bytes, const int32_t* tree_lens,
+                            size_t tree_lens_bytes, const int32_t* positions,
+                            size_t positions_bytes, const uint64_t* masks, size_t masks_bytes,
+                            uint64_t max_tokens, uint64_t q_heads, uint64_t kv_heads,
+                            uint64_t head_dim, const fa_config* cfg, const fa_rotary* rot,
+                            int dtype) {
+    uint64_t capacity, row, lse, elements;
+    if (int rc = check_batch(b, true, &capacity)) return rc;
+    if (int rc = check_tree_tokens(max_tokens)) return rc;
+    if (!q_heads) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
+    if (int rc = check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)) return rc;
+    if (q_heads % kv_heads)
+        return fail(FA_ERR_INVALID_HEAD_GROUPING,
+                    "q_heads (%llu) must be exactly divisible by kv_heads (%llu)",
+                    (unsigned long long)q_heads, (unsigned long long)kv_heads);
+    if (int rc = check_head_dim(head_dim, dtype)) return rc;
+    float scale;
+    if (int rc = resolve_scale(cfg, head_dim, &scale)) return rc;
+    if (rot)
+        if (int rc = check_rotary(rot->theta, rot->position_offset, head_dim, capacity)) return rc;
+    const uint64_t n = b->n_seqs, words = (max_tokens + 63) / 64;
+    if (q_heads > kI32 || n * max_tokens > kI32 || mul_ov(n * max_tokens, q_heads, &lse) || lse > kI32)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "drafted tokens exceed the i32 index space");
+    elements = lse * head_dim;
+    fa_packed_layout lay;
+    if (int rc = fa_packed_layout_for(elements, lse, dtype, &lay)) return rc;
+    if (int rc = check_buffer("Q", q, q_bytes, elements * elem_bytes(dtype))) return rc;
+    if (int rc = check_buffer("O|LSE", out_lse, out_bytes, lay.combined_bytes)) return rc;
+    if (int rc = check_aligned("Q", q)) return rc;
+    if (int rc = check_aligned("O|LSE", out_lse)) return rc;
+    if (int rc = check_buffer("tree lengths", tree_lens, tree_lens_bytes, n * 4)) return rc;
+    if (positions)
+        if (int rc = check_buffer("positions", positions, positions_bytes, n * max_tokens * 4)) return rc;
+    if (masks)
+        if (int rc = check_buffer("masks", masks, masks_bytes, n * max_tokens * words * 8)) return rc;
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int rc = set_device(ctx)) return rc;
+    fa::TreeArgs a{};
+    if (rot)
+        if (int rc = ensure_rope(ctx, rot->theta, head_dim, rot->position_offset + capacity,
+                                 &a.rope_table))
+            return rc;
+    a.q = q;
+    a.k_pool = k_pool;
+    a.v_pool = v_pool;
+    a.o = out_lse;
+    a.lse = (float*)((uint8_t*)out_lse + lay.lse_byte_offset);
+    a.block_tables = b->block_tables;
+    a.ctx_lens = b->ctx_lens;
+    a.tree_lens = tree_lens;
+    a.positions = positions;
+    a.masks = masks;
+    a.rope_positions = (int64_t)capacity;
+    a.rope_offset = rot ? (int)rot->position_offset : 0;
+    a.n_seqs = (int)n;
+    a.max_tokens = (int)max_tokens;
+    a.words = (int)words;
+    a.q_heads = (int)q_heads;
+    a.kv_heads = (int)kv_heads;
+    a.group = (int)(q_heads / kv_heads);
+    a.head_dim = (int)head_dim;
+    a.max_pages = (int)b->max_pages;
+    a.page_size = (int)b->page_size;
+    a.physical_pages = (int)b->physical_pages;
+    a.scale = scale;
+    unsigned grid[3], block, dispatches;
+    begin_span(ctx);
+    fa::launch_tree_attention((Dtype)dtype, a, ctx->stream, grid, &block, &dispatches);
+    end_span(ctx, FA_KERNEL_TREE_ATTENTION);
+    HIP_TRY(hipGetLastError());
+    record(ctx, FA_KERNEL_TREE_ATTENTION, "tree_rows", 1, 64, grid, block, dispatches, 1, nullptr);
+    return ok();
+}
+
+int fa_paged_accept(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* paths,
+                    size_t paths_bytes, uint64_t max_accept, const int32_t* accepted,
+                    size_t accepted_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                    int32_t* ctx_lens_out, size_t ctx_lens_out_bytes, void* k_pool, void* v_pool,
+                    size_t pool_bytes, uint64_t kv_heads, uint64_t head_dim, int dtype) {
+    uint64_t capacity, row, cells;
+    if (int rc = check_batch(b, true, &capacity)) return rc;
+    if (int rc = check_tree_tokens(max_accept)) return rc;
+    if (int rc = check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)) return rc;
+    const uint64_t n = b->n_seqs;
+    if (mul_ov(n, max_accept, &cells) || cells > kI32)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "accepted paths exceed the i32 index space");
+    if (int rc = check_buffer("paths", paths, paths_bytes, cells * 4)) return rc;
+    if (int rc = check_buffer("accepted", accepted, accepted_bytes, n * 4)) return rc;
+    if (int rc = check_buffer("tree lengths", tree_lens, tree_lens_bytes, n * 4)) return rc;
+    if (int rc = check_buffer("context lengths out", ctx_lens_out, ctx_lens_out_bytes, n * 4)) return rc;
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int rc = set_device(ctx)) return rc;
+    fa::AcceptArgs a{};
+    a.block_tables = b->block_tables;
+    a.ctx_lens = b->ctx_lens;
+    a.ctx_lens_out = ctx_lens_out;
+    a.paths = paths;
+    a.accepted = accepted;
+    a.tree_lens = tree_lens;
+    a.k_pool = k_pool;
+    a.v_pool = v_pool;
+    a.n_seqs = (int)n;
+    a.max_pages = (int)b->max_pages;
+    a.page_size = (int)b->page_size;
+    a.physical_pages = (int)b->physical_pages;
+    a.max_tokens = fa::kTreeTokens;
+    a.max_accept = (int)max_accept;
+    a.row_pieces = (int)(row / 16);
+    unsigned grid[3], block;
+    begin_span(ctx);
+    fa::launch_accept(a, ctx->stream, grid, &block);
+    end_span(ctx, FA_KERNEL_PAGED_ACCEPT);
+    HIP_TRY(hipGetLastError());
+    record(ctx, FA_KERNEL_PAGED_ACCEPT, "accept_rows", (uint32_t)max_accept, (uint32_t)b->page_size,
+           grid, block, 1, 1, nullptr);
+    return ok();
 }
 
 }  // extern "C"

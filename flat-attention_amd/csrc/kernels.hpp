@@ -317,4 +317,90 @@ void launch_rotate_rows_split(const void* in, void* hi, void* lo, int rows, int 
 void launch_rotate_rows(Dtype dt, const void* in, void* out, int rows, int heads, int head_dim,
                         int64_t period, const float2* table, int offset, hipStream_t s);
 
+// Most tokens of a drafted tree.
+constexpr int kTreeTokens = 512;
+
+// Slots for new tokens from request lengths (all pointers on the device). `plan` is scratch of
+// n_seqs + 1 entries, used where reserve_fused() is false.
+struct ReserveArgs {
+    int* block_tables;  // [n_seqs, max_pages]
+    int* ctx_lens;      // [n_seqs], zeroed for ended sequences
+    const int* new_lens;
+    const int* mapped;
+    int* mapped_out;
+    int* free_pages;  // stack of free_capacity entries
+    const int* free_count;
+    int* free_count_out;
+    int* granted;
+    int* slots;  // [n_seqs, max_new]
+    int4* plan;
+    int n_seqs, max_pages, max_new, page_size, physical_pages, free_capacity;
+};
+bool reserve_fused(int n_seqs, int max_new);
+void launch_reserve(const ReserveArgs& a, hipStream_t s, unsigned grid[3], unsigned* block,
+                    unsigned* dispatches);
+
+// Ancestor masks and positions of drafted trees of at most kTreeTokens tokens.
+struct TreeMaskArgs {
+    const int* parents;    // [n_seqs, max_tokens]
+    const int* tree_lens;  // [n_seqs]
+    const int* ctx_lens;
+    uint64_t* masks;  // [n_seqs, max_tokens, words]
+    int* positions;   // [n_seqs, max_tokens]
+    int n_seqs, max_tokens, words;
+};
+void launch_tree_masks(const TreeMaskArgs& a, hipStream_t s, unsigned grid[3], unsigned* block);
+
+// Rows to pool slots, optionally rotating K rows.
+struct SlotAppendArgs {
+    const void* k_src;  // [n_seqs, max_new, kv_heads*head_dim]
+    const void* v_src;
+    void* k_pool;
+    void* v_pool;
+    const int* slots;      // [n_seqs, max_new]
+    const int* positions;  // [n_seqs, max_new], null: ctx_lens + token
+    const int* ctx_lens;
+    const float2* rope_table;  // null: copy K as is
+    int64_t rope_positions;    // positions the table has behind rope_offset
+    int rope_offset;
+    int n_rows, max_new, pool_rows, kv_heads, head_dim;
+};
+void launch_append_slots(Dtype dt, const SlotAppendArgs& a, hipStream_t s, unsigned grid[3]);
+
+// Accepted rows of drafted trees moved behind the live ones; row_pieces 16-byte pieces a row.
+struct AcceptArgs {
+    const int* block_tables;
+    const int* ctx_lens;
+    int* ctx_lens_out;
+    const int* paths;  // [n_seqs, max_accept]
+    const int* accepted;
+    const int* tree_lens;
+    void* k_pool;
+    void* v_pool;
+    int n_seqs, max_pages, page_size, physical_pages, max_tokens, max_accept, row_pieces;
+};
+void launch_accept(const AcceptArgs& a, hipStream_t s, unsigned grid[3], unsigned* block);
+
+// Attention of drafted tokens over the paged cache, lengths and tables on the device.
+struct TreeArgs {
+    const void* q;  // [n_seqs, max_tokens, q_heads*head_dim]
+    const void* k_pool;
+    const void* v_pool;
+    void* o;     // like q
+    float* lse;  // [n_seqs, q_heads, max_tokens]
+    const int* block_tables;
+    const int* ctx_lens;
+    const int* tree_lens;
+    const int* positions;    // [n_seqs, max_tokens], null: ctx_lens + token
+    const uint64_t* masks;   // [n_seqs, max_tokens, words], null: token t sees drafted ones 0..t
+    const float2* rope_table;  // null: Q as it is
+    int64_t rope_positions;    // positions the table has behind rope_offset
+    int rope_offset;
+    int n_seqs, max_tokens, words, q_heads, kv_heads, group, head_dim;
+    int max_pages, page_size, physical_pages;
+    float scale;
+};
+void launch_tree_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned grid[3],
+                           unsigned* block, unsigned* dispatches);
+
 }  // namespace fa

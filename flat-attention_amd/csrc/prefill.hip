@@ -31,20 +31,6 @@
 
 namespace fa {
 
-// Fast unsigned division by a runtime constant (Granlund-Montgomery round-up method).
-struct FastDiv {
-    uint32_t d, m, s;
-    __host__ __device__ FastDiv() : d(1), m(0), s(0) {}
-    __host__ explicit FastDiv(uint32_t div) : d(div) {
-        s = 0;
-        while ((1u << s) < div) ++s;
-        m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - div)) / div + 1);
-    }
-    __device__ __forceinline__ uint32_t div(uint32_t n) const {
-        return (uint32_t)(((uint64_t)__umulhi(n, m) + n) >> s);
-    }
-};
-
 // The divisors of the block map are known on the host: an integer division by a kernel argument
 // is some thirty instructions, and a lone wave issues one in about six cycles.
 struct PrefillKArgs {

@@ -11,7 +11,8 @@ from .api import (AsymmetricGroupedAttentionShape, AsymmetricRotaryEmbeddingConf
                   AttentionShape, DeviceBuffer, FlatAttentionConfig, FlatAttentionOutput,
                   GroupedAttentionShape, HipAsymmetricProjectionPipeline,
                   HipChunkedProjectionPrefillPipeline, HipContext, HipFlatAttention, HipGraph,
-                  HipPagedDecodePipeline, HipPagedKvCache, HipProjectionRotaryGroupedPipeline, HipResidentDecodePipeline,
+                  HipPagedBatch, HipPagedDecodePipeline,
+                  HipPagedKvCache, HipProjectionRotaryGroupedPipeline, HipResidentDecodePipeline,
                   HipResidentKvCache, HipRotaryGroupedAttention, ResidentDecodePlan,
                   PackedLayout, PagedChunkedPrefillPlan, PagedDecodePlan, PagedKvAddress,
                   PagedKvConfig, PagedKvTable, PagedKvTelemetry, RotaryEmbeddingConfig,

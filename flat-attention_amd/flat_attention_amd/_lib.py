@@ -33,7 +33,7 @@ STATUS = {
     30: "InvalidPage", 31: "EmptyCache", 32: "InvalidCacheLength", 33: "ForeignBuffer", 34: "CandidateNotEnabled",
     35: "UnsupportedCandidateShape", 40: "PagedZeroDimension", 41: "CapacityOverflow",
     42: "CapacityExceeded", 43: "GenerationOverflow", 50: "NullArgument", 60: "Hip",
-    61: "ScratchExceeded", 62: "GraphCapture",
+    61: "ScratchExceeded", 62: "GraphCapture", 63: "Misaligned",
 }
 
 KERNEL_IDS = {
@@ -41,7 +41,8 @@ KERNEL_IDS = {
     4: "PrefillMfmaBf16PreRotatedK", 5: "PrefillMfmaF16PreRotatedK",
     6: "PrefillMfmaF32PreRotatedK", 10: "DecodePagedSplitK", 11: "DecodeCombine",
     12: "PagedAppend", 13: "RopeTable", 14: "RopeRotate", 15: "DecodePagedMfma", 16: "TransposeV",
-    17: "BackwardRecompute",
+    17: "BackwardRecompute", 18: "TreeAttention", 19: "TreeCombine", 20: "PagedReserve",
+    21: "TreeMasks", 22: "PagedAccept",
 }
 
 
@@ -106,6 +107,12 @@ class KvAddressC(ctypes.Structure):
 class KvTelemetryC(ctypes.Structure):
     _fields_ = [("live_tokens", U64), ("capacity_tokens", U64), ("mapped_pages", U64),
                 ("free_pages", U64), ("internal_fragmentation_tokens", U64), ("generation", U64)]
+
+
+class PagedBatchC(ctypes.Structure):
+    _fields_ = [("block_tables", VP), ("block_tables_bytes", SZ), ("ctx_lens", VP),
+                ("ctx_lens_bytes", SZ), ("n_seqs", U64), ("max_pages", U64), ("page_size", U64),
+                ("physical_pages", U64)]
 
 
 # name -> (restype, argtypes)
@@ -209,6 +216,15 @@ PROTOTYPES = {
                                         INT]),
     "fa_backward_grouped": (INT, [VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, P(GroupedShapeC),
                                   P(ConfigC), INT]),
+    "fa_paged_reserve_slots": (INT, [VP, P(PagedBatchC), VP, SZ, U64, VP, VP, SZ, VP, SZ, VP, VP,
+                                     SZ, VP, SZ, VP, SZ]),
+    "fa_paged_tree_masks": (INT, [VP, P(PagedBatchC), VP, SZ, VP, SZ, U64, VP, SZ, VP, SZ]),
+    "fa_paged_append_slots": (INT, [VP, P(PagedBatchC), VP, SZ, VP, SZ, U64, VP, VP, SZ, VP, VP,
+                                    SZ, U64, U64, P(RotaryC), INT]),
+    "fa_paged_tree_attention": (INT, [VP, P(PagedBatchC), VP, SZ, VP, VP, SZ, VP, SZ, VP, SZ, VP,
+                                      SZ, VP, SZ, U64, U64, U64, U64, P(ConfigC), P(RotaryC), INT]),
+    "fa_paged_accept": (INT, [VP, P(PagedBatchC), VP, SZ, U64, VP, SZ, VP, SZ, VP, SZ, VP, VP, SZ,
+                              U64, U64, INT]),
     "fa_last_telemetry": (INT, [VP, P(TelemetryC)]),
     "fa_forward_gqa_rope_telemetry": (INT, [VP, P(GroupedShapeC), P(ConfigC), P(RotaryC), INT,
                                             P(TelemetryC)]),

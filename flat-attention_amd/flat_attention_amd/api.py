@@ -1123,6 +1123,95 @@ def paged_append_batched(ctx: HipContext, block_tables: np.ndarray, start_lens: 
                                         min(k_pool.nbytes, v_pool.nbytes), rot, dtype))
 
 
+class HipPagedBatch:
+    """A batch of sequences over one page pool whose block tables and lengths stay on the GPU
+    (fa_paged_batch; no reference counterpart). One serving step with drafted tokens is reserve,
+    tree_masks, append, tree_attention and accept, none of which needs a length on the host; a plain
+    step is reserve, append and tree_attention with one token and no masks. The methods only enqueue
+    kernels; every array is a :class:`DeviceBuffer` of int32 (masks: uint64) in the shapes that
+    include/flat_hip.h gives, and is kept alive by the caller until the stream has passed the call.
+
+    ``block_tables`` [n_seqs, max_pages] and ``ctx_lens`` [n_seqs] are bound to the batch.
+    ``block_tables`` may be None for a batch that only builds masks or appends."""
+
+    def __init__(self, ctx: HipContext, block_tables: Optional[DeviceBuffer],
+                 ctx_lens: DeviceBuffer, n_seqs: int, max_pages: int, page_size: int,
+                 physical_pages: int):
+        self.ctx, self.block_tables, self.ctx_lens = ctx, block_tables, ctx_lens
+        self.n_seqs, self.max_pages = n_seqs, max_pages
+        self.page_size, self.physical_pages = page_size, physical_pages
+        self._c = L.PagedBatchC(block_tables.ptr if block_tables is not None else None,
+                                block_tables.nbytes if block_tables is not None else 0,
+                                ctx_lens.ptr, ctx_lens.nbytes, n_seqs, max_pages, page_size,
+                                physical_pages)
+
+    def reserve(self, new_lens: DeviceBuffer, max_new: int, mapped: DeviceBuffer,
+                free_pages: DeviceBuffer, free_count: DeviceBuffer, granted: DeviceBuffer,
+                slots: DeviceBuffer, mapped_out: Optional[DeviceBuffer] = None,
+                free_count_out: Optional[DeviceBuffer] = None):
+        """Slots for the new tokens of every sequence (fa_paged_reserve_slots). ``mapped`` and
+        ``free_count`` are updated in place unless their ``_out`` arrays are given."""
+        mo, fo = mapped_out or mapped, free_count_out or free_count
+        check(lib().fa_paged_reserve_slots(
+            self.ctx.handle, self._c, new_lens.ptr, new_lens.nbytes, max_new, mapped.ptr, mo.ptr,
+            min(mapped.nbytes, mo.nbytes), free_pages.ptr, free_pages.nbytes, free_count.ptr,
+            fo.ptr, min(free_count.nbytes, fo.nbytes), granted.ptr, granted.nbytes, slots.ptr,
+            slots.nbytes))
+
+    def tree_masks(self, parents: DeviceBuffer, tree_lens: DeviceBuffer, max_tokens: int,
+                   masks: DeviceBuffer, positions: DeviceBuffer):
+        """Ancestor masks and positions of drafted trees (fa_paged_tree_masks)."""
+        check(lib().fa_paged_tree_masks(
+            self.ctx.handle, self._c, parents.ptr, parents.nbytes, tree_lens.ptr, tree_lens.nbytes,
+            max_tokens, masks.ptr, masks.nbytes, positions.ptr, positions.nbytes))
+
+    def append(self, slots: DeviceBuffer, max_new: int, k_src: DeviceBuffer, v_src: DeviceBuffer,
+               k_pool: DeviceBuffer, v_pool: DeviceBuffer, kv_heads: int, head_dim: int,
+               rotary: Optional[RotaryEmbeddingConfig], dtype: int,
+               positions: Optional[DeviceBuffer] = None):
+        """New rows to their slots, K rotated on the way (fa_paged_append_slots)."""
+        check(lib().fa_paged_append_slots(
+            self.ctx.handle, self._c, slots.ptr, slots.nbytes,
+            positions.ptr if positions is not None else None,
+            positions.nbytes if positions is not None else 0, max_new, k_src.ptr, v_src.ptr,
+            min(k_src.nbytes, v_src.nbytes), k_pool.ptr, v_pool.ptr,
+            min(k_pool.nbytes, v_pool.nbytes), kv_heads, head_dim,
+            rotary.c() if rotary is not None else None, dtype))
+
+    def layout(self, max_tokens: int, q_heads: int, head_dim: int, dtype: int) -> PackedLayout:
+        """[O | LSE] geometry of tree_attention: O like q, LSE [n_seqs, q_heads, max_tokens]."""
+        rows = self.n_seqs * max_tokens * q_heads
+        return packed_layout(rows * head_dim, rows, dtype)
+
+    def tree_attention(self, q: DeviceBuffer, k_pool: DeviceBuffer, v_pool: DeviceBuffer,
+                       out_and_lse: DeviceBuffer, tree_lens: DeviceBuffer, max_tokens: int,
+                       q_heads: int, kv_heads: int, head_dim: int, config: FlatAttentionConfig,
+                       rotary: Optional[RotaryEmbeddingConfig], dtype: int,
+                       positions: Optional[DeviceBuffer] = None,
+                       masks: Optional[DeviceBuffer] = None):
+        """Attention of the drafted tokens over the cache (fa_paged_tree_attention); no masks: a
+        chain, no positions: those of a chain."""
+        check(lib().fa_paged_tree_attention(
+            self.ctx.handle, self._c, q.ptr, q.nbytes, k_pool.ptr, v_pool.ptr,
+            min(k_pool.nbytes, v_pool.nbytes), out_and_lse.ptr, out_and_lse.nbytes, tree_lens.ptr,
+            tree_lens.nbytes, positions.ptr if positions is not None else None,
+            positions.nbytes if positions is not None else 0,
+            masks.ptr if masks is not None else None,
+            masks.nbytes if masks is not None else 0, max_tokens, q_heads, kv_heads, head_dim,
+            config.c(), rotary.c() if rotary is not None else None, dtype))
+
+    def accept(self, paths: DeviceBuffer, max_accept: int, accepted: DeviceBuffer,
+               tree_lens: DeviceBuffer, k_pool: DeviceBuffer, v_pool: DeviceBuffer, kv_heads: int,
+               head_dim: int, dtype: int, ctx_lens_out: Optional[DeviceBuffer] = None):
+        """Accepted rows into place and the lengths past them (fa_paged_accept), in ``ctx_lens`` unless
+        ``ctx_lens_out`` is given."""
+        out = ctx_lens_out or self.ctx_lens
+        check(lib().fa_paged_accept(
+            self.ctx.handle, self._c, paths.ptr, paths.nbytes, max_accept, accepted.ptr,
+            accepted.nbytes, tree_lens.ptr, tree_lens.nbytes, out.ptr, out.nbytes, k_pool.ptr,
+            v_pool.ptr, min(k_pool.nbytes, v_pool.nbytes), kv_heads, head_dim, dtype))
+
+
 # ----------------------------------------------------------------------------- backward
 
 @dataclass

@@ -82,8 +82,10 @@ typedef enum fa_status {
     FA_ERR_NULL_ARGUMENT = 50,
     FA_ERR_HIP = 60,
     FA_ERR_SCRATCH_EXCEEDED = 61, /* no reference variant: fa_paged_decode_noalloc's scratch */
-    FA_ERR_GRAPH_CAPTURE = 62     /* no reference variant: a call that allocates, uploads from the
+    FA_ERR_GRAPH_CAPTURE = 62,    /* no reference variant: a call that allocates, uploads from the
                                      host, fills or waits while the stream is being captured */
+    FA_ERR_MISALIGNED = 63        /* no reference variant: a tensor of a device-resident batch
+                                     (fa_paged_batch) that does not start at a multiple of 16 bytes */
 } fa_status;
 
 /* Storage dtype of Q/K/V/O. Math is always f32 (f32 online-softmax state, f32 accumulation);
@@ -152,7 +154,12 @@ typedef enum fa_kernel_id {
     FA_KERNEL_ROPE_ROTATE = 14,
     FA_KERNEL_DECODE_PAGED_MFMA = 15,     /* 16-bit KV, page_size % 16 == 0: P.V on MFMA */
     /* 16: retired (a transposed-V pre-pass that measured level) */
-    FA_KERNEL_BACKWARD_RECOMPUTE = 17     /* delta + dK/dV + dQ recompute backward (MFMA) */
+    FA_KERNEL_BACKWARD_RECOMPUTE = 17,    /* delta + dK/dV + dQ recompute backward (MFMA) */
+    FA_KERNEL_TREE_ATTENTION = 18,        /* drafted tokens over the paged cache */
+    FA_KERNEL_TREE_COMBINE = 19,
+    FA_KERNEL_PAGED_RESERVE = 20,         /* slots from request lengths (one or two launches) */
+    FA_KERNEL_TREE_MASKS = 21,
+    FA_KERNEL_PAGED_ACCEPT = 22
 } fa_kernel_id;
 
 /* RuntimeDispatchTelemetry src/runtime_telemetry.rs:159 + RuntimeTileGeometry :151 +
@@ -529,6 +536,108 @@ int fa_paged_append_batched(fa_ctx* ctx, const int32_t* block_tables, uint64_t m
                             uint64_t head_dim, const void* k_src, const void* v_src,
                             size_t src_bytes, void* k_pool, void* v_pool, size_t pool_bytes,
                             const fa_rotary* rotary, int dtype);
+
+/* ------------------------------------------------------------ device-resident batch ------
+ * A batch of sequences over one page pool whose block tables and lengths stay on the GPU, so that a
+ * serving step whose lengths are known there only (how many drafted tokens were accepted) runs
+ * without the host: slots are reserved, the drafted rows appended, attended over and the accepted
+ * ones moved into place by calls that read every length on the device. No counterpart in the
+ * reference, whose tables are host metadata (PagedKvTable src/paged_kv.rs:76). The calls only enqueue
+ * kernels (capturable once the context's workspaces and (cos, sin) table are sized, by one earlier
+ * call of the same or a larger shape) and give the same results each time. The pool is that of the
+ * paged cache and decode: [physical_pages, page_size, kv_heads*head_dim], K stored rotated.
+ *
+ * The host cannot check what device arrays hold. A sequence, token, slot or page that does not fit
+ * takes no part, as each call says; nothing outside the buffers is read or written. Pools, K/V
+ * sources, Q and outputs start at multiples of 16 bytes (FA_ERR_MISALIGNED). */
+typedef struct fa_paged_batch {
+    int32_t* block_tables;      /* device [n_seqs, max_pages] physical page ids */
+    size_t block_tables_bytes;
+    int32_t* ctx_lens;          /* device [n_seqs] live tokens */
+    size_t ctx_lens_bytes;
+    uint64_t n_seqs, max_pages, page_size, physical_pages;
+} fa_paged_batch;
+
+/* Slots for the new tokens of every sequence, in sequence order. All arrays are device int32:
+ *   new_lens [n_seqs]   tokens to come (<= max_new; 0: none; < 0: the sequence has ended, its mapped
+ *                       pages go back on the free stack and ctx_lens becomes 0)
+ *   mapped [n_seqs]     pages each block-table row holds; mapped_out (may be the same array) receives
+ *                       the new counts
+ *   free_pages          stack of free page ids, free_count of them from the start (capacity:
+ *                       free_pages_bytes / 4); pages come from its end, the last first, and those of
+ *                       ended sequences are put on it before any is taken, in sequence order;
+ *                       free_count_out (may be the same) receives the new count
+ *   granted [n_seqs]    new_lens, or 0 for a sequence that got no slots: it ended, it asks for none or
+ *                       for more than max_new or its table row can hold, its length is negative, or
+ *                       it needs pages and the free ones do not cover it and all sequences before it
+ *                       that fit their row. Its pages stay as they were.
+ *   slots [n_seqs, max_new]  pool row (page * page_size + offset) of token ctx_lens[s] + t, -1 for
+ *                       t >= granted[s] (and on a page id outside the pool)
+ * Lengths of sequences that go on are left for fa_paged_accept or the caller to advance. */
+int fa_paged_reserve_slots(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* new_lens,
+                           size_t new_lens_bytes, uint64_t max_new, const int32_t* mapped,
+                           int32_t* mapped_out, size_t mapped_bytes, int32_t* free_pages,
+                           size_t free_pages_bytes, const int32_t* free_count,
+                           int32_t* free_count_out, size_t free_count_bytes, int32_t* granted,
+                           size_t granted_bytes, int32_t* slots, size_t slots_bytes);
+
+/* Masks and positions of drafted trees (or forests) of at most max_tokens <= 512 tokens.
+ *   parents [n_seqs, max_tokens]  index of each token's parent, an earlier one, -1 for a root
+ *   tree_lens [n_seqs]            tokens of each tree (out of range: none)
+ *   masks [n_seqs, max_tokens, ceil(max_tokens / 64)] uint64: bit j of token t's mask (word j / 64)
+ *                                 is set for t itself and its ancestors
+ *   positions [n_seqs, max_tokens] ctx_lens + number of ancestors
+ * Tokens past tree_lens, and those with a parent that is not an earlier token, or such an ancestor,
+ * get an empty mask and position -1. The batch's block_tables are not used (may be null). */
+int fa_paged_tree_masks(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* parents,
+                        size_t parents_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                        uint64_t max_tokens, uint64_t* masks, size_t masks_bytes,
+                        int32_t* positions, size_t positions_bytes);
+
+/* Rows of k_src, v_src [n_seqs, max_new, kv_heads*head_dim] to the pool rows in slots [n_seqs,
+ * max_new] (fa_paged_reserve_slots), K rotated at rotary->position_offset + positions[s, t]
+ * (positions == NULL: ctx_lens[s] + t) when rotary != NULL. Rows with a slot outside the pool, or a
+ * position outside [0, max_pages * page_size) when rotating, are left out; two rows must not share a
+ * slot. block_tables are not used (may be null). head_dim: a multiple of 8 (f32: of 4). */
+int fa_paged_append_slots(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* slots,
+                          size_t slots_bytes, const int32_t* positions, size_t positions_bytes,
+                          uint64_t max_new, const void* k_src, const void* v_src,
+                          size_t src_bytes, void* k_pool, void* v_pool, size_t pool_bytes,
+                          uint64_t kv_heads, uint64_t head_dim, const fa_rotary* rotary, int dtype);
+
+/* Attention of the drafted tokens q [n_seqs, max_tokens, q_heads*head_dim] (max_tokens <= 512) over
+ * the cache: token t of sequence s sees the ctx_lens[s] live rows and, of the tree_lens[s] rows behind
+ * them (appended already), those whose bit is set in its mask [words of masks as in
+ * fa_paged_tree_masks; bits past tree_lens are not read]. masks == NULL: the tokens are a chain, t
+ * sees 0..t (max_tokens 1: a decode step). Q is rotated at rotary->position_offset + positions[s, t]
+ * (NULL: ctx_lens[s] + t) when rotary != NULL. config gives the softmax scale; `causal` is not
+ * consulted, the masks say what is seen. out_lse: [O like q | LSE [n_seqs, q_heads, max_tokens]] as for
+ * fa_forward_projection_asymmetric. Rows past tree_lens, rows that see nothing, rows whose position is
+ * outside [0, max_pages * page_size) when rotating, and all rows of a sequence whose lengths are
+ * negative or do not fit max_tokens and its table, get O = 0 and LSE = -inf. Keys on a page id outside
+ * the pool are as if masked, and what masked rows and rows past the live ones hold, NaN and
+ * infinities too, reaches no result. */
+int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* batch, const void* q, size_t q_bytes,
+                            const void* k_pool, const void* v_pool, size_t pool_bytes,
+                            void* out_lse, size_t out_bytes, const int32_t* tree_lens,
+                            size_t tree_lens_bytes, const int32_t* positions,
+                            size_t positions_bytes, const uint64_t* masks, size_t masks_bytes,
+                            uint64_t max_tokens, uint64_t q_heads, uint64_t kv_heads,
+                            uint64_t head_dim, const fa_config* config, const fa_rotary* rotary,
+                            int dtype);
+
+/* Accepted tokens move into place: row ctx_lens[s] + paths[s, i] of K and V to ctx_lens[s] + i for
+ * i < accepted[s], and ctx_lens_out[s] = ctx_lens[s] + accepted[s] (ctx_lens_out may be the batch's
+ * ctx_lens). paths [n_seqs, max_accept] (max_accept <= 512) holds each accepted path
+ * from the root: token indices, strictly increasing, below tree_lens[s]. K keeps its rotation: a
+ * token's position is ctx_lens + its depth, which is where its row goes. A sequence whose path is not
+ * like that, whose accepted is negative or more than max_accept or tree_lens, whose lengths do not fit
+ * or whose rows lie on a page id outside the pool is left as it is. */
+int fa_paged_accept(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* paths,
+                    size_t paths_bytes, uint64_t max_accept, const int32_t* accepted,
+                    size_t accepted_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                    int32_t* ctx_lens_out, size_t ctx_lens_out_bytes, void* k_pool, void* v_pool,
+                    size_t pool_bytes, uint64_t kv_heads, uint64_t head_dim, int dtype);
 
 /* ------------------------------------------------------------ telemetry ------------------
  * runtime_telemetry src/wgpu_backend.rs:374: metadata of the last logical call on `ctx`. */

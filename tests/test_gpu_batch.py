@@ -1,0 +1,329 @@
+"""GPU parity of the device-resident batch (fa_paged_reserve_slots, fa_paged_tree_masks,
+fa_paged_append_slots, fa_paged_tree_attention, fa_paged_accept) against plain models in integers and
+float64, alone and as the steps of a decoding loop, eager and replayed from a graph.
+
+Tolerances. h is half a rounding step of the storage type relative to the value (bf16 2^-8, f16 2^-11,
+f32 2^-24). A rotated value comes from two products and a sum in f32 of factors that are off by a few
+2^-24 themselves, then one rounding: h |x| + 2^-21 (|e| + |o|). A score is a sum of D products in f32 of
+a query kept to h^2 (or f32): off by at most B ((D + 16) 2^-24 + h^2), B = scale * sum |q k|. LSE takes
+that and the sum of n probabilities in f32 (each off by 2^-21): n 2^-24 + 2^-20, and the rounding of its
+own value and of the running maximum. O adds the rounding of each probability and of itself:
+h (|O| + sum p |v|).
+"""
+import numpy as np
+import pytest
+
+import _batch_model as model
+import flat_attention_amd as fa
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = fa.DTYPE_F32, fa.DTYPE_F16, fa.DTYPE_BF16
+HALF_STEP = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+THETA = 10000.0
+
+
+def i32(hip, x):
+    return fa.DeviceBuffer.from_array(hip, np.ascontiguousarray(x, np.int32))
+
+
+def storage(x, dtype):
+    """Values rounded to the storage type, as float64, and their stored form."""
+    st = fa.host_storage(np.ascontiguousarray(x, np.float32), dtype)
+    return fa.storage_to_f32(st.ravel(), dtype).reshape(x.shape).astype(np.float64), st
+
+
+def load(buf, shape, dtype):
+    raw = buf.download(fa.storage_np_dtype(dtype), int(np.prod(shape)))
+    return fa.storage_to_f32(raw, dtype).reshape(shape).astype(np.float64)
+
+
+def paged(rng, tokens, page, spare=3, width=None):
+    """Tables over a shuffled pool for `tokens` rows of each sequence: (table, pages)."""
+    need = [-(-int(t) // page) for t in tokens]
+    total = sum(need) + spare
+    ids = rng.permutation(total)
+    table = np.full((len(need), width or max(1, max(need))), -1, np.int32)
+    at = 0
+    for s, m in enumerate(need):
+        table[s, :m] = ids[at:at + m]
+        at += m
+    return table, total, ids[at:]
+
+
+def drafts(rng, n, most, wide=8):
+    """Random trees of at most `most` tokens: (parents, lengths), the first tree full."""
+    lens = rng.integers(1, most + 1, n)
+    lens[0] = most
+    at = np.arange(most)
+    return np.maximum(at - rng.integers(1, wide + 1, (n, most)), -1).astype(np.int32), lens
+
+
+# ------------------------------------------------------------------------------- reservation
+
+def _reserve(hip, table, ctx, new, mapped, free, count, max_new, page, pages, inplace):
+    n, width = table.shape
+    t, c, nl, m, f, k = (i32(hip, x) for x in (table, ctx, new, mapped, free, [count]))
+    granted, slots = i32(hip, np.full(n, 77)), i32(hip, np.full((n, max_new), 77))
+    out = {} if inplace else {"mapped_out": i32(hip, np.full(n, 77)), "free_count_out": i32(hip, [77])}
+    batch = fa.HipPagedBatch(hip, t, c, n, width, page, pages)
+    batch.reserve(nl, max_new, m, f, k, granted, slots, **out)
+    mo, ko = out.get("mapped_out", m), out.get("free_count_out", k)
+    if not inplace:
+        assert np.array_equal(m.download(np.int32, n), mapped)
+        assert k.download(np.int32, 1)[0] == count
+    return {"table": t.download(np.int32, n * width).reshape(n, width),
+            "ctx": c.download(np.int32, n), "mapped": mo.download(np.int32, n),
+            "free": f.download(np.int32, len(free)), "count": ko.download(np.int32, 1)[0],
+            "granted": granted.download(np.int32, n),
+            "slots": slots.download(np.int32, n * max_new).reshape(n, max_new)}
+
+
+def _compare(got, want):
+    for k, w in want.items():
+        assert np.array_equal(got[k], w), k
+
+
+@pytest.mark.parametrize("inplace", [True, False])
+@pytest.mark.parametrize("n,max_new,page,high,short,seed", [
+    (1, 1, 16, 0, 1.0, 0), (1, 1, 16, 500, 1.0, 1), (3, 7, 5, 60, 1.0, 2), (64, 32, 16, 300, 0.5, 3),
+    (65, 3, 1, 40, 0.3, 4), (300, 9, 16, 100, 0.7, 5), (1024, 8, 16, 64, 1.0, 6),
+    (1030, 4, 16, 64, 0.6, 7), (2500, 20, 8, 50, 0.8, 8), (40, 2100, 16, 200, 0.6, 9),
+    (2, 5000, 64, 100, 1.0, 10)])
+def test_reserve_matches_the_model(hip, n, max_new, page, high, short, seed, inplace):
+    """Some sequences end, some ask for nothing or too much, and the free pages cover `short` of what
+    is asked."""
+    rng = np.random.default_rng(seed)
+    ctx = rng.integers(0, high + 1, n)
+    mapped = -(-ctx // page) + rng.integers(0, 2, n)
+    new = rng.integers(0, max_new + 1, n)
+    width = int(max(mapped.max(), np.quantile(-(-(ctx + new) // page), 0.98), 1))
+    table, pages, spare = paged(rng, mapped * page, page, spare=1 + n * (1 + max_new // page), width=width)
+    if n > 2:
+        new[rng.random(n) < 0.15] = -1
+        new[rng.integers(0, n)] = max_new + 1
+    wanted = int(np.maximum(-(-(ctx + np.maximum(new, 0)) // page) - mapped, 0).sum())
+    count = min(spare.size, int(short * wanted) + 1)
+    free = np.concatenate([spare[:count], np.full(int(mapped.sum()) + 1, -5)])
+    want = model.reserve(table, ctx, new, mapped, free, count, max_new, page, pages)
+    _compare(_reserve(hip, table, ctx, new, mapped, free, count, max_new, page, pages, inplace), want)
+
+
+def test_reserve_with_arrays_that_hold_nonsense(hip):
+    """Negative lengths, mapped counts and free counts out of range, pages outside the pool, a stack too
+    short for what comes back: those take no part, nothing else changes."""
+    page, pages, width, max_new = 4, 20, 5, 6
+    ctx = np.array([-3, 2147483647, 7, 3, 4, 0])
+    new = np.array([2, 6, 2147483647, -2147483648, 3, 6])
+    mapped = np.array([0, 3, -4, 99, 1, 0])
+    table = np.arange(30).reshape(6, 5) - 3
+    free = np.array([1, 2, 50, -9, 4, 5, 6, 7])
+    for count in (6, -2, 1000):
+        c = min(max(count, 0), free.size)
+        want = model.reserve(table, ctx, new, mapped, free, c, max_new, page, pages)
+        _compare(_reserve(hip, table, ctx, new, mapped, free, count, max_new, page, pages, False), want)
+
+
+# ------------------------------------------------------------------------------- masks
+
+@pytest.mark.parametrize("n,most,wide", [(1, 1, 1), (1, 64, 1), (3, 65, 4), (5, 7, 8), (2, 512, 1),
+                                         (4, 512, 40), (200, 33, 3), (70, 256, 8)])
+def test_tree_masks_match_a_walk(hip, n, most, wide):
+    rng = np.random.default_rng(most)
+    parents, lens = drafts(rng, n, most, wide)
+    ctx = rng.integers(0, 100000, n)
+    if n > 2:  # parents that are no earlier token, lengths out of range
+        parents[1, rng.integers(0, most)] = most
+        parents[2, most // 2] = -2
+        if most > 3:
+            parents[2, 3] = 3
+    if n > 4:
+        lens[3], lens[4], ctx[n - 1] = most + 1, 0, -1
+    words = (most + 63) // 64
+    masks, pos = fa.DeviceBuffer(hip, n * most * words * 8), i32(hip, np.full((n, most), 77))
+    masks.fill_u32(0xffffffff)
+    batch = fa.HipPagedBatch(hip, None, i32(hip, ctx), n, 1, 1, 1)
+    batch.tree_masks(i32(hip, parents), i32(hip, lens), most, masks, pos)
+    seen, want = model.tree(parents, lens, ctx, most)
+    assert np.array_equal(pos.download(np.int32, n * most).reshape(n, most), want)
+    assert np.array_equal(masks.download(np.uint64, n * most * words).reshape(n, most, words),
+                          model.pack(seen))
+
+
+# ------------------------------------------------------------------------------- append
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,most,page,hkv,D,rope,positions", [
+    (1, 1, 16, 1, 8, True, False), (3, 7, 5, 2, 64, True, True), (2, 40, 16, 3, 80, True, False),
+    (4, 33, 24, 8, 128, True, True), (5, 19, 16, 4, 40, False, False)])
+def test_append_writes_the_slots_and_nothing_else(hip, dtype, n, most, page, hkv, D, rope, positions):
+    rng = np.random.default_rng(most + D)
+    ctx, new = rng.integers(0, 70, n), rng.integers(0, most + 1, n)
+    table, pages, _ = paged(rng, ctx + most, page)
+    rows = [(table[s, (c + np.arange(most)) // page].astype(np.int64) * page
+             + (c + np.arange(most)) % page) for s, c in enumerate(ctx)]
+    slots = np.where(np.arange(most) < new[:, None], np.array(rows), -1)
+    if n > 2:
+        slots[1, 0] = pages * page  # outside the pool
+        slots[2, 0] = -2147483648
+    pos = ctx[:, None] + rng.integers(0, 4, (n, most)) if positions else ctx[:, None] + np.arange(most)
+    if positions:
+        pos[0, 0] = -1  # no position: left out when rotating
+        pos[0, 1] = table.shape[1] * page
+    k, ks = storage(rng.standard_normal((n, most, hkv, D)), dtype)
+    v, vs = storage(rng.standard_normal((n, most, hkv, D)), dtype)
+    kp, kps = storage(rng.standard_normal((pages * page, hkv, D)), dtype)
+    vp, vps = storage(rng.standard_normal((pages * page, hkv, D)), dtype)
+    bufs = [fa.DeviceBuffer.from_array(hip, x) for x in (ks, vs, kps, vps)]
+    batch = fa.HipPagedBatch(hip, None, i32(hip, ctx), n, table.shape[1], page, pages)
+    off = 1000
+    batch.append(i32(hip, slots), most, *bufs, hkv, D,
+                 fa.RotaryEmbeddingConfig(THETA, off) if rope else None, dtype,
+                 positions=i32(hip, pos) if positions else None)
+    tol = np.zeros(kp.shape)
+    for s in range(n):
+        for t in range(most):
+            r = int(slots[s, t])
+            if not 0 <= r < pages * page or (rope and not 0 <= pos[s, t] < table.shape[1] * page):
+                continue
+            vp[r] = v[s, t]
+            kp[r] = model.rotate(k[s, t][None], [pos[s, t] + off], THETA)[0] if rope else k[s, t]
+            if rope:
+                size = np.abs(k[s, t, :, 0::2]) + np.abs(k[s, t, :, 1::2])
+                tol[r] = HALF_STEP[dtype] * np.abs(kp[r]) + 2.0 ** -21 * np.repeat(size, 2, -1)
+                if dtype == F16:
+                    tol[r] += 2.0 ** -25  # half a step of the smallest numbers
+    assert np.array_equal(load(bufs[3], vp.shape, dtype), vp)
+    assert (np.abs(load(bufs[2], kp.shape, dtype) - kp) <= tol).all()
+
+
+# ------------------------------------------------------------------------------- attention
+
+class Case:
+    """Inputs of an attention call over a shuffled pool, its buffers and its float64 result."""
+
+    def __init__(self, hip, dtype, ctx, lens, most, hq, hkv, D, page, seed, tree=True, rope=True,
+                 scale=None, offset=0, magnitude=1.0, nan_outside=True, wide=5):
+        self.hip, self.dtype, self.most, self.dims = hip, dtype, most, (hq, hkv, D)
+        rng = np.random.default_rng(seed)
+        self.ctx, self.lens, self.page = np.asarray(ctx), np.asarray(lens), page
+        n = len(ctx)
+        fit = [c + m if c >= 0 and 0 <= m <= most else 0 for c, m in zip(ctx, lens)]
+        self.table, self.pages, _ = paged(rng, fit, page)
+        self.q, qs = storage(magnitude * rng.standard_normal((n, most, hq, D)), dtype)
+        rows = self.pages * page
+        self.k, self.ks = storage(rng.standard_normal((rows, hkv, D)), dtype)
+        self.v, self.vs = storage(rng.standard_normal((rows, hkv, D)), dtype)
+        live = np.zeros(rows, bool)
+        for s in range(n):
+            live[self.rows(s, fit[s])] = True
+        if nan_outside:  # rows that are nobody's: not a number
+            nan = fa.host_storage(np.array([np.nan], np.float32), dtype)[0]
+            self.ks[~live] = nan
+            self.vs[~live] = nan
+        self.seen, self.pos, self.masks = None, None, None
+        at = np.arange(most)
+        self.sees = np.broadcast_to(np.tril(np.ones((most, most), bool)), (n, most, most))
+        self.where = self.ctx[:, None] + at
+        if tree:
+            parents, _ = drafts(rng, n, most, wide)
+            self.sees, self.where = model.tree(parents, self.lens, self.ctx, most)
+            self.masks, self.pos = model.pack(self.sees), self.where
+        self.scale, self.offset, self.rope = scale, offset, rope
+        self.bufs = [fa.DeviceBuffer.from_array(hip, x) for x in (qs, self.ks, self.vs)]
+        self.batch = fa.HipPagedBatch(hip, i32(hip, self.table), i32(hip, self.ctx), n,
+                                      self.table.shape[1], page, self.pages)
+        self.len_buf = i32(hip, self.lens)
+        self.lay = self.batch.layout(most, hq, D, dtype)
+        self.out = fa.DeviceBuffer(hip, self.lay.combined_bytes)
+
+    def rows(self, s, count):
+        at = np.arange(count)
+        return self.table[s, at // self.page].astype(np.int64) * self.page + at % self.page
+
+    def upload(self):
+        for buf, x in zip(self.bufs[1:], (self.ks, self.vs)):
+            buf.upload(x)
+
+    def call(self):
+        hq, hkv, D = self.dims
+        m = None if self.masks is None else fa.DeviceBuffer.from_array(self.hip, self.masks)
+        p = None if self.pos is None else i32(self.hip, self.pos)
+        self.keep = (m, p)
+        self.batch.tree_attention(
+            *self.bufs, self.out, self.len_buf, self.most, hq, hkv, D,
+            fa.FlatAttentionConfig(True, self.scale),
+            fa.RotaryEmbeddingConfig(THETA, self.offset) if self.rope else None, self.dtype,
+            positions=p, masks=m)
+
+    def get(self):
+        hq, hkv, D = self.dims
+        n = len(self.ctx)
+        r = fa.download_attention(self.out, self.lay, self.dtype)
+        o = fa.storage_to_f32(r.output, self.dtype).reshape(n, self.most, hq, D)
+        return o, r.lse.reshape(n, hq, self.most)
+
+    def run(self):
+        self.out.fill_u32(0x7fc07fc0)
+        self.call()
+        return self.get()
+
+    def check(self, only=None):
+        """Every row (or those of sequences `only`) against float64."""
+        o, lse = self.run()
+        hq, hkv, D = self.dims
+        scale = self.scale if self.scale is not None else float(np.float32(1) / np.sqrt(np.float32(D)))
+        h = HALF_STEP[self.dtype]
+        for s in range(len(self.ctx)) if only is None else only:
+            c, m = int(self.ctx[s]), int(self.lens[s])
+            ok = c >= 0 and 0 <= m <= self.most and c + m <= self.table.shape[1] * self.page
+            m = m if ok else 0
+            sees = np.ones((m, c + m if ok else 0), bool)
+            if ok:
+                sees[:, c:] = self.sees[s, :m, :m]
+            at = self.rows(s, c + m if ok else 0)
+            q = self.q[s, :m]
+            if self.rope:
+                q = model.rotate(q, self.where[s, :m] + self.offset, THETA)
+                sees = sees & (self.where[s, :m] >= 0)[:, None]
+            eo, el, av, size = model.attend(q, self.k[at], self.v[at], sees, scale)
+            n = sees.shape[1]
+            assert (o[s, m:] == 0).all() and (lse[s, :, m:] == -np.inf).all()
+            ds = size * ((D + 16) * 2.0 ** -24 + (h * h if self.dtype != F32 and self.rope else 0))
+            empty = el == -np.inf
+            assert np.array_equal(np.isneginf(lse[s, :, :m]), empty), s
+            assert (o[s, :m][empty.T] == 0).all()
+            tl = ds + n * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -22 * (np.abs(np.where(empty, 0, el)) + size)
+            err = np.abs(np.where(empty, 0, lse[s, :, :m] - np.where(empty, 0, el)))
+            assert (err <= tl).all(), (s, (err / tl).max())
+            to = h * (np.abs(eo) + av) + (2 * ds.T[..., None] + n * 2.0 ** -23 + 2.0 ** -19) * av
+            if self.dtype == F16:
+                to = to + 2.0 ** -25
+            err = np.abs(o[s, :m] - eo)
+            assert (err <= to).all(), (s, (err / np.maximum(to, 1e-30)).max())
+        return o, lse
+
+
+SHAPES = [  # context lengths, tree lengths, most, q heads, kv heads, head dim, page
+    ([0], [1], 1, 1, 1, 64, 16),
+    ([1], [1], 1, 4, 1, 128, 16),
+    ([63, 0, 5], [3, 5, 0], 5, 4, 2, 64, 16),
+    ([200, 17, 64], [7, 16, 1], 16, 8, 2, 128, 16),
+    ([31, 32, 33, 96], [33, 31, 1, 32], 33, 4, 4, 64, 5),
+    ([1000, 3, 257], [13, 2, 9], 13, 6, 2, 128, 24),
+    ([513, 90], [64, 40], 64, 16, 2, 128, 16),
+    ([129], [70], 70, 3, 1, 40, 1),
+    ([700, 129], [130, 65], 130, 2, 1, 96, 32),
+    ([40], [512], 512, 2, 2, 32, 16),
+    ([2500, 11], [4, 4], 4, 12, 12, 80, 64),
+    ([300, 150, 1], [3, 2, 3], 3, 40, 1, 64, 8),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+@pytest.mark.parametrize("tree,rope", [(True, True), (False, True), (True, False)])
+def test_tree_attention_matches_float64(hip, dtype, shape, tree, rope):
+    ctx, lens, most, hq, hkv, D, page = SHAPES[shape]
+    Case(hip, dtype, ctx, lens, most, hq, hkv, D, page, 100 + shape, tree, rope,
+         offset=37 if shape % 2 else 0, scale=0.2 if shape % 3 == 0 else None).check()
