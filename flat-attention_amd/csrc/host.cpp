@@ -3499,6 +3499,9 @@ int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q,
     const uint64_t n = b->n_seqs, words = (max_tokens + 63) / 64;
     if (q_heads > kI32 || n * max_tokens > kI32 || mul_ov(n * max_tokens, q_heads, &lse) || lse > kI32)
         return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "drafted tokens exceed the i32 index space");
+    // steps of 32 keys or more of every (sequence, kv head), counted in 32 bits
+    if (mul_ov(n * kv_heads, capacity / 32 + 1, &elements) || elements > kI32)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the i32 index space");
     elements = lse * head_dim;
     fa_packed_layout lay;
     if (int rc = fa_packed_layout_for(elements, lse, dtype, &lay)) return rc;
@@ -3529,7 +3532,7 @@ int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q,
     a.tree_lens = tree_lens;
     a.positions = positions;
     a.masks = masks;
-    a.rope_positions = (int64_t)capacity;
+    a.rope_positions = (int)capacity;
     a.rope_offset = rot ? (int)rot->position_offset : 0;
     a.n_seqs = (int)n;
     a.max_tokens = (int)max_tokens;
@@ -3542,12 +3545,25 @@ int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q,
     a.page_size = (int)b->page_size;
     a.physical_pages = (int)b->physical_pages;
     a.scale = scale;
-    unsigned grid[3], block, dispatches;
+    size_t ml_offset, plan_offset;
+    const size_t bytes = fa::tree_workspace((Dtype)dtype, a, &ml_offset, &plan_offset);
+    void* ws = nullptr;
+    if (int rc = grow(ctx, &ctx->ws_tree, &ctx->ws_tree_bytes, bytes, &ws)) return rc;
+    a.part_o = (float*)ws;
+    a.part_ml = (float2*)((uint8_t*)ws + ml_offset);
+    a.plan = (int*)((uint8_t*)ws + plan_offset);
+    unsigned grid[3], block, q_rows;
     begin_span(ctx);
-    fa::launch_tree_attention((Dtype)dtype, a, ctx->stream, grid, &block, &dispatches);
-    end_span(ctx, FA_KERNEL_TREE_ATTENTION);
+    fa::launch_tree_attention((Dtype)dtype, a, ctx->stream, grid, &block, &q_rows,
+                              [](void* c) {
+                                  end_span((fa_ctx*)c, FA_KERNEL_TREE_ATTENTION);
+                                  begin_span((fa_ctx*)c);
+                              },
+                              ctx);
+    end_span(ctx, FA_KERNEL_TREE_COMBINE);
     HIP_TRY(hipGetLastError());
-    record(ctx, FA_KERNEL_TREE_ATTENTION, "tree_rows", 1, 64, grid, block, dispatches, 1, nullptr);
+    record(ctx, FA_KERNEL_TREE_ATTENTION, "tree_split + tree_combine", q_rows, 32, grid, block, 2, 1,
+           nullptr);
     return ok();
 }
 

@@ -394,13 +394,23 @@ struct TreeArgs {
     const int* positions;    // [n_seqs, max_tokens], null: ctx_lens + token
     const uint64_t* masks;   // [n_seqs, max_tokens, words], null: token t sees drafted ones 0..t
     const float2* rope_table;  // null: Q as it is
-    int64_t rope_positions;    // positions the table has behind rope_offset
+    int rope_positions;        // positions the table has behind rope_offset
     int rope_offset;
     int n_seqs, max_tokens, words, q_heads, kv_heads, group, head_dim;
     int max_pages, page_size, physical_pages;
     float scale;
+    // Scratch (tree_workspace): partial O and (m, l) of the units that several key ranges share, and
+    // the plan that the split kernel leaves for the combine: each sequence's first step, the number of
+    // all steps and those of a range.
+    float* part_o;
+    float2* part_ml;
+    int* plan;
 };
+// Bytes of the scratch of a launch of `a` and where part_ml and plan begin in it.
+size_t tree_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset);
+// Split kernel and combine; `between(user)` (if set) runs on the host between the launches. *rows: query
+// rows of a workgroup.
 void launch_tree_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned grid[3],
-                           unsigned* block, unsigned* dispatches);
+                           unsigned* block, unsigned* rows, void (*between)(void*), void* user);
 
 }  // namespace fa

@@ -16,102 +16,735 @@
 
 namespace fa {
 
-template <typename T>
-__device__ __forceinline__ float element(const void* p, int64_t i) {
-    if constexpr (std::is_same<T, float>::value) return ((const float*)p)[i];
-    else return Half<T>::lo(((const uint16_t*)p)[i]);
-}
-template <typename T>
-__device__ __forceinline__ void put(void* p, int64_t i, float x) {
-    if constexpr (std::is_same<T, float>::value) ((float*)p)[i] = x;
-    else ((uint16_t*)p)[i] = (uint16_t)Half<T>::pack(x, 0.0f);
+// Rows of one (sequence, kv head) are flattened as row = t * group + head, so every K/V byte read
+// serves all of them. A workgroup holds 32 RW rows; its waves are RW row blocks times KW key groups.
+// Per 32 keys and wave, the products transposed so that a lane owns one query row:
+//   S^T[32 keys x 32 rows] = K . Q^T     K from LDS (A operand), Q in registers (B)
+//   P^T = exp2((S - m) scale log2 e)     one lane exchange (lane ^ 32) for the row maximum
+//   O^T[dims x 32 rows]   += V^T . P^T   V read transposed from LDS; the S^T accumulator is the P^T
+//                                        operand as it stands, V's keys are taken in its order
+// K and V rows go straight from memory into LDS, 16 bytes a lane, two stages; the LDS column of a piece
+// is XORed with its row so that both operand reads are free of bank conflicts without padding. Rows
+// that do not exist, and dims past head_dim, are fetched from 16 zero bytes.
+// 16-bit storage: the rotated Q is kept as a 16-bit high part and the rounding of its residual, two
+// MFMAs a step, so that scores and LSE carry f32 accuracy; P is rounded once to the storage type (its
+// sum is taken before), an error of the size of O's own rounding.
+//
+// The lengths are known on the GPU only, so the launch has a fixed number of workgroups; each finds its
+// share by a prefix sum over the sequences: the steps (KT keys) of all (sequence, kv head) units laid
+// end to end are cut into equal ranges. A unit that one range covers is finished there; the others
+// leave partial (O, m, l), at most two a workgroup, that tree_combine merges in their order.
+
+// Sixteen zero bytes: what rows and dims that do not exist are fetched from.
+__device__ __attribute__((aligned(16))) uint32_t tree_zero[4];
+
+constexpr int kTreePages = 1024;  // block-table entries held in LDS at a time
+
+template <typename T, int DPAD, int RW>
+struct TreeCfg {
+    static constexpr bool F32 = std::is_same<T, float>::value;
+    static constexpr int EB = F32 ? 4 : 2;
+    static constexpr int NW = RW == 8 ? 8 : F32 && RW < 4 ? 2 : 4;  // waves
+    static constexpr int KW = NW / RW;                              // key groups
+    static constexpr int BN = !F32 && RW == 8 ? 64 : 32;            // keys of a group's tile
+    static constexpr int KT = KW * BN;                              // keys of a step
+    static constexpr int ROWB = DPAD * EB;                          // bytes of an LDS row
+    static constexpr int CPR = ROWB / 16;                           // 16-byte pieces of it
+    static constexpr int TILE = BN * ROWB;
+    static constexpr int STAGE = 2 * TILE;  // K and V of a group
+    static constexpr int NST = F32 || RW < 4 ? 2 : 4;  // stages: NST - 1 tiles are on their way
+    static constexpr int SMEM_KV = KW * NST * STAGE;
+    static constexpr int MROW = DPAD * 4 + 16;  // row of the O exchange
+    static constexpr int SMEM_O = NW * 32 * MROW;
+    static constexpr int SMEM = SMEM_KV > SMEM_O ? SMEM_KV : SMEM_O;
+    static constexpr int ROWS = 32 * RW;
+    // transfer instructions (64 pieces each) of K (or V) a wave issues per tile
+    static constexpr int NI = BN * CPR / 64 / RW;
+    static constexpr int WAVES = (SMEM > 72 * 1024 && NW < 8) || (F32 && DPAD > 64) ? 1 : 2;  // per SIMD
+};
+
+// Which column a piece of an LDS row is kept in: piece ^ swizzle(row). 16 columns of 16 bytes are the 64
+// banks. K is read one row a lane (8 rows at a time have to lie in different columns), V with four rows
+// times four neighbouring pieces (16-bit) or eight pieces of two rows four apart (f32) at a time.
+template <int CPR, bool F32>
+__device__ __forceinline__ int swizzle(int row) {
+    if constexpr (F32) return (((row >> 2) & 1) << 3) | ((row & 3) << 1) | ((row >> 3) & 1);
+    else if constexpr (CPR == 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
-// One wave a row (sequence, token, head): a key per lane for the scores, two dims per lane for P.V.
-template <typename T>
-__global__ __launch_bounds__(64) void tree_rows(TreeArgs a, FastDiv ps) {
-    __shared__ float qv[128];
-    const int lane = threadIdx.x, D = a.head_dim;
-    const int hq = blockIdx.x % a.q_heads, r = blockIdx.x / a.q_heads;
-    const int s = r / a.max_tokens, t = r % a.max_tokens;
+__device__ __forceinline__ void global_to_lds16(const void* p, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(lds));
+}
+
+struct TreeKArgs {
+    TreeArgs a;
+    FastDiv ps, grp, ranges, row_blocks;
+};
+
+// Live rows of a sequence, drafted ones included; 0: it has no part in this call.
+__device__ __forceinline__ int tree_rows_of(const TreeArgs& a, int s) {
     const int ctx = a.ctx_lens[s], len = a.tree_lens[s];
-    bool live = ctx >= 0 && len >= 0 && len <= a.max_tokens && t < len &&
-                (int64_t)ctx + len <= (int64_t)a.max_pages * a.page_size;
-    int64_t pos = 0;
-    if (live && a.rope_table) {
-        pos = a.positions ? a.positions[r] : ctx + t;
-        live = pos >= 0 && pos < a.rope_positions;
-    }
-    const int64_t q0 = ((int64_t)r * a.q_heads + hq) * D;
-    if (live) {
-        for (int d = 2 * lane; d < D; d += 128) {
-            float e = element<T>(a.q, q0 + d), o = element<T>(a.q, q0 + d + 1);
-            if (a.rope_table) {
-                const float2 cs = a.rope_table[(pos + a.rope_offset) * (D / 2) + d / 2];
-                rope_pair(e, o, cs.x, cs.y);
+    const bool ok = ctx >= 0 && len > 0 && len <= a.max_tokens &&
+                    (int64_t)ctx + len <= (int64_t)a.max_pages * a.page_size;
+    return ok ? ctx + len : 0;
+}
+
+// Whether a word's values (one f32, two 16-bit) hold an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    if constexpr (std::is_same<T, float>::value) return (w & 0x7f800000u) == 0x7f800000u;
+    constexpr uint32_t e = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+    return (w & e) == e || (w & (e << 16)) == (e << 16);
+}
+
+// Wait for the result of a 32x32 MFMA, written out because branches come between the last product and
+// its readers (see wait_mfma).
+template <bool F32>
+__device__ __forceinline__ void wait_mfma32(f32x16_t& v) {
+    if constexpr (F32) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(v));
+    else asm volatile("s_nop 11" : "+v"(v));
+}
+
+// V operands of P.V from the stage: dims 32 mb + (lane & 31) of the keys that the lane's half of S^T
+// holds. 16-bit: eight keys, in S^T's order, transposed on the way; f32: the key of accumulator i.
+template <int DPAD>
+__device__ __forceinline__ u32x4_t tree_v16(const uint8_t* smem, int va0, int k2, int mb) {
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4s lds_v4s;
+    // column bits: mb in 6 and up (two rows share 256 bytes at 64 dims), e in 5
+    const int x0 = va0 ^ (mb << 6), x1 = va0 ^ (mb << 6) ^ (1 << 5);
+    const u32x2_t a = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                      (lds_v4s*)(smem + x0 + 16 * k2 * DPAD * 2)));
+    const u32x2_t b = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                      (lds_v4s*)(smem + x1 + (16 * k2 + 8) * DPAD * 2)));
+    return u32x4_t{a[0], a[1], b[0], b[1]};
+}
+template <int DPAD>
+__device__ __forceinline__ float tree_v32(const uint8_t* smem, int va0, int i, int mb) {
+    const int col = ((i & 3) << 1 | ((i >> 2) & 1)) << 4;  // swizzle of the row's part in i
+    return *(const float*)(smem + (va0 ^ (mb << 7) ^ col) + (8 * (i / 4) + i % 4) * DPAD * 4);
+}
+
+// P.V of a block whose V holds infinities or NaN, in which rows may not see every key: 0 * inf would
+// make NaN of what a row must not see. Those values are taken out of V, and for the rows that see them
+// +inf, -inf and NaN are counted by a product with the visibility and added.
+template <typename T, int DPAD>
+__device__ __forceinline__ void pv_special(const uint8_t* smem, int va0, const f32x16_t& p,
+                                           uint32_t see, f32x16_t* oacc) {
+    constexpr bool F32 = std::is_same<T, float>::value;
+#pragma unroll
+    for (int mb = 0; mb < DPAD / 32; ++mb) {
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {  // finite values, +inf, -inf, NaN
+            f32x16_t n;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) n[i] = 0.0f;
+            auto pick = [&](float v) {
+                const bool is = x == 1 ? v == INFINITY : x == 2 ? v == -INFINITY : v != v;
+                return x == 0 ? (fabsf(v) < INFINITY ? v : 0.0f) : is ? 1.0f : 0.0f;
+            };
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float seen = (see >> (8 * (i / 4) + i % 4)) & 1 ? 1.0f : 0.0f;
+                    n = __builtin_amdgcn_mfma_f32_32x32x2f32(pick(tree_v32<DPAD>(smem, va0, i, mb)),
+                                                             x ? seen : p[i], n, 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int k2 = 0; k2 < 2; ++k2) {
+                    const u32x4_t v = tree_v16<DPAD>(smem, va0, k2, mb);
+                    u32x4_t av, bv;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = 8 * k2 + 2 * j;
+                        const uint32_t w = see >> (8 * (i / 4) + i % 4);
+                        av[j] = Half<T>::pack(pick(Half<T>::lo(v[j])), pick(Half<T>::hi(v[j])));
+                        bv[j] = x ? Half<T>::pack(w & 1 ? 1.0f : 0.0f, w & 2 ? 1.0f : 0.0f)
+                                  : Half<T>::pack(p[i], p[i + 1]);
+                    }
+                    n = Half<T>::mfma32(av, bv, n);
+                }
             }
-            qv[d] = e;
-            qv[d + 1] = o;
+            wait_mfma32<F32>(n);
+            const float special = x == 1 ? INFINITY : x == 2 ? -INFINITY : NAN;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) oacc[mb][i] += x == 0 ? n[i] : n[i] > 0.0f ? special : 0.0f;
         }
     }
+}
+
+// Four dims of a finished row: O / l and, with the first dims, LSE. A row without a key: 0 and -inf.
+template <typename T>
+__device__ __forceinline__ void write_row4(const TreeArgs& a, int s, int kvh, int row, int d, f32x4_t o,
+                                           float m, float l, const FastDiv& grp) {
+    const int t = (int)grp.div((uint32_t)row), hq = kvh * a.group + row - t * a.group;
+    const bool none = m == -INFINITY;  // (NaN and +inf maxima go the usual way)
+    const float inv = none ? 0.0f : 1.0f / l;
+    const int64_t at = (((int64_t)s * a.max_tokens + t) * a.q_heads + hq) * a.head_dim + d;
+    if (none) o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if constexpr (std::is_same<T, float>::value)
+        *(f32x4_t*)((float*)a.o + at) = o * inv;
+    else
+        *(u32x2_t*)((uint16_t*)a.o + at) = u32x2_t{Half<T>::pack(o[0] * inv, o[1] * inv),
+                                                   Half<T>::pack(o[2] * inv, o[3] * inv)};
+    if (d == 0)
+        a.lse[((int64_t)s * a.q_heads + hq) * a.max_tokens + t] =
+            none ? -INFINITY : m * a.scale + logf(l);
+}
+
+template <typename T, int DPAD, int RW, bool SPLIT>
+__global__ __launch_bounds__((64 * TreeCfg<T, DPAD, RW>::NW),
+                             (TreeCfg<T, DPAD, RW>::WAVES))
+void tree_split(TreeKArgs ka) {
+    using C = TreeCfg<T, DPAD, RW>;
+    constexpr bool F32 = C::F32;
+    constexpr int MB = DPAD / 32;                   // 32-dim blocks of O^T
+    constexpr int KS = F32 ? DPAD / 8 : DPAD / 16;  // K pieces a lane reads per 32 keys
+    constexpr int NT = 64 * C::NW;
+    constexpr int E = 16 / C::EB;                   // elements of a piece
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[C::SMEM];
+    __shared__ int bt_lds[kTreePages];
+    __shared__ int scan_lds[C::NW + 2];
+    __shared__ float2 ml_lds[C::NW * 32];
+    const TreeArgs& a = ka.a;
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rw = wave % RW, kg = wave / RW;
+    const int D = a.head_dim;
+    const int logical = xcd_remap(blockIdx.x, gridDim.x);
+    const int range = __builtin_amdgcn_readfirstlane((int)ka.row_blocks.div((uint32_t)logical));
+    const int rb = logical - range * (int)ka.row_blocks.d;
+
+    // ---- this workgroup's range of steps [pos, end), and the sequence that holds the first
+    auto steps_of = [&](int i) {
+        return i < a.n_seqs ? a.kv_heads * ((tree_rows_of(a, i) + C::KT - 1) / C::KT) : 0;
+    };
+    auto scan = [&](int v, int* sum) {  // inclusive over the workgroup
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(v, o, 64);
+            if (lane >= o) v += up;
+        }
+        __syncthreads();
+        if (lane == 63) scan_lds[wave] = v;
+        __syncthreads();
+        int all = 0, before = 0;
+#pragma unroll
+        for (int w = 0; w < C::NW; ++w) {
+            if (w == wave) before = all;
+            all += scan_lds[w];
+        }
+        *sum = all;
+        return v + before;
+    };
+    int sum0, total;
+    int mine = steps_of(tid);
+    int upto = scan(mine, &sum0);
+    total = sum0;
+    for (int base = NT; base < a.n_seqs; base += NT) {
+        int sum;
+        scan(steps_of(base + tid), &sum);
+        total += sum;
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    const int share = max(1, (int)ka.ranges.div((uint32_t)total + ka.ranges.d - 1));
+    int64_t pos = (int64_t)range * share;
+    const int64_t end = pos + share < total ? pos + share : total;
+    const bool plans = logical == 0;  // writes what tree_combine needs
+    if (pos >= end && !plans) return;
+    for (int base = 0, carry = 0; base < a.n_seqs; base += NT) {
+        int sum = sum0;
+        if (base > 0) {
+            mine = steps_of(base + tid);
+            upto = scan(mine, &sum);
+        }
+        if (plans && base + tid < a.n_seqs) a.plan[base + tid] = carry + upto - mine;
+        if (mine > 0 && carry + upto - mine <= pos && pos < carry + upto) {
+            scan_lds[C::NW] = base + tid;
+            scan_lds[C::NW + 1] = carry + upto - mine;
+        }
+        carry += sum;
+    }
+    if (plans && tid == 0) {
+        a.plan[a.n_seqs] = total;
+        a.plan[a.n_seqs + 1] = share;
+    }
+    if (pos >= end) return;
     __syncthreads();
-    float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    const int n = live ? ctx + len : 0;
-    const int64_t width = (int64_t)a.kv_heads * D, head = (int64_t)(hq / a.group) * D;
-    for (int base = 0; base < n; base += 64) {
-        const int key = base + lane, j = key - ctx;
-        bool seen = key < n;
-        int64_t row = -1;
-        if (seen && j >= 0)
-            seen = a.masks ? (a.masks[(int64_t)r * a.words + (j >> 6)] >> (j & 63)) & 1 : j <= t;
-        if (seen) {
-            const int lp = (int)ps.div((uint32_t)key);
-            const int page = a.block_tables[(int64_t)s * a.max_pages + lp];
-            if ((unsigned)page < (unsigned)a.physical_pages)
-                row = (int64_t)page * a.page_size + (key - lp * a.page_size);
+    int s = __builtin_amdgcn_readfirstlane(scan_lds[C::NW]);
+    int first = __builtin_amdgcn_readfirstlane(scan_lds[C::NW + 1]);  // first step of sequence s
+
+    // ---- lane constants
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)smem;
+    const int group_base = kg * C::NST * C::STAGE;
+    const int n16 = lane & 15;
+    // K operand: row lane & 31, piece 2 c + h: the column's XOR takes c by itself
+    const int kbase = group_base + (lane & 31) * C::ROWB +
+                      ((h ^ swizzle<C::CPR, F32>(lane & 31)) << 4);
+    // V operand. 16-bit: rows 16 k2 + 8 e + 4 h + (n16 >> 2), pieces 4 mb + 2 (lane >> 4 & 1) +
+    // ((n16 & 3) >> 1); e and mb enter the column by XOR. f32: row 8 (i / 4) + 4 h + i % 4, piece
+    // 8 mb + (lane & 31) / 4.
+    int vbase;
+    if constexpr (F32) {
+        vbase = group_base + C::TILE + 4 * h * C::ROWB + ((((lane & 31) >> 2) ^ (h << 3)) << 4) +
+                4 * (lane & 3);
+    } else {
+        const int r = 4 * h + (n16 >> 2), p = 2 * ((lane >> 4) & 1) + ((n16 & 3) >> 1);
+        vbase = group_base + C::TILE + r * C::ROWB + ((p ^ swizzle<C::CPR, F32>(r)) << 4) +
+                8 * (n16 & 1);
+    }
+    const int64_t row_bytes = (int64_t)a.kv_heads * D * C::EB;
+    const float c2 = a.scale * kLog2e;
+    const int page_size = a.page_size;
+
+    while (pos < end) {
+        // ---- the unit that holds step pos and this range's part of it
+        int rows_s = 0, steps = 0;
+        for (;; ++s) {
+            rows_s = __builtin_amdgcn_readfirstlane(tree_rows_of(a, s));
+            steps = (rows_s + C::KT - 1) / C::KT;
+            if (pos < (int64_t)first + (int64_t)steps * a.kv_heads) break;
+            first += steps * a.kv_heads;
         }
-        float sc = -INFINITY;
-        if (row >= 0) {
-            float x = 0.0f;
-            for (int d = 0; d < D; ++d) x = fmaf(qv[d], element<T>(a.k_pool, row * width + head + d), x);
-            sc = x * a.scale;
+        const int in_seq = (int)(pos - first);
+        const int kvh = __builtin_amdgcn_readfirstlane(in_seq / steps);
+        const int st0 = in_seq - kvh * steps;
+        const int st1 = (int)min((int64_t)steps, st0 + (end - pos));
+        pos += st1 - st0;
+        const int len = __builtin_amdgcn_readfirstlane(a.tree_lens[s]);
+        const int ctx = rows_s - len;
+        const int rows_total = len * a.group, r0 = rb * C::ROWS;
+        if (r0 >= rows_total) continue;
+
+        // ---- this lane's query row
+        const int row = r0 + rw * 32 + (lane & 31);
+        const int t = (int)ka.grp.div((uint32_t)row), hq = kvh * a.group + row - t * a.group;
+        bool row_ok = row < rows_total;
+        const int tok = s * a.max_tokens + t;
+        int rope_pos = 0;
+        if (row_ok && a.rope_table) {
+            rope_pos = a.positions ? a.positions[tok] : ctx + t;
+            row_ok = rope_pos >= 0 && rope_pos < a.rope_positions;
         }
-        float mt = sc;
-        for (int k = 32; k; k >>= 1) mt = fmaxf(mt, shfl_xor(mt, k));
-        if (mt == -INFINITY) continue;
-        const float mn = fmaxf(m, mt), keep = fast_exp2((m - mn) * kLog2e);
-        const float p = fast_exp2((sc - mn) * kLog2e);
-        m = mn;
-        l = l * keep + p;
-        o0 *= keep;
-        o1 *= keep;
-        for (int k = 0; k < 64; ++k) {
-            const float pk = __shfl(p, k, 64);
-            const int64_t rk = __shfl((long long)row, k, 64);
-            if (pk == 0.0f) continue;
-            if (lane < D) o0 = fmaf(pk, element<T>(a.v_pool, rk * width + head + lane), o0);
-            if (lane + 64 < D) o1 = fmaf(pk, element<T>(a.v_pool, rk * width + head + lane + 64), o1);
+        u32x4_t qop[KS], qlo[SPLIT ? KS : 1];
+        auto load_q = [&]() {
+            int hh = h;
+            asm volatile("" : "+v"(hh));  // (no address is kept past this)
+            const uint8_t* const qrow = (const uint8_t*)a.q + ((int64_t)tok * a.q_heads + hq) * (D * C::EB);
+            const float2* const cs = a.rope_table + (int64_t)(rope_pos + a.rope_offset) * (D >> 1);
+#pragma unroll
+            for (int c = 0; c < KS; ++c) {
+                // (four pieces and their angles at a time: all of them do not fit the registers)
+                if (c % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                const int d0 = (2 * c + hh) * E;
+                qop[c] = u32x4_t{0u, 0u, 0u, 0u};
+                if constexpr (SPLIT) qlo[c] = u32x4_t{0u, 0u, 0u, 0u};
+                if (!row_ok || d0 >= D) continue;
+                u32x4_t raw = *(const u32x4_t*)(qrow + d0 * C::EB);
+                if constexpr (F32) {
+                    if (a.rope_table) {
+                        const f32x4_t w = *(const f32x4_t*)(cs + d0 / 2);
+                        float x[4] = {__uint_as_float(raw[0]), __uint_as_float(raw[1]),
+                                      __uint_as_float(raw[2]), __uint_as_float(raw[3])};
+                        rope_pair(x[0], x[1], w[0], w[1]);
+                        rope_pair(x[2], x[3], w[2], w[3]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) raw[j] = __float_as_uint(x[j]);
+                    }
+                } else if constexpr (SPLIT) {
+                    const f32x4_t w0 = *(const f32x4_t*)(cs + d0 / 2);
+                    const f32x4_t w1 = *(const f32x4_t*)(cs + d0 / 2 + 2);
+                    const float c8[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[2 * j] = Half<T>::lo(raw[j]);
+                        x[2 * j + 1] = Half<T>::hi(raw[j]);
+                    }
+                    rope4(x, c8);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        raw[j] = Half<T>::pack(x[2 * j], x[2 * j + 1]);
+                        qlo[c][j] = Half<T>::pack(x[2 * j] - Half<T>::lo(raw[j]),
+                                                  x[2 * j + 1] - Half<T>::hi(raw[j]));
+                    }
+                }
+                qop[c] = raw;
+            }
+        };
+
+        f32x16_t oacc[MB];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) oacc[mb][i] = 0.0f;
+        float m_run = -INFINITY, l_run = 0.0f;
+        const uint8_t* const kpool = (const uint8_t*)a.k_pool + (int64_t)kvh * D * C::EB;
+        const uint8_t* const vpool = (const uint8_t*)a.v_pool + (int64_t)kvh * D * C::EB;
+        const int* const table = a.block_tables + (int64_t)s * a.max_pages;
+
+        for (int c0 = st0; c0 < st1;) {
+            // ---- table entries of as many steps as they cover: first pool row of each page, -1 where
+            // the id lies outside the pool
+            const int p0 = (int)ka.ps.div((uint32_t)c0 * C::KT);
+            const int64_t reach = ((int64_t)p0 + kTreePages) * page_size;  // keys below are covered
+            const int c1 = (int)min((int64_t)st1, max((int64_t)c0 + 1, reach / C::KT));
+            const int k_end = min(c1 * C::KT, rows_s);
+            const int n_pages = (int)ka.ps.div((uint32_t)k_end - 1) - p0 + 1;
+            bool bad = false;
+            __syncthreads();  // (the stages and entries before have been read)
+            for (int i = tid; i < n_pages; i += NT) {
+                const int page = table[p0 + i];
+                const bool in = (unsigned)page < (unsigned)a.physical_pages;
+                bt_lds[i] = in ? page * page_size : -1;
+                bad |= !in;
+            }
+            // (a vote of its own: __syncthreads_or goes by the block's three dimensions, registers that
+            // are missed later)
+            bad = __any(bad);
+            if (lane == 0) scan_lds[wave] = bad;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < C::NW; ++w) bad |= scan_lds[w] != 0;
+            bad = __builtin_amdgcn_readfirstlane(bad);
+
+            // ---- one tile of this wave's key group into a stage
+            auto transfer = [&](int step, int stage) {
+                const int tile = step * C::KT + kg * C::BN;
+                if (tile >= k_end) return;
+                int ln = lane;
+                asm volatile("" : "+v"(ln));  // (what depends on the lane alone is not kept)
+                constexpr int RPI = 64 / C::CPR;  // rows of an instruction
+                const int r1 = ln / C::CPR, col = ln % C::CPR;
+#pragma unroll
+                for (int i = 0; i < C::NI; ++i) {
+                    const int r = (rw * C::NI + i) * RPI + r1;
+                    const int piece = col ^ swizzle<C::CPR, F32>(r);
+                    const int key = tile + r;
+                    const uint8_t *kp = (const uint8_t*)tree_zero, *vp = (const uint8_t*)tree_zero;
+                    if (key < k_end && piece * E < D) {
+                        const int lp = (int)ka.ps.div((uint32_t)key);
+                        const int base = bt_lds[lp - p0];
+                        if (base >= 0) {
+                            const int64_t off =
+                                (int64_t)(base + key - lp * page_size) * row_bytes + piece * 16;
+                            kp = kpool + off;
+                            vp = vpool + off;
+                        }
+                    }
+                    const uint32_t dst = lds0 + group_base + stage + (rw * C::NI + i) * 1024;
+                    global_to_lds16(kp, dst);
+                    global_to_lds16(vp, dst + C::TILE);
+                }
+            };
+
+            // ---- 32 keys from `key0` at `at` of a stage: scores, softmax, P.V
+            auto block = [&](int key0, int at) {
+                f32x16_t sc;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+                const int ka0 = kbase + at;
+#pragma unroll
+                for (int c = 0; c < KS; ++c) {
+                    const u32x4_t kv = *(const u32x4_t*)(smem + (ka0 ^ (c << 5)));
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            sc = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                                __uint_as_float(kv[j]), __uint_as_float(qop[c][j]), sc, 0, 0, 0);
+                    } else {
+                        sc = Half<T>::mfma32(kv, qop[c], sc);
+                        if constexpr (SPLIT) sc = Half<T>::mfma32(kv, qlo[c], sc);
+                    }
+                }
+                wait_mfma32<F32>(sc);
+                // Blocks in which some row may not see some key.
+                uint32_t see = 0xffffffffu;  // bit k: this row sees key0 + k
+                bool odd_v = false;          // V holds infinities or NaN there
+                if (key0 + 32 > ctx || bad) {
+                    const int j0 = key0 - ctx;  // drafted token of the first key
+                    uint64_t w;
+                    if (a.masks) {
+                        const uint64_t* const m = a.masks + (int64_t)tok * a.words;
+                        const int at64 = j0 >= 0 ? j0 >> 6 : 0, sh = j0 & 63;
+                        const uint64_t w0 = row_ok && at64 < a.words ? m[at64] : 0;
+                        const uint64_t w1 = row_ok && j0 >= 0 && at64 + 1 < a.words ? m[at64 + 1] : 0;
+                        if (j0 >= 0) w = (w0 >> sh) | (sh ? w1 << (64 - sh) : 0);
+                        else if (j0 > -32) w = w0 << -j0 | ((1u << -j0) - 1u);
+                        else w = 0xffffffffu;
+                    } else {
+                        const int last = t - j0;  // keys 0..last
+                        w = last >= 31 ? 0xffffffffu : last >= 0 ? (2u << last) - 1u : 0u;
+                    }
+                    // keys past the live rows, and on pages that are not there
+                    const int left = k_end - key0;
+                    uint32_t live = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+                    if (bad) {
+                        const int key = min(key0 + (lane & 31), k_end - 1);
+                        const int lp = (int)ka.ps.div((uint32_t)key);
+                        live &= (uint32_t)__ballot(bt_lds[lp - p0] >= 0);
+                    }
+                    see = (uint32_t)w & live;
+                    const uint32_t mine = see >> (4 * h);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!((mine >> (8 * (i / 4) + i % 4)) & 1)) sc[i] = -INFINITY;
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int i = 0; i < 32 * C::ROWB / 1024; ++i) {
+                        const u32x4_t v =
+                            *(const u32x4_t*)(smem + group_base + C::TILE + at + i * 1024 + lane * 16);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) any |= not_finite<T>(v[j]);
+                    }
+                    odd_v = __any(any != 0);
+                }
+                float mt = sc[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) mt = fmaxf(mt, sc[i]);
+                mt = fmaxf(mt, xor32(mt));
+                // the running maximum only moves when a block's exceeds it by more than 2^8 in
+                // probability, so O is rarely rescaled
+                const bool need = mt * c2 > m_run * c2 + 8.0f;
+                if (__any(need)) {
+                    const float m_use = need ? mt : m_run;
+                    const float alpha = m_run == m_use ? 1.0f : fast_exp2((m_run - m_use) * c2);
+                    l_run *= alpha;
+#pragma unroll
+                    for (int mb = 0; mb < MB; ++mb) oacc[mb] *= alpha;
+                    m_run = m_use;
+                }
+                const float neg = m_run == -INFINITY ? 0.0f : -m_run * c2;  // (no key seen yet)
+                float ls = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sc[i] = fast_exp2(fmaf(sc[i], c2, neg));
+                    ls += sc[i];
+                }
+                l_run += ls;
+                const int va0 = vbase + at;
+                if (__builtin_expect(odd_v, 0)) {
+                    pv_special<T, DPAD>(smem, va0, sc, see >> (4 * h), oacc);
+                } else if constexpr (F32) {
+#pragma unroll
+                    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            oacc[mb] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                                tree_v32<DPAD>(smem, va0, i, mb), sc[i], oacc[mb], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; ++k2) {
+                        u32x4_t pb;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            pb[j] = Half<T>::pack(sc[8 * k2 + 2 * j], sc[8 * k2 + 2 * j + 1]);
+#pragma unroll
+                        for (int mb = 0; mb < MB; ++mb)
+                            oacc[mb] = Half<T>::mfma32(tree_v16<DPAD>(smem, va0, k2, mb), pb, oacc[mb]);
+                    }
+                }
+            };
+
+            // ---- the steps, NST - 1 transfers ahead
+#pragma unroll
+            for (int i = 0; i < C::NST - 1; ++i)
+                if (c0 + i < c1) transfer(c0 + i, i * C::STAGE);
+            if (c0 == st0) load_q();
+            int stage = 0;
+            for (int step = c0; step < c1; ++step) {
+                // (transfers complete in order: those of the NST - 2 tiles behind this one may be on
+                // their way; near the end there are fewer)
+                if (C::NST > 2 && step + C::NST - 2 < c1 - 1) wait_vmcnt<(C::NST - 2) * 2 * C::NI>();
+                else wait_dma();
+                if constexpr (RW > 1) __syncthreads();
+                else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                const int ahead = stage == 0 ? (C::NST - 1) * C::STAGE : stage - C::STAGE;
+                if (step + C::NST - 1 < c1) transfer(step + C::NST - 1, ahead);
+                const int tile = step * C::KT + kg * C::BN;
+#pragma unroll 1
+                for (int kb = 0; kb < C::BN; kb += 32)
+                    if (tile + kb < k_end) block(tile + kb, stage + kb * C::ROWB);
+                stage = stage == (C::NST - 1) * C::STAGE ? 0 : stage + C::STAGE;
+            }
+            c0 = c1;
+        }
+
+        // ---- merge the key groups in LDS and write the rows
+        l_run += xor32(l_run);
+        int te = tid;
+        asm volatile("" : "+v"(te));  // (no address is kept from unit to unit)
+        const int le = te & 63, he = le >> 5;
+        if (he == 0) ml_lds[wave * 32 + (le & 31)] = make_float2(m_run, l_run);
+        __syncthreads();  // (every stage has been read)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(f32x4_t*)(smem + (wave * 32 + (le & 31)) * C::MROW + (32 * mb + 8 * i + 4 * he) * 4) =
+                    f32x4_t{oacc[mb][4 * i], oacc[mb][4 * i + 1], oacc[mb][4 * i + 2], oacc[mb][4 * i + 3]};
+        __syncthreads();
+        const bool whole = st0 == 0 && st1 == steps;
+        const int64_t slot = 2 * ((int64_t)range * ka.row_blocks.d + rb) + (st0 == 0 ? 1 : 0);
+        constexpr int LPR = DPAD / 4;  // threads a row, four dims each
+        for (int i = te; i < C::ROWS * LPR; i += NT) {
+            const int r = i / LPR, d = 4 * (i % LPR);
+            if (r0 + r >= rows_total || d >= D) continue;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int g = 0; g < C::KW; ++g) M = fmaxf(M, ml_lds[g * C::ROWS + r].x);
+            f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < C::KW; ++g) {
+                const float2 ml = ml_lds[g * C::ROWS + r];
+                const float w = ml.x == -INFINITY ? 0.0f : fast_exp2((ml.x - M) * c2);
+                if (ml.x == -INFINITY) continue;  // (saw nothing: O = 0, l = 0)
+                const f32x4_t x = *(const f32x4_t*)(smem + (g * C::ROWS + r) * C::MROW + 4 * d);
+                L = fmaf(ml.y, w, L);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], w, o[j]);
+            }
+            if (!whole) {
+                *(f32x4_t*)(a.part_o + (slot * C::ROWS + r) * D + d) = o;
+                if (d == 0) a.part_ml[slot * C::ROWS + r] = make_float2(M, L);
+                continue;
+            }
+            write_row4<T>(a, s, kvh, r0 + r, d, o, M, L, ka.grp);
         }
     }
-    for (int k = 32; k; k >>= 1) l += shfl_xor(l, k);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    if (lane < D) put<T>(a.o, q0 + lane, o0 * inv);
-    if (lane + 64 < D) put<T>(a.o, q0 + lane + 64, o1 * inv);
-    if (lane == 0) a.lse[((int64_t)s * a.q_heads + hq) * a.max_tokens + t] =
-        l > 0.0f ? m + logf(l) : -INFINITY;
+}
+
+// Merges the partials of the units that several ranges share, and writes the rows past each tree. A wave
+// takes 64 / LPR rows at a time, LPR lanes (four dims each) a row; the partials of a row in their order.
+template <typename T, int LPR>
+__global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rows_block) {
+    const TreeArgs& a = ka.a;
+    const int rows_seq = a.max_tokens * a.q_heads;
+    const int64_t i = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    const int s = (int)(i / rows_seq);
+    if (s >= a.n_seqs) return;
+    const int d = 4 * (threadIdx.x % LPR), D = a.head_dim;
+    const int in = (int)(i - (int64_t)s * rows_seq);
+    const int per = a.max_tokens * a.group;
+    const int kvh = in / per, row = in - kvh * per;
+    if (d >= D) return;
+    const int rows_s = tree_rows_of(a, s);
+    const int len = rows_s ? a.tree_lens[s] : 0;
+    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+    if (row >= len * a.group) {
+        write_row4<T>(a, s, kvh, row, d, zero, -INFINITY, 0.0f, ka.grp);
+        return;
+    }
+    const int share = a.plan[a.n_seqs + 1];
+    const int steps = (rows_s + kt - 1) / kt;
+    const uint32_t u0 = (uint32_t)a.plan[s] + (uint32_t)kvh * (uint32_t)steps;
+    const int g0 = (int)(u0 / (uint32_t)share), g1 = (int)((u0 + steps - 1) / (uint32_t)share);
+    if (g0 == g1) return;  // finished by the range that covers it
+    const int rb = row / rows_block, r = row - rb * rows_block;
+    const float c2 = a.scale * kLog2e;
+    float M = -INFINITY, L = 0.0f;
+    f32x4_t o = zero;
+    for (int g = g0; g <= g1; ++g) {
+        const int64_t slot = 2 * ((int64_t)g * ka.row_blocks.d + rb) + (g == g0 ? 1 : 0);
+        const float2 ml = a.part_ml[slot * rows_block + r];
+        const f32x4_t x = *(const f32x4_t*)(a.part_o + (slot * rows_block + r) * D + d);
+        if (ml.x == -INFINITY) continue;
+        const float mx = fmaxf(M, ml.x);
+        const float w0 = M == -INFINITY ? 0.0f : fast_exp2((M - mx) * c2);
+        const float w1 = fast_exp2((ml.x - mx) * c2);
+        M = mx;
+        L = fmaf(ml.y, w1, L * w0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], w1, o[j] * w0);
+    }
+    write_row4<T>(a, s, kvh, row, d, o, M, L, ka.grp);
+}
+
+// Rows of a workgroup: as few row blocks of 32 as hold every row of a (sequence, kv head), at most 4;
+// the waves left over are key groups.
+static int tree_row_waves(Dtype dt, const TreeArgs& a) {
+    const int rows = a.max_tokens * a.group;
+    return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || dt == Dtype::F32 ? 4 : 8;
+}
+
+// Key ranges of the launch: one round of workgroups, one or (64 to 128 rows) two a CU.
+static void tree_shape(Dtype dt, const TreeArgs& a, int* ranges, int* row_blocks) {
+    const int rw = tree_row_waves(dt, a), rows = 32 * rw;
+    *row_blocks = (a.max_tokens * a.group + rows - 1) / rows;
+    *ranges = std::max(1, (rw == 2 || rw == 4 ? 2 : 1) * device_cus() / *row_blocks);
+}
+
+size_t tree_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset) {
+    int ranges, row_blocks;
+    tree_shape(dt, a, &ranges, &row_blocks);
+    const size_t rows = (size_t)2 * ranges * row_blocks * 32 * tree_row_waves(dt, a);
+    *ml_offset = rows * a.head_dim * 4;
+    *plan_offset = *ml_offset + rows * 8;
+    return *plan_offset + ((size_t)a.n_seqs + 2) * 4;
+}
+
+template <typename T, int DPAD, int RW>
+static void launch_rw(const TreeKArgs& ka, hipStream_t s, unsigned wgs) {
+    using C = TreeCfg<T, DPAD, RW>;
+    if constexpr (!C::F32) {
+        if (ka.a.rope_table) {
+            tree_split<T, DPAD, RW, true><<<wgs, 64 * C::NW, 0, s>>>(ka);
+            return;
+        }
+    }
+    tree_split<T, DPAD, RW, false><<<wgs, 64 * C::NW, 0, s>>>(ka);
+}
+
+template <typename T, int DPAD>
+static void launch_t(const TreeKArgs& ka, hipStream_t s, unsigned grid[3], unsigned* block,
+                     void (*between)(void*), void* user) {
+    const TreeArgs& a = ka.a;
+    grid[0] = (unsigned)(ka.ranges.d * ka.row_blocks.d);
+    grid[1] = grid[2] = 1;
+    constexpr Dtype dt = std::is_same<T, float>::value ? Dtype::F32 : Dtype::BF16;  // (16-bit: alike)
+    const int rw = tree_row_waves(dt, a);
+    int kt = 0;
+    auto run = [&](auto waves) {
+        constexpr int RW = decltype(waves)::value;
+        launch_rw<T, DPAD, RW>(ka, s, grid[0]);
+        kt = TreeCfg<T, DPAD, RW>::KT;
+        *block = 64 * TreeCfg<T, DPAD, RW>::NW;
+    };
+    if (rw == 1) run(std::integral_constant<int, 1>{});
+    else if (rw == 2) run(std::integral_constant<int, 2>{});
+    else if (rw == 4) run(std::integral_constant<int, 4>{});
+    else if constexpr (dt != Dtype::F32) run(std::integral_constant<int, 8>{});
+    if (between) between(user);
+    constexpr int LPR = DPAD / 4;
+    const int64_t rows = (int64_t)a.n_seqs * a.max_tokens * a.q_heads;
+    const unsigned g = (unsigned)((rows + 256 / LPR - 1) / (256 / LPR));
+    tree_combine<T, LPR><<<g, 256, 0, s>>>(ka, kt, 32 * rw);
+}
+
+template <typename T>
+static void launch_d(const TreeKArgs& ka, hipStream_t s, unsigned grid[3], unsigned* block,
+                     void (*between)(void*), void* user) {
+    if (ka.a.head_dim <= 64) launch_t<T, 64>(ka, s, grid, block, between, user);
+    else launch_t<T, 128>(ka, s, grid, block, between, user);
 }
 
 void launch_tree_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned grid[3],
-                           unsigned* block, unsigned* dispatches) {
-    const FastDiv ps((uint32_t)a.page_size);
-    grid[0] = (unsigned)((int64_t)a.n_seqs * a.max_tokens * a.q_heads);
-    grid[1] = grid[2] = 1;
-    *block = 64;
-    *dispatches = 1;
+                           unsigned* block, unsigned* rows, void (*between)(void*), void* user) {
+    TreeKArgs ka;
+    ka.a = a;
+    int ranges, row_blocks;
+    tree_shape(dt, a, &ranges, &row_blocks);
+    ka.ps = FastDiv((uint32_t)a.page_size);
+    ka.grp = FastDiv((uint32_t)a.group);
+    ka.ranges = FastDiv((uint32_t)ranges);
+    ka.row_blocks = FastDiv((uint32_t)row_blocks);
+    *rows = (unsigned)(32 * tree_row_waves(dt, a));
     switch (dt) {
-        case Dtype::BF16: tree_rows<bf16_t><<<grid[0], 64, 0, s>>>(a, ps); break;
-        case Dtype::F16: tree_rows<f16_t><<<grid[0], 64, 0, s>>>(a, ps); break;
-        default: tree_rows<float><<<grid[0], 64, 0, s>>>(a, ps); break;
+        case Dtype::BF16: launch_d<bf16_t>(ka, s, grid, block, between, user); break;
+        case Dtype::F16: launch_d<f16_t>(ka, s, grid, block, between, user); break;
+        default: launch_d<float>(ka, s, grid, block, between, user); break;
     }
 }
 
