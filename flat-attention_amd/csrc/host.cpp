@@ -3306,7 +3306,7 @@ int check_pools(const fa_paged_batch* b, const void* k_pool, const void* v_pool,
         return fail(FA_ERR_UNSUPPORTED_HEAD_DIM, "head_dim %llu is not a multiple of %llu, required for %s storage",
                     (unsigned long long)head_dim, (unsigned long long)unit, dtype_name(dtype));
     uint64_t need;
-    if (mul_ov(kv_heads, head_dim, row) || *row > kI32 || mul_ov(*row, elem_bytes(dtype), row) ||
+    if (mul_ov(kv_heads, head_dim, row) || *row > kI32 / 4 || mul_ov(*row, elem_bytes(dtype), row) ||
         mul_ov(b->page_size * b->physical_pages, *row, &need))
         return fail(FA_ERR_SHAPE_OVERFLOW, "attention shape overflows the address space");
     if (int rc = check_buffer("K pool", k_pool, pool_bytes, need)) return rc;
@@ -3545,13 +3545,14 @@ int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q,
     a.page_size = (int)b->page_size;
     a.physical_pages = (int)b->physical_pages;
     a.scale = scale;
-    size_t ml_offset, plan_offset;
-    const size_t bytes = fa::tree_workspace((Dtype)dtype, a, &ml_offset, &plan_offset);
+    size_t ml_offset, plan_offset, odd_offset;
+    const size_t bytes = fa::tree_workspace((Dtype)dtype, a, &ml_offset, &plan_offset, &odd_offset);
     void* ws = nullptr;
     if (int rc = grow(ctx, &ctx->ws_tree, &ctx->ws_tree_bytes, bytes, &ws)) return rc;
     a.part_o = (float*)ws;
     a.part_ml = (float2*)((uint8_t*)ws + ml_offset);
     a.plan = (int*)((uint8_t*)ws + plan_offset);
+    a.odd = (int*)((uint8_t*)ws + odd_offset);
     unsigned grid[3], block, q_rows;
     begin_span(ctx);
     fa::launch_tree_attention((Dtype)dtype, a, ctx->stream, grid, &block, &q_rows,

@@ -405,9 +405,11 @@ struct TreeArgs {
     float* part_o;
     float2* part_ml;
     int* plan;
+    int* odd;  // per workgroup: it took infinities or NaN out of V
 };
-// Bytes of the scratch of a launch of `a` and where part_ml and plan begin in it.
-size_t tree_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset);
+// Bytes of the scratch of a launch of `a` and where part_ml, plan and odd begin in it.
+size_t tree_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset,
+                      size_t* odd_offset);
 // Split kernel and combine; `between(user)` (if set) runs on the host between the launches. *rows: query
 // rows of a workgroup.
 void launch_tree_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned grid[3],

@@ -77,9 +77,23 @@ __device__ __forceinline__ void global_to_lds16(const void* p, uint32_t lds) {
     asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(lds));
 }
 
+// Division of numbers below 2^31 by a constant of the launch, in 32 bits: with s = ceil(log2 d) and
+// m = floor(2^(31 + s) / d) + 1, m d - 2^(31 + s) <= 2^s, so n m / 2^(31 + s) is off by less than 1 / d.
+struct SmallDiv {
+    uint32_t m, s;
+    __host__ SmallDiv() : m(0), s(0) {}
+    __host__ explicit SmallDiv(uint32_t d) {
+        for (s = 0; (1ull << s) < d; ++s) {
+        }
+        m = (uint32_t)((1ull << (31 + s)) / d + 1);
+    }
+    __device__ __forceinline__ int div(int n) const { return (int)(__umulhi((uint32_t)n << 1, m) >> s); }
+};
+
 struct TreeKArgs {
     TreeArgs a;
-    FastDiv ps, grp, ranges, row_blocks;
+    SmallDiv ps, grp;
+    FastDiv ranges, row_blocks;
 };
 
 // Live rows of a sequence, drafted ones included; 0: it has no part in this call.
@@ -90,12 +104,12 @@ __device__ __forceinline__ int tree_rows_of(const TreeArgs& a, int s) {
     return ok ? ctx + len : 0;
 }
 
-// Whether a word's values (one f32, two 16-bit) hold an infinity or NaN.
+// Bits of a word's values (one f32, two 16-bit) that are infinite or NaN.
 template <typename T>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-    if constexpr (std::is_same<T, float>::value) return (w & 0x7f800000u) == 0x7f800000u;
+    if constexpr (std::is_same<T, float>::value) return (w & 0x7f800000u) == 0x7f800000u ? ~0u : 0u;
     constexpr uint32_t e = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
-    return (w & e) == e || (w & (e << 16)) == (e << 16);
+    return ((w & e) == e ? 0xffffu : 0u) | ((w & (e << 16)) == (e << 16) ? 0xffff0000u : 0u);
 }
 
 // Wait for the result of a 32x32 MFMA, written out because branches come between the last product and
@@ -126,61 +140,13 @@ __device__ __forceinline__ float tree_v32(const uint8_t* smem, int va0, int i, i
     return *(const float*)(smem + (va0 ^ (mb << 7) ^ col) + (8 * (i / 4) + i % 4) * DPAD * 4);
 }
 
-// P.V of a block whose V holds infinities or NaN, in which rows may not see every key: 0 * inf would
-// make NaN of what a row must not see. Those values are taken out of V, and for the rows that see them
-// +inf, -inf and NaN are counted by a product with the visibility and added.
-template <typename T, int DPAD>
-__device__ __forceinline__ void pv_special(const uint8_t* smem, int va0, const f32x16_t& p,
-                                           uint32_t see, f32x16_t* oacc) {
-    constexpr bool F32 = std::is_same<T, float>::value;
-#pragma unroll
-    for (int mb = 0; mb < DPAD / 32; ++mb) {
-#pragma unroll 1
-        for (int x = 0; x < 4; ++x) {  // finite values, +inf, -inf, NaN
-            f32x16_t n;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) n[i] = 0.0f;
-            auto pick = [&](float v) {
-                const bool is = x == 1 ? v == INFINITY : x == 2 ? v == -INFINITY : v != v;
-                return x == 0 ? (fabsf(v) < INFINITY ? v : 0.0f) : is ? 1.0f : 0.0f;
-            };
-            if constexpr (F32) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float seen = (see >> (8 * (i / 4) + i % 4)) & 1 ? 1.0f : 0.0f;
-                    n = __builtin_amdgcn_mfma_f32_32x32x2f32(pick(tree_v32<DPAD>(smem, va0, i, mb)),
-                                                             x ? seen : p[i], n, 0, 0, 0);
-                }
-            } else {
-#pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) {
-                    const u32x4_t v = tree_v16<DPAD>(smem, va0, k2, mb);
-                    u32x4_t av, bv;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int i = 8 * k2 + 2 * j;
-                        const uint32_t w = see >> (8 * (i / 4) + i % 4);
-                        av[j] = Half<T>::pack(pick(Half<T>::lo(v[j])), pick(Half<T>::hi(v[j])));
-                        bv[j] = x ? Half<T>::pack(w & 1 ? 1.0f : 0.0f, w & 2 ? 1.0f : 0.0f)
-                                  : Half<T>::pack(p[i], p[i + 1]);
-                    }
-                    n = Half<T>::mfma32(av, bv, n);
-                }
-            }
-            wait_mfma32<F32>(n);
-            const float special = x == 1 ? INFINITY : x == 2 ? -INFINITY : NAN;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) oacc[mb][i] += x == 0 ? n[i] : n[i] > 0.0f ? special : 0.0f;
-        }
-    }
-}
-
-// Four dims of a finished row: O / l and, with the first dims, LSE. A row without a key: 0 and -inf.
+// Four dims of a finished row: O / l and, with the first dims, LSE. l = 0: the row saw no key, 0 and
+// -inf. (A row whose keys are all NaN has m = -inf too, but l = NaN.)
 template <typename T>
 __device__ __forceinline__ void write_row4(const TreeArgs& a, int s, int kvh, int row, int d, f32x4_t o,
-                                           float m, float l, const FastDiv& grp) {
-    const int t = (int)grp.div((uint32_t)row), hq = kvh * a.group + row - t * a.group;
-    const bool none = m == -INFINITY;  // (NaN and +inf maxima go the usual way)
+                                           float m, float l, const SmallDiv& grp) {
+    const int t = grp.div(row), hq = kvh * a.group + row - t * a.group;
+    const bool none = l == 0.0f;
     const float inv = none ? 0.0f : 1.0f / l;
     const int64_t at = (((int64_t)s * a.max_tokens + t) * a.q_heads + hq) * a.head_dim + d;
     if (none) o = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -208,6 +174,7 @@ void tree_split(TreeKArgs ka) {
     __shared__ int bt_lds[kTreePages];
     __shared__ int scan_lds[C::NW + 2];
     __shared__ float2 ml_lds[C::NW * 32];
+    __shared__ int odd_lds[C::NW];  // this wave took infinities or NaN out of V (2: on any key, 1: behind ctx)
     const TreeArgs& a = ka.a;
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -272,6 +239,7 @@ void tree_split(TreeKArgs ka) {
         a.plan[a.n_seqs + 1] = share;
     }
     if (pos >= end) return;
+    if (lane == 0) odd_lds[wave] = 0;
     __syncthreads();
     int s = __builtin_amdgcn_readfirstlane(scan_lds[C::NW]);
     int first = __builtin_amdgcn_readfirstlane(scan_lds[C::NW + 1]);  // first step of sequence s
@@ -295,7 +263,7 @@ void tree_split(TreeKArgs ka) {
         vbase = group_base + C::TILE + r * C::ROWB + ((p ^ swizzle<C::CPR, F32>(r)) << 4) +
                 8 * (n16 & 1);
     }
-    const int64_t row_bytes = (int64_t)a.kv_heads * D * C::EB;
+    const uint32_t row_bytes = (uint32_t)(a.kv_heads * D) * C::EB;
     const float c2 = a.scale * kLog2e;
     const int page_size = a.page_size;
 
@@ -320,7 +288,7 @@ void tree_split(TreeKArgs ka) {
 
         // ---- this lane's query row
         const int row = r0 + rw * 32 + (lane & 31);
-        const int t = (int)ka.grp.div((uint32_t)row), hq = kvh * a.group + row - t * a.group;
+        const int t = ka.grp.div(row), hq = kvh * a.group + row - t * a.group;
         bool row_ok = row < rows_total;
         const int tok = s * a.max_tokens + t;
         int rope_pos = 0;
@@ -328,24 +296,26 @@ void tree_split(TreeKArgs ka) {
             rope_pos = a.positions ? a.positions[tok] : ctx + t;
             row_ok = rope_pos >= 0 && rope_pos < a.rope_positions;
         }
+        // (without branches: a row that does not exist reads another one, and is set to zero)
         u32x4_t qop[KS], qlo[SPLIT ? KS : 1];
         auto load_q = [&]() {
             int hh = h;
             asm volatile("" : "+v"(hh));  // (no address is kept past this)
-            const uint8_t* const qrow = (const uint8_t*)a.q + ((int64_t)tok * a.q_heads + hq) * (D * C::EB);
-            const float2* const cs = a.rope_table + (int64_t)(rope_pos + a.rope_offset) * (D >> 1);
+            const int rq = min(row, a.max_tokens * a.group - 1), tq = ka.grp.div(rq);
+            const int hr = s * a.max_tokens + tq;
+            const uint8_t* const qrow = (const uint8_t*)a.q + ((int64_t)hr * a.q_heads + kvh * a.group +
+                                                               rq - tq * a.group) * (D * C::EB);
+            const float2* const cs =
+                a.rope_table + (int64_t)((row_ok ? rope_pos : 0) + a.rope_offset) * (D >> 1);
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
                 // (four pieces and their angles at a time: all of them do not fit the registers)
                 if (c % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-                const int d0 = (2 * c + hh) * E;
-                qop[c] = u32x4_t{0u, 0u, 0u, 0u};
-                if constexpr (SPLIT) qlo[c] = u32x4_t{0u, 0u, 0u, 0u};
-                if (!row_ok || d0 >= D) continue;
-                u32x4_t raw = *(const u32x4_t*)(qrow + d0 * C::EB);
+                const int d0 = (2 * c + hh) * E, dl = min(d0, D - E);
+                u32x4_t raw = *(const u32x4_t*)(qrow + dl * C::EB), lo = {0u, 0u, 0u, 0u};
                 if constexpr (F32) {
                     if (a.rope_table) {
-                        const f32x4_t w = *(const f32x4_t*)(cs + d0 / 2);
+                        const f32x4_t w = *(const f32x4_t*)(cs + dl / 2);
                         float x[4] = {__uint_as_float(raw[0]), __uint_as_float(raw[1]),
                                       __uint_as_float(raw[2]), __uint_as_float(raw[3])};
                         rope_pair(x[0], x[1], w[0], w[1]);
@@ -354,8 +324,8 @@ void tree_split(TreeKArgs ka) {
                         for (int j = 0; j < 4; ++j) raw[j] = __float_as_uint(x[j]);
                     }
                 } else if constexpr (SPLIT) {
-                    const f32x4_t w0 = *(const f32x4_t*)(cs + d0 / 2);
-                    const f32x4_t w1 = *(const f32x4_t*)(cs + d0 / 2 + 2);
+                    const f32x4_t w0 = *(const f32x4_t*)(cs + dl / 2);
+                    const f32x4_t w1 = *(const f32x4_t*)(cs + dl / 2 + 2);
                     const float c8[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
                     float x[8];
 #pragma unroll
@@ -367,11 +337,16 @@ void tree_split(TreeKArgs ka) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         raw[j] = Half<T>::pack(x[2 * j], x[2 * j + 1]);
-                        qlo[c][j] = Half<T>::pack(x[2 * j] - Half<T>::lo(raw[j]),
-                                                  x[2 * j + 1] - Half<T>::hi(raw[j]));
+                        lo[j] = Half<T>::pack(x[2 * j] - Half<T>::lo(raw[j]),
+                                              x[2 * j + 1] - Half<T>::hi(raw[j]));
                     }
                 }
-                qop[c] = raw;
+                const bool ok = row_ok && d0 < D;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    qop[c][j] = ok ? raw[j] : 0u;
+                    if constexpr (SPLIT) qlo[c][j] = ok ? lo[j] : 0u;
+                }
             }
         };
 
@@ -388,11 +363,11 @@ void tree_split(TreeKArgs ka) {
         for (int c0 = st0; c0 < st1;) {
             // ---- table entries of as many steps as they cover: first pool row of each page, -1 where
             // the id lies outside the pool
-            const int p0 = (int)ka.ps.div((uint32_t)c0 * C::KT);
+            const int p0 = ka.ps.div(c0 * C::KT);
             const int64_t reach = ((int64_t)p0 + kTreePages) * page_size;  // keys below are covered
             const int c1 = (int)min((int64_t)st1, max((int64_t)c0 + 1, reach / C::KT));
             const int k_end = min(c1 * C::KT, rows_s);
-            const int n_pages = (int)ka.ps.div((uint32_t)k_end - 1) - p0 + 1;
+            const int n_pages = ka.ps.div(k_end - 1) - p0 + 1;
             bool bad = false;
             __syncthreads();  // (the stages and entries before have been read)
             for (int i = tid; i < n_pages; i += NT) {
@@ -414,56 +389,71 @@ void tree_split(TreeKArgs ka) {
             auto transfer = [&](int step, int stage) {
                 const int tile = step * C::KT + kg * C::BN;
                 if (tile >= k_end) return;
-                int ln = lane;
+                uint32_t ln = lane, zero;
                 asm volatile("" : "+v"(ln));  // (what depends on the lane alone is not kept)
+                // (left to itself the compiler takes the zeros above 32-bit offsets from a vector of 16)
+                asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
                 constexpr int RPI = 64 / C::CPR;  // rows of an instruction
-                const int r1 = ln / C::CPR, col = ln % C::CPR;
+                const int r1 = (int)(ln / C::CPR), col = (int)(ln % C::CPR);
 #pragma unroll
                 for (int i = 0; i < C::NI; ++i) {
                     const int r = (rw * C::NI + i) * RPI + r1;
                     const int piece = col ^ swizzle<C::CPR, F32>(r);
-                    const int key = tile + r;
-                    const uint8_t *kp = (const uint8_t*)tree_zero, *vp = (const uint8_t*)tree_zero;
-                    if (key < k_end && piece * E < D) {
-                        const int lp = (int)ka.ps.div((uint32_t)key);
-                        const int base = bt_lds[lp - p0];
-                        if (base >= 0) {
-                            const int64_t off =
-                                (int64_t)(base + key - lp * page_size) * row_bytes + piece * 16;
-                            kp = kpool + off;
-                            vp = vpool + off;
-                        }
-                    }
+                    const int key = min(tile + r, k_end - 1);
+                    const int lp = ka.ps.div(key), base = bt_lds[lp - p0];
+                    const bool there = tile + r < k_end && base >= 0 && piece * E < D;
+                    const uint64_t off = (uint64_t)(uint32_t)(base + key - lp * page_size) * row_bytes +
+                                         ((uint64_t)zero << 32 | (uint32_t)piece * 16);
+                    const uint8_t* const kp = there ? kpool + off : (const uint8_t*)tree_zero;
+                    const uint8_t* const vp = there ? vpool + off : (const uint8_t*)tree_zero;
                     const uint32_t dst = lds0 + group_base + stage + (rw * C::NI + i) * 1024;
                     global_to_lds16(kp, dst);
                     global_to_lds16(vp, dst + C::TILE);
                 }
             };
 
-            // ---- 32 keys from `key0` at `at` of a stage: scores, softmax, P.V
-            auto block = [&](int key0, int at) {
+            // ---- 32 keys from `key0` at `at` of a stage: scores, softmax, P.V. MASKED: blocks in which
+            // some row may not see some key.
+            auto block = [&](int key0, int at, auto masked_c) {
+                constexpr bool MASKED = decltype(masked_c)::value;
+                const int ka0 = kbase + at, va0 = vbase + at;
                 f32x16_t sc;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
-                const int ka0 = kbase + at;
+                // all K pieces are asked for before the first product (f32: half of them)
+                constexpr int KH = F32 ? KS / 2 : KS;
 #pragma unroll
-                for (int c = 0; c < KS; ++c) {
-                    const u32x4_t kv = *(const u32x4_t*)(smem + (ka0 ^ (c << 5)));
-                    if constexpr (F32) {
+                for (int c0k = 0; c0k < KS; c0k += KH) {
+                    u32x4_t kf[KH];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            sc = __builtin_amdgcn_mfma_f32_32x32x2f32(
-                                __uint_as_float(kv[j]), __uint_as_float(qop[c][j]), sc, 0, 0, 0);
-                    } else {
-                        sc = Half<T>::mfma32(kv, qop[c], sc);
-                        if constexpr (SPLIT) sc = Half<T>::mfma32(kv, qlo[c], sc);
+                    for (int c = 0; c < KH; ++c)
+                        kf[c] = *(const u32x4_t*)(smem + (ka0 ^ ((c0k + c) << 5)));
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int c = 0; c < KH; ++c) {
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                sc = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                                    __uint_as_float(kf[c][j]), __uint_as_float(qop[c0k + c][j]), sc, 0,
+                                    0, 0);
+                        } else {
+                            sc = Half<T>::mfma32(kf[c], qop[c], sc);
+                            if constexpr (SPLIT) sc = Half<T>::mfma32(kf[c], qlo[c], sc);
+                        }
                     }
                 }
-                wait_mfma32<F32>(sc);
-                // Blocks in which some row may not see some key.
-                uint32_t see = 0xffffffffu;  // bit k: this row sees key0 + k
-                bool odd_v = false;          // V holds infinities or NaN there
-                if (key0 + 32 > ctx || bad) {
+                // 16-bit: V's operands are on their way while the softmax runs
+                u32x4_t vf[F32 ? 1 : 2][F32 ? 1 : MB];
+                if constexpr (!F32 && !MASKED) {
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+                        for (int mb = 0; mb < MB; ++mb) vf[k2][mb] = tree_v16<DPAD>(smem, va0, k2, mb);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (MASKED) {
+                    wait_mfma32<F32>(sc);
                     const int j0 = key0 - ctx;  // drafted token of the first key
                     uint64_t w;
                     if (a.masks) {
@@ -483,23 +473,13 @@ void tree_split(TreeKArgs ka) {
                     uint32_t live = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
                     if (bad) {
                         const int key = min(key0 + (lane & 31), k_end - 1);
-                        const int lp = (int)ka.ps.div((uint32_t)key);
+                        const int lp = ka.ps.div(key);
                         live &= (uint32_t)__ballot(bt_lds[lp - p0] >= 0);
                     }
-                    see = (uint32_t)w & live;
-                    const uint32_t mine = see >> (4 * h);
+                    const uint32_t see = ((uint32_t)w & live) >> (4 * h);  // this row sees these keys
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (!((mine >> (8 * (i / 4) + i % 4)) & 1)) sc[i] = -INFINITY;
-                    uint32_t any = 0;
-#pragma unroll
-                    for (int i = 0; i < 32 * C::ROWB / 1024; ++i) {
-                        const u32x4_t v =
-                            *(const u32x4_t*)(smem + group_base + C::TILE + at + i * 1024 + lane * 16);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) any |= not_finite<T>(v[j]);
-                    }
-                    odd_v = __any(any != 0);
+                        if (!((see >> (8 * (i / 4) + i % 4)) & 1)) sc[i] = -INFINITY;
                 }
                 float mt = sc[0];
 #pragma unroll
@@ -516,7 +496,8 @@ void tree_split(TreeKArgs ka) {
                     for (int mb = 0; mb < MB; ++mb) oacc[mb] *= alpha;
                     m_run = m_use;
                 }
-                const float neg = m_run == -INFINITY ? 0.0f : -m_run * c2;  // (no key seen yet)
+                // (MASKED: maybe no key seen yet)
+                const float neg = MASKED && m_run == -INFINITY ? 0.0f : -m_run * c2;
                 float ls = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -524,16 +505,22 @@ void tree_split(TreeKArgs ka) {
                     ls += sc[i];
                 }
                 l_run += ls;
-                const int va0 = vbase + at;
-                if (__builtin_expect(odd_v, 0)) {
-                    pv_special<T, DPAD>(smem, va0, sc, see >> (4 * h), oacc);
-                } else if constexpr (F32) {
+                // MASKED: a key that some row does not see may hold infinities and NaN, and 0 * inf would
+                // bring them to that row. V is taken without them; tree_combine adds what is missing.
+                uint32_t off = 0;
+                if constexpr (F32) {
 #pragma unroll
                     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            oacc[mb] = __builtin_amdgcn_mfma_f32_32x32x2f32(
-                                tree_v32<DPAD>(smem, va0, i, mb), sc[i], oacc[mb], 0, 0, 0);
+                        for (int i = 0; i < 16; ++i) {
+                            float v = tree_v32<DPAD>(smem, va0, i, mb);
+                            if constexpr (MASKED) {
+                                const uint32_t x = not_finite<T>(__float_as_uint(v));
+                                off |= x;
+                                v = x ? 0.0f : v;
+                            }
+                            oacc[mb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[i], oacc[mb], 0, 0, 0);
+                        }
                 } else {
 #pragma unroll
                     for (int k2 = 0; k2 < 2; ++k2) {
@@ -542,33 +529,57 @@ void tree_split(TreeKArgs ka) {
                         for (int j = 0; j < 4; ++j)
                             pb[j] = Half<T>::pack(sc[8 * k2 + 2 * j], sc[8 * k2 + 2 * j + 1]);
 #pragma unroll
-                        for (int mb = 0; mb < MB; ++mb)
-                            oacc[mb] = Half<T>::mfma32(tree_v16<DPAD>(smem, va0, k2, mb), pb, oacc[mb]);
+                        for (int mb = 0; mb < MB; ++mb) {
+                            u32x4_t v;
+                            if constexpr (MASKED) {
+                                v = tree_v16<DPAD>(smem, va0, k2, mb);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const uint32_t x = not_finite<T>(v[j]);
+                                    off |= x;
+                                    v[j] &= ~x;
+                                }
+                            } else {
+                                v = vf[k2][mb];
+                            }
+                            oacc[mb] = Half<T>::mfma32(v, pb, oacc[mb]);
+                        }
                     }
                 }
+                if constexpr (MASKED)
+                    if (__any(off != 0) && lane == 0) odd_lds[wave] = bad ? 2 : 1;
             };
 
-            // ---- the steps, NST - 1 transfers ahead
+            // ---- the steps, NST - 1 transfers ahead: first those whose keys every row sees
 #pragma unroll
             for (int i = 0; i < C::NST - 1; ++i)
                 if (c0 + i < c1) transfer(c0 + i, i * C::STAGE);
             if (c0 == st0) load_q();
             int stage = 0;
-            for (int step = c0; step < c1; ++step) {
-                // (transfers complete in order: those of the NST - 2 tiles behind this one may be on
-                // their way; near the end there are fewer)
-                if (C::NST > 2 && step + C::NST - 2 < c1 - 1) wait_vmcnt<(C::NST - 2) * 2 * C::NI>();
-                else wait_dma();
-                if constexpr (RW > 1) __syncthreads();
-                else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                const int ahead = stage == 0 ? (C::NST - 1) * C::STAGE : stage - C::STAGE;
-                if (step + C::NST - 1 < c1) transfer(step + C::NST - 1, ahead);
-                const int tile = step * C::KT + kg * C::BN;
+            auto run = [&](int from, int to, auto masked_c) {
 #pragma unroll 1
-                for (int kb = 0; kb < C::BN; kb += 32)
-                    if (tile + kb < k_end) block(tile + kb, stage + kb * C::ROWB);
-                stage = stage == (C::NST - 1) * C::STAGE ? 0 : stage + C::STAGE;
-            }
+                for (int step = from; step < to; ++step) {
+                    // (transfers complete in order: those of the NST - 2 tiles behind this one may be
+                    // on their way; near the end there are fewer)
+                    if (C::NST > 2 && step + C::NST - 2 < c1 - 1)
+                        wait_vmcnt<(C::NST - 2) * 2 * C::NI>();
+                    else
+                        wait_dma();
+                    if constexpr (RW > 1) __syncthreads();
+                    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    const int ahead = stage == 0 ? (C::NST - 1) * C::STAGE : stage - C::STAGE;
+                    if (step + C::NST - 1 < c1) transfer(step + C::NST - 1, ahead);
+                    const int tile = step * C::KT + kg * C::BN;
+#pragma unroll 1
+                    for (int kb = 0; kb < C::BN; kb += 32)
+                        if (!decltype(masked_c)::value || tile + kb < k_end)
+                            block(tile + kb, stage + kb * C::ROWB, masked_c);
+                    stage = stage == (C::NST - 1) * C::STAGE ? 0 : stage + C::STAGE;
+                }
+            };
+            const int cm = bad ? c0 : max(c0, min(c1, ctx / C::KT));
+            run(c0, cm, std::false_type{});
+            run(cm, c1, std::true_type{});
             c0 = c1;
         }
 
@@ -577,7 +588,8 @@ void tree_split(TreeKArgs ka) {
         int te = tid;
         asm volatile("" : "+v"(te));  // (no address is kept from unit to unit)
         const int le = te & 63, he = le >> 5;
-        if (he == 0) ml_lds[wave * 32 + (le & 31)] = make_float2(m_run, l_run);
+        // (a token without a position has run with Q = 0: as if it had seen nothing)
+        if (he == 0) ml_lds[wave * 32 + (le & 31)] = make_float2(m_run, row_ok ? l_run : 0.0f);
         __syncthreads();  // (every stage has been read)
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
@@ -599,8 +611,8 @@ void tree_split(TreeKArgs ka) {
 #pragma unroll
             for (int g = 0; g < C::KW; ++g) {
                 const float2 ml = ml_lds[g * C::ROWS + r];
-                const float w = ml.x == -INFINITY ? 0.0f : fast_exp2((ml.x - M) * c2);
-                if (ml.x == -INFINITY) continue;  // (saw nothing: O = 0, l = 0)
+                if (ml.y == 0.0f) continue;  // (saw nothing)
+                const float w = fast_exp2((ml.x - M) * c2);
                 const f32x4_t x = *(const f32x4_t*)(smem + (g * C::ROWS + r) * C::MROW + 4 * d);
                 L = fmaf(ml.y, w, L);
 #pragma unroll
@@ -613,6 +625,13 @@ void tree_split(TreeKArgs ka) {
             }
             write_row4<T>(a, s, kvh, r0 + r, d, o, M, L, ka.grp);
         }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int odd = 0;
+#pragma unroll
+        for (int w = 0; w < C::NW; ++w) odd = max(odd, odd_lds[w]);
+        a.odd[logical] = odd;
     }
 }
 
@@ -641,25 +660,71 @@ __global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int ro
     const int steps = (rows_s + kt - 1) / kt;
     const uint32_t u0 = (uint32_t)a.plan[s] + (uint32_t)kvh * (uint32_t)steps;
     const int g0 = (int)(u0 / (uint32_t)share), g1 = (int)((u0 + steps - 1) / (uint32_t)share);
-    if (g0 == g1) return;  // finished by the range that covers it
     const int rb = row / rows_block, r = row - rb * rows_block;
     const float c2 = a.scale * kLog2e;
+    int odd = 0;
+    if (g0 == g1) {
+        odd = a.odd[(int64_t)g0 * ka.row_blocks.d + rb];
+        if (!odd) return;  // finished by the range that covers it
+    }
     float M = -INFINITY, L = 0.0f;
     f32x4_t o = zero;
-    for (int g = g0; g <= g1; ++g) {
-        const int64_t slot = 2 * ((int64_t)g * ka.row_blocks.d + rb) + (g == g0 ? 1 : 0);
-        const float2 ml = a.part_ml[slot * rows_block + r];
-        const f32x4_t x = *(const f32x4_t*)(a.part_o + (slot * rows_block + r) * D + d);
-        if (ml.x == -INFINITY) continue;
-        const float mx = fmaxf(M, ml.x);
-        const float w0 = M == -INFINITY ? 0.0f : fast_exp2((M - mx) * c2);
-        const float w1 = fast_exp2((ml.x - mx) * c2);
-        M = mx;
-        L = fmaf(ml.y, w1, L * w0);
+    if (g0 < g1)
+        for (int g = g0; g <= g1; ++g) {
+            const int64_t slot = 2 * ((int64_t)g * ka.row_blocks.d + rb) + (g == g0 ? 1 : 0);
+            const float2 ml = a.part_ml[slot * rows_block + r];
+            const f32x4_t x = *(const f32x4_t*)(a.part_o + (slot * rows_block + r) * D + d);
+            odd = max(odd, a.odd[(int64_t)g * ka.row_blocks.d + rb]);
+            if (ml.y == 0.0f) continue;
+            const float mx = fmaxf(M, ml.x);
+            const float w0 = L == 0.0f ? 0.0f : fast_exp2((M - mx) * c2);
+            const float w1 = fast_exp2((ml.x - mx) * c2);
+            M = mx;
+            L = fmaf(ml.y, w1, L * w0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], w1, o[j] * w0);
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], w1, o[j] * w0);
+        }
+    if (!odd) {
+        write_row4<T>(a, s, kvh, row, d, o, M, L, ka.grp);
+        return;
     }
-    write_row4<T>(a, s, kvh, row, d, o, M, L, ka.grp);
+    // ---- V held infinities or NaN where rows do not see every key: the values that this row sees
+    const int ctx = rows_s - len, t = ka.grp.div(row);
+    const int hq = kvh * a.group + row - t * a.group;
+    if (g0 == g1) {
+        L = a.lse[((int64_t)s * a.q_heads + hq) * a.max_tokens + t] == -INFINITY ? 0.0f : 1.0f;
+    } else {
+        write_row4<T>(a, s, kvh, row, d, o, M, L, ka.grp);
+    }
+    if (L == 0.0f) return;  // (sees nothing)
+    f32x4_t add = zero;
+    for (int key = odd > 1 ? 0 : ctx / kt * kt; key < rows_s; ++key) {
+        const int j = key - ctx;
+        const bool seen = j < 0 ? true
+                          : a.masks
+                              ? (a.masks[((int64_t)s * a.max_tokens + t) * a.words + (j >> 6)] >> (j & 63)) & 1
+                              : j <= t;
+        if (!seen) continue;
+        const int lp = ka.ps.div(key), page = a.block_tables[(int64_t)s * a.max_pages + lp];
+        if ((unsigned)page >= (unsigned)a.physical_pages) continue;
+        const int64_t at = (((int64_t)page * a.page_size + key - lp * a.page_size) * a.kv_heads + kvh) * D + d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float v;
+            if constexpr (std::is_same<T, float>::value) v = ((const float*)a.v_pool)[at + e];
+            else v = Half<T>::lo(((const uint16_t*)a.v_pool)[at + e]);
+            if (!(fabsf(v) < INFINITY)) add[e] += v;
+        }
+    }
+    const int64_t to = (((int64_t)s * a.max_tokens + t) * a.q_heads + hq) * D + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (add[e] == 0.0f) continue;
+        if constexpr (std::is_same<T, float>::value) ((float*)a.o)[to + e] += add[e];
+        else
+            ((uint16_t*)a.o)[to + e] = (uint16_t)Half<T>::pack(
+                Half<T>::lo(((const uint16_t*)a.o)[to + e]) + add[e], 0.0f);
+    }
 }
 
 // Rows of a workgroup: as few row blocks of 32 as hold every row of a (sequence, kv head), at most 4;
@@ -676,13 +741,15 @@ static void tree_shape(Dtype dt, const TreeArgs& a, int* ranges, int* row_blocks
     *ranges = std::max(1, (rw == 2 || rw == 4 ? 2 : 1) * device_cus() / *row_blocks);
 }
 
-size_t tree_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset) {
+size_t tree_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset,
+                      size_t* odd_offset) {
     int ranges, row_blocks;
     tree_shape(dt, a, &ranges, &row_blocks);
     const size_t rows = (size_t)2 * ranges * row_blocks * 32 * tree_row_waves(dt, a);
     *ml_offset = rows * a.head_dim * 4;
     *plan_offset = *ml_offset + rows * 8;
-    return *plan_offset + ((size_t)a.n_seqs + 2) * 4;
+    *odd_offset = *plan_offset + ((size_t)a.n_seqs + 2) * 4;
+    return *odd_offset + (size_t)ranges * row_blocks * 4;
 }
 
 template <typename T, int DPAD, int RW>
@@ -736,8 +803,8 @@ void launch_tree_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned 
     ka.a = a;
     int ranges, row_blocks;
     tree_shape(dt, a, &ranges, &row_blocks);
-    ka.ps = FastDiv((uint32_t)a.page_size);
-    ka.grp = FastDiv((uint32_t)a.group);
+    ka.ps = SmallDiv((uint32_t)a.page_size);
+    ka.grp = SmallDiv((uint32_t)a.group);
     ka.ranges = FastDiv((uint32_t)ranges);
     ka.row_blocks = FastDiv((uint32_t)row_blocks);
     *rows = (unsigned)(32 * tree_row_waves(dt, a));

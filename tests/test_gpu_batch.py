@@ -208,7 +208,7 @@ class Case:
         rng = np.random.default_rng(seed)
         self.ctx, self.lens, self.page = np.asarray(ctx), np.asarray(lens), page
         n = len(ctx)
-        fit = [c + m if c >= 0 and 0 <= m <= most else 0 for c, m in zip(ctx, lens)]
+        fit = [c + m if 0 <= c < 1 << 20 and 0 <= m <= most else 0 for c, m in zip(ctx, lens)]
         self.table, self.pages, _ = paged(rng, fit, page)
         self.q, qs = storage(magnitude * rng.standard_normal((n, most, hq, D)), dtype)
         rows = self.pages * page
@@ -245,11 +245,12 @@ class Case:
         for buf, x in zip(self.bufs[1:], (self.ks, self.vs)):
             buf.upload(x)
 
-    def call(self):
+    def call(self, upload=True):
         hq, hkv, D = self.dims
-        m = None if self.masks is None else fa.DeviceBuffer.from_array(self.hip, self.masks)
-        p = None if self.pos is None else i32(self.hip, self.pos)
-        self.keep = (m, p)
+        if upload:
+            self.keep = (None if self.masks is None else fa.DeviceBuffer.from_array(self.hip, self.masks),
+                         None if self.pos is None else i32(self.hip, self.pos))
+        m, p = self.keep
         self.batch.tree_attention(
             *self.bufs, self.out, self.len_buf, self.most, hq, hkv, D,
             fa.FlatAttentionConfig(True, self.scale),
@@ -327,3 +328,361 @@ def test_tree_attention_matches_float64(hip, dtype, shape, tree, rope):
     ctx, lens, most, hq, hkv, D, page = SHAPES[shape]
     Case(hip, dtype, ctx, lens, most, hq, hkv, D, page, 100 + shape, tree, rope,
          offset=37 if shape % 2 else 0, scale=0.2 if shape % 3 == 0 else None).check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("page,ctx,hq,hkv,most", [(1, 5000, 4, 2, 9), (2, 2600, 2, 2, 65),
+                                                  (16, 20000, 2, 1, 3)])
+def test_more_table_entries_than_are_held_at_a_time(hip, dtype, page, ctx, hq, hkv, most):
+    Case(hip, dtype, [ctx, 3, ctx // 2], [most, 1, most - 1], most, hq, hkv, 64, page, 7).check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n,most", [(70, 3), (300, 2), (700, 1)])
+def test_many_sequences(hip, dtype, n, most):
+    """More sequences than a workgroup has threads; some without drafted tokens."""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, most + 1, n)
+    case = Case(hip, dtype, rng.integers(0, 90, n), lens, most, 4, 2, 32, 16, 8)
+    case.check()
+
+
+def test_large_scores_and_empty_rows(hip):
+    """Scores of hundreds (the running maximum moves), and a mask that leaves rows nothing."""
+    for dtype in (BF16, F16, F32):
+        Case(hip, dtype, [700, 33], [20, 12], 20, 8, 2, 128, 16, 9, magnitude=60.0).check()
+        case = Case(hip, dtype, [0, 64, 0], [20, 18, 1], 20, 4, 2, 64, 16, 10)
+        case.masks = np.zeros_like(case.masks)  # no token sees a drafted one
+        case.sees = np.zeros_like(case.sees)
+        o, lse = case.check()
+        assert np.isneginf(lse[0]).all() and np.isfinite(lse[1, :, :18]).all()
+
+
+def test_sequences_and_tokens_that_do_not_fit(hip):
+    """Lengths out of range, positions outside the table: O = 0 and LSE = -inf there, the others as
+    without them."""
+    for dtype in (BF16, F32):
+        ctx, lens = [40, -1, 2147483647, 40, 17, 60], [6, 3, 2, -2, 9, 8]
+        case = Case(hip, dtype, ctx, lens, 8, 4, 2, 64, 16, 11)
+        case.pos = case.pos.copy()
+        case.pos[5, :3] = [-1, 5 * 16, 2147483647]  # (the table row holds 5 pages)
+        case.where = np.where(case.pos < 5 * 16, case.pos, -1)
+        assert case.table.shape[1] == 5
+        o, lse = case.check()
+        assert (o[1:5] == 0).all() and np.isneginf(lse[1:5]).all()
+        assert (o[5, :3] == 0).all() and np.isneginf(lse[5, :, :3]).all()
+        assert np.isfinite(lse[5, :, 3:]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("hq,most", [(2, 6), (8, 30), (8, 70)])
+def test_pages_outside_the_pool_are_as_if_masked(hip, dtype, hq, most):
+    case = Case(hip, dtype, [300, 90], [most, most - 1], most, hq, 2, 64, 16, 12)
+    for s, lp, page in ((0, 2, -1), (0, 11, case.pages), (1, 0, 2147483647), (1, 3, -2147483648)):
+        case.table[s, lp] = page
+    case.batch.block_tables.upload(case.table.astype(np.int32))
+    o, lse = case.run()
+    for s in range(2):
+        c, m = int(case.ctx[s]), int(case.lens[s])
+        keys = np.arange(c + m)
+        there = (case.table[s, keys // 16] >= 0) & (case.table[s, keys // 16] < case.pages)
+        sees = np.ones((m, c + m), bool)
+        sees[:, c:] = case.sees[s, :m, :m]
+        q = model.rotate(case.q[s, :m], case.where[s, :m], THETA)
+        at = np.where(there, case.table[s, keys // 16], 0).astype(np.int64) * 16 + keys % 16
+        eo, el, av, size = model.attend(q, case.k[at], case.v[at], sees & there, 64.0 ** -0.5)
+        h = HALF_STEP[dtype]
+        ds = size * (80 * 2.0 ** -24 + (h * h if dtype != F32 else 0)) + 2.0 ** -15
+        assert (np.abs(lse[s, :, :m] - el) <= ds).all()
+        assert (np.abs(o[s, :m] - eo) <= h * (np.abs(eo) + av) + 3 * ds.T[..., None] * av + 2.0 ** -25).all()
+
+
+@pytest.mark.filterwarnings("ignore:invalid value")
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("hq,most,ctx", [(2, 6, 40), (8, 40, 500), (4, 64, 31), (16, 33, 2000)])
+def test_special_values_reach_the_rows_that_see_them(hip, dtype, hq, most, ctx):
+    """NaN and infinities in K and V of drafted rows and of the last live rows: rows that do not see the
+    key are bitwise what they are without it; in those that do, a V value brings its own kind to its
+    column, a K that is NaN all columns."""
+    clean = Case(hip, dtype, [ctx, 5], [most, 2], most, hq, 2, 64, 16, 13)
+    o0, l0 = clean.run()
+    case = Case(hip, dtype, [ctx, 5], [most, 2], most, hq, 2, 64, 16, 13)
+    group = hq // 2
+    rows = case.rows(0, ctx + most)
+    sees = np.ones((most, ctx + most), bool)
+    sees[:, ctx:] = case.sees[0]
+    vs = case.vs.reshape(case.v.shape)
+    put = {x: fa.host_storage(np.array([x], np.float32), dtype)[0] for x in (np.nan, np.inf, -np.inf)}
+    spots = [(ctx + most - 1, 0, 3, np.nan), (ctx + most // 2, 0, 3, np.inf), (ctx, 1, 9, np.inf),
+             (ctx + most // 3, 1, 9, -np.inf), (ctx - 1, 1, 60, -np.inf), (ctx + 1, 0, 17, -np.inf)]
+    want = np.zeros((most, hq, 64))
+    for key, head, d, x in spots:
+        vs[rows[key], head, d] = put[x]
+        add = np.where(sees[:, key], x, 0.0)
+        want[:, head * group:(head + 1) * group, d] += add[:, None]
+    case.upload()
+    o1, l1 = case.run()
+    assert np.array_equal(l1.view(np.uint32), l0.view(np.uint32))
+    hit = want != 0
+    assert np.array_equal(o1[0][~hit].view(np.uint32), o0[0][~hit].view(np.uint32))
+    assert np.array_equal(o1[1].view(np.uint32), o0[1].view(np.uint32))
+    assert np.array_equal(o1[0][hit], want[hit], equal_nan=True)
+    # K: a drafted token that not every row sees
+    ks = case.ks.reshape(case.k.shape)
+    case.vs[:] = clean.vs
+    key = ctx + most // 2
+    ks[rows[key], 1, 7] = put[np.nan]
+    case.upload()
+    o2, l2 = case.run()
+    hit = np.zeros((most, hq), bool)
+    hit[:, group:] = sees[:, key][:, None]
+    assert np.isnan(o2[0][hit]).all() and np.isnan(l2[0].T[hit]).all()
+    assert np.array_equal(o2[0][~hit].view(np.uint32), o0[0][~hit].view(np.uint32))
+    assert np.array_equal(l2[0].T[~hit].view(np.uint32), l0[0].T[~hit].view(np.uint32))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_results_do_not_depend_on_page_order_or_repetition(hip, dtype):
+    a = Case(hip, dtype, [900, 31, 400], [16, 9, 3], 16, 8, 2, 128, 16, 14)
+    o0, l0 = a.run()
+    for _ in range(3):
+        o1, l1 = a.run()
+        assert np.array_equal(o0, o1) and np.array_equal(l0, l1)
+    # the same rows on other pages
+    rng = np.random.default_rng(99)
+    order = rng.permutation(a.pages)
+    inv = np.argsort(order)
+    ks, vs = (x.reshape(a.pages, -1)[order].reshape(x.shape) for x in (a.ks, a.vs))
+    a.ks, a.vs = ks, vs
+    a.upload()
+    moved = np.where(a.table >= 0, inv[np.maximum(a.table, 0)], -1)
+    a.batch.block_tables.upload(moved.astype(np.int32))
+    o1, l1 = a.run()
+    assert np.array_equal(o0, o1) and np.array_equal(l0, l1)
+
+
+def test_single_tokens_match_the_paged_decode(hip):
+    """One token a sequence without masks is the decode step of fa_paged_decode_*."""
+    for dtype in (BF16, F16, F32):
+        case = Case(hip, dtype, [511, 0, 2047, 76], [1] * 4, 1, 16, 4, 128, 16, 15, tree=False)
+        o, lse = case.check()
+        plan = fa.PagedDecodePlan(hip, case.table.clip(0), case.ctx + 1, 16, case.pages, 16, 4, 128,
+                                  fa.FlatAttentionConfig(True), THETA, dtype)
+        out = fa.DeviceBuffer(hip, plan.layout().combined_bytes)
+        plan.launch(*case.bufs, out)
+        r = fa.download_attention(out, plan.layout(), dtype)
+        ref = fa.storage_to_f32(r.output, dtype).reshape(o.shape)
+        assert np.abs(lse.reshape(-1) - r.lse).max() < 2e-5
+        assert np.abs(o - ref).max() <= (4 * HALF_STEP[dtype] + 2e-6) * np.abs(ref).max()
+
+
+# ------------------------------------------------------------------------------- accept
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("inplace", [True, False])
+@pytest.mark.parametrize("n,most,width,page,hkv,D", [(1, 1, 1, 16, 1, 8), (6, 20, 9, 5, 2, 64),
+                                                     (40, 64, 64, 16, 8, 128), (5, 512, 200, 24, 3, 40)])
+def test_accept_moves_rows_like_the_model(hip, dtype, inplace, n, most, width, page, hkv, D):
+    rng = np.random.default_rng(most)
+    ctx, lens = rng.integers(0, 60, n), rng.integers(1, most + 1, n)
+    table, pages, _ = paged(rng, ctx + lens, page)
+    accepted = np.array([rng.integers(0, min(l, width) + 1) for l in lens])
+    paths = np.full((n, width), -7)
+    for s in range(n):
+        paths[s, :accepted[s]] = np.sort(rng.permutation(lens[s])[:accepted[s]])
+    if n > 4:  # what is no path, no length, no page
+        k = 2
+        accepted[0], lens[0] = k, max(lens[0], 3)
+        paths[0, :k] = [1, 1]
+        accepted[1] = lens[1] + 1 if lens[1] < width else -1
+        accepted[2], paths[2, 0] = 1, lens[2]
+        lens[3] = 600
+        accepted[4], paths[4, 0] = 1, lens[4] - 1
+        table[4, (ctx[4] + lens[4] - 1) // page] = pages
+    rows = pages * page
+    k, ks = storage(rng.standard_normal((rows, hkv * D)), dtype)
+    v, vs = storage(rng.standard_normal((rows, hkv * D)), dtype)
+    kb, vb = fa.DeviceBuffer.from_array(hip, ks), fa.DeviceBuffer.from_array(hip, vs)
+    c = i32(hip, ctx)
+    out = None if inplace else i32(hip, np.full(n, 77))
+    batch = fa.HipPagedBatch(hip, i32(hip, table), c, n, table.shape[1], page, pages)
+    batch.accept(i32(hip, paths), width, i32(hip, accepted), i32(hip, lens), kb, vb, hkv, D, dtype,
+                 ctx_lens_out=out)
+    ek, ev, ec = model.accept(k, v, table, ctx, paths, accepted, lens, page, pages, 512)
+    assert np.array_equal((out or c).download(np.int32, n), ec)
+    assert np.array_equal(load(kb, k.shape, dtype), ek)
+    assert np.array_equal(load(vb, v.shape, dtype), ev)
+    if out is not None:
+        assert np.array_equal(c.download(np.int32, n), ctx)
+
+
+# ------------------------------------------------------------------------------- the loop
+
+class Loop:
+    """A speculative decoding loop on the GPU beside its float64 model: requests come and go, every
+    step drafts a tree, appends it, attends, and accepts a path."""
+
+    def __init__(self, hip, dtype, seed):
+        self.hip, self.dtype, self.n, self.most, self.page = hip, dtype, 3, 12, 8
+        self.hq, self.hkv, self.D, self.width, self.pages, self.accept = 8, 2, 64, 12, 24, 5
+        self.rng = np.random.default_rng(seed)
+        n, most = self.n, self.most
+        self.state = {"table": np.zeros((n, self.width), np.int64), "ctx": np.zeros(n, np.int64),
+                      "mapped": np.zeros(n, np.int64), "count": self.pages,
+                      "free": self.rng.permutation(self.pages)}
+        s = self.state
+        self.b = {k: i32(hip, np.atleast_1d(s[k])) for k in s}
+        for name, shape in (("new", (n,)), ("granted", (n,)), ("slots", (n, most)),
+                            ("parents", (n, most)), ("pos", (n, most)), ("paths", (n, self.accept)),
+                            ("accepted", (n,))):
+            self.b[name] = i32(hip, np.zeros(shape))
+        self.b["masks"] = fa.DeviceBuffer(hip, n * most * 8)
+        eb = 4 if dtype == F32 else 2
+        self.k, self.v = (np.zeros((self.pages * self.page, self.hkv, self.D)) for _ in range(2))
+        self.kp, self.vp = (fa.DeviceBuffer.from_array(hip, fa.host_storage(
+            np.zeros(self.k.size, np.float32), dtype)) for _ in range(2))
+        self.q, self.ks, self.vs = (fa.DeviceBuffer(hip, n * most * h * self.D * eb)
+                                    for h in (self.hq, self.hkv, self.hkv))
+        self.batch = fa.HipPagedBatch(hip, self.b["table"], self.b["ctx"], n, self.width, self.page,
+                                      self.pages)
+        self.lay = self.batch.layout(most, self.hq, self.D, dtype)
+        self.out = fa.DeviceBuffer(hip, self.lay.combined_bytes)
+
+    def enqueue(self):
+        b, rot = self.b, fa.RotaryEmbeddingConfig(THETA, 0)
+        self.batch.reserve(b["new"], self.most, b["mapped"], b["free"], b["count"], b["granted"],
+                           b["slots"])
+        self.batch.tree_masks(b["parents"], b["granted"], self.most, b["masks"], b["pos"])
+        self.batch.append(b["slots"], self.most, self.ks, self.vs, self.kp, self.vp, self.hkv, self.D,
+                          rot, self.dtype, positions=b["pos"])
+        self.batch.tree_attention(self.q, self.kp, self.vp, self.out, b["granted"], self.most, self.hq,
+                                  self.hkv, self.D, fa.FlatAttentionConfig(), rot, self.dtype,
+                                  positions=b["pos"], masks=b["masks"])
+        self.batch.accept(b["paths"], self.accept, b["accepted"], b["granted"], self.kp, self.vp,
+                          self.hkv, self.D, self.dtype)
+
+    def step(self, launch):
+        n, most, rng, b, s = self.n, self.most, self.rng, self.b, self.state
+        new = rng.integers(1, most + 1, n)
+        new[rng.random(n) < 0.2] = -1
+        parents, _ = drafts(rng, n, most, 4)
+        q, qs = storage(rng.standard_normal((n, most, self.hq, self.D)), self.dtype)
+        k, ks = storage(rng.standard_normal((n, most, self.hkv, self.D)), self.dtype)
+        v, vs = storage(rng.standard_normal((n, most, self.hkv, self.D)), self.dtype)
+        want = model.reserve(s["table"], s["ctx"], new, s["mapped"], s["free"], s["count"], most,
+                             self.page, self.pages)
+        granted, ctx = want["granted"], want["ctx"]
+        seen, pos = model.tree(parents, granted, ctx, most)
+        paths, accepted = np.zeros((n, self.accept), np.int64), np.zeros(n, np.int64)
+        for i in range(n):
+            if granted[i]:
+                leaf = int(rng.integers(0, granted[i]))
+                path = np.flatnonzero(seen[i, leaf])[:self.accept]
+                accepted[i] = path.size
+                paths[i, :path.size] = path
+        for name, x in (("new", new), ("parents", parents), ("paths", paths), ("accepted", accepted)):
+            b[name].upload(x.astype(np.int32))
+        for buf, x in ((self.q, qs), (self.ks, ks), (self.vs, vs)):
+            buf.upload(x)
+        self.out.fill_u32(0x7fc07fc0)
+        launch()
+        # the model's step; K as the GPU rotated and rounded it is read back below
+        assert np.array_equal(b["slots"].download(np.int32, n * most).reshape(n, most), want["slots"])
+        assert np.array_equal(b["granted"].download(np.int32, n), granted)
+        assert np.array_equal(b["pos"].download(np.int32, n * most).reshape(n, most), pos)
+        r = fa.download_attention(self.out, self.lay, self.dtype)
+        o = fa.storage_to_f32(r.output, self.dtype).reshape(n, most, self.hq, self.D)
+        lse = r.lse.reshape(n, self.hq, most)
+        for i in range(n):
+            for t in range(int(granted[i])):
+                row = want["slots"][i, t]
+                x, _ = storage(model.rotate(k[i, t][None], [pos[i, t]], THETA)[0], self.dtype)
+                self.k[row], self.v[row] = x, v[i, t]
+        h = HALF_STEP[self.dtype]
+        for i in range(n):
+            c, m = int(ctx[i]), int(granted[i])
+            at = np.arange(c + m)
+            at = want["table"][i, at // self.page] * self.page + at % self.page
+            sees = np.ones((m, c + m), bool)
+            sees[:, c:] = seen[i, :m, :m]
+            eo, el, av, size = model.attend(model.rotate(q[i, :m], pos[i, :m], THETA), self.k[at],
+                                            self.v[at], sees, self.D ** -0.5)
+            # (the model's K may be rounded to the other neighbour: another h of every score)
+            ds = size * (80 * 2.0 ** -24 + 2 * h + 2.0 ** -20) + 2.0 ** -15
+            assert (np.abs(lse[i, :, :m] - el) <= ds).all()
+            assert (np.abs(o[i, :m] - eo) <= h * (np.abs(eo) + av) + 3 * ds.T[..., None] * av).all()
+            assert (o[i, m:] == 0).all() and np.isneginf(lse[i, :, m:]).all()
+        width = self.hkv * self.D
+        k2, v2, ctx2 = model.accept(self.k.reshape(-1, width), self.v.reshape(-1, width), want["table"],
+                                    ctx, paths, accepted, granted, self.page, self.pages, 512)
+        self.k, self.v = k2.reshape(self.k.shape), v2.reshape(self.v.shape)
+        want["ctx"] = ctx2
+        assert np.array_equal(b["ctx"].download(np.int32, n), ctx2)
+        assert b["count"].download(np.int32, 1)[0] == want["count"]
+        assert np.array_equal(b["mapped"].download(np.int32, n), want["mapped"])
+        got = load(self.kp, self.k.shape, self.dtype)
+        size = np.abs(self.k[..., 0::2]) + np.abs(self.k[..., 1::2])
+        assert (np.abs(got - self.k) <= 2 * h * np.abs(self.k) + 2.0 ** -20 * np.repeat(size, 2, -1)
+                + 2.0 ** -24).all()
+        assert np.array_equal(load(self.vp, self.v.shape, self.dtype), self.v)
+        self.state = {x: want[x] for x in self.state}
+        return ctx2
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_decoding_loop_on_the_gpu(hip, dtype):
+    loop = Loop(hip, dtype, 21)
+    longest = 0
+    for _ in range(25):
+        longest = max(longest, int(loop.step(loop.enqueue).max()))
+    assert longest > 2 * loop.page
+
+
+def test_decoding_loop_replayed_from_a_graph(hip):
+    """The five calls captured once: every replay reads the lengths that the one before it left. Eager
+    calls of another shape, which use the same workspaces, run between the replays."""
+    loop = Loop(hip, BF16, 22)
+    loop.step(loop.enqueue)  # (sizes the context's workspaces and tables)
+    other = Case(hip, BF16, [300, 20], [7, 3], 7, 8, 2, 64, 16, 16)
+    o0, l0 = other.run()
+    with hip.capture() as cap:
+        loop.enqueue()
+    with hip.capture() as cap2:
+        other.call(upload=False)
+    for i in range(8):
+        loop.step(cap.graph.launch)
+        other.out.fill_u32(0x7fc07fc0)
+        if i % 2:
+            other.call(upload=False)  # (the graph reads the same masks and positions)
+        else:
+            cap2.graph.launch()
+        o1, l1 = other.get()
+        assert np.array_equal(o0, o1) and np.array_equal(l0, l1)
+
+
+def test_capture_refuses_calls_that_would_allocate(hip):
+    ctx = fa.HipContext(0)
+    try:
+        case = Case(ctx, BF16, [300], [7], 7, 8, 2, 64, 16, 17)
+        m, p = fa.DeviceBuffer.from_array(ctx, case.masks), i32(ctx, case.pos)
+        with ctx.capture():
+            with pytest.raises(fa.FlatHipError) as e:
+                case.batch.tree_attention(*case.bufs, case.out, case.len_buf, 7, 8, 2, 64,
+                                          fa.FlatAttentionConfig(), fa.RotaryEmbeddingConfig(THETA), BF16,
+                                          positions=p, masks=m)
+            assert e.value.variant == "GraphCapture"
+        case.check()
+    finally:
+        ctx.close()
+
+
+def test_telemetry_and_kernel_timing(hip):
+    case = Case(hip, BF16, [300, 20], [7, 3], 7, 8, 2, 64, 16, 18)
+    hip.set_kernel_timing(True)
+    case.run()
+    t = hip.last_telemetry()
+    assert t.kernel_id == "TreeAttention" and t.query_rows == 32 and t.dispatch_count == 2
+    for name in ("TreeAttention", "TreeCombine"):
+        ms, launches = hip.kernel_timing(name)
+        assert launches == 1 and 0 < ms < 10
+    hip.set_kernel_timing(False)
