@@ -38,14 +38,20 @@ namespace fa {
 // Sixteen zero bytes: what rows and dims that do not exist are fetched from.
 __device__ __attribute__((aligned(16))) uint32_t tree_zero[4];
 
+// Scheduling groups (LLVM sched_group_barrier masks: 0x2 VALU, 0x8 MFMA, 0x100 DS read, 0x400 transcendental).
+#define FA_SG(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
+
 constexpr int kTreePages = 1024;  // block-table entries held in LDS at a time
 
-template <typename T, int DPAD, int RW>
+// RW row blocks of 32 rows, HW kv heads side by side: NW / RW groups of waves, of which HW KW = NW / RW
+// with KW key groups a head.
+template <typename T, int DPAD, int RW, int HW>
 struct TreeCfg {
     static constexpr bool F32 = std::is_same<T, float>::value;
     static constexpr int EB = F32 ? 4 : 2;
     static constexpr int NW = RW == 8 ? 8 : F32 && RW < 4 ? 2 : 4;  // waves
-    static constexpr int KW = NW / RW;                              // key groups
+    static constexpr int GR = NW / RW;                              // groups
+    static constexpr int KW = GR / HW;                              // key groups
     static constexpr int BN = !F32 && RW == 8 ? 64 : 32;            // keys of a group's tile
     static constexpr int KT = KW * BN;                              // keys of a step
     static constexpr int ROWB = DPAD * EB;                          // bytes of an LDS row
@@ -53,14 +59,18 @@ struct TreeCfg {
     static constexpr int TILE = BN * ROWB;
     static constexpr int STAGE = 2 * TILE;  // K and V of a group
     static constexpr int NST = F32 || RW < 4 ? 2 : 4;  // stages: NST - 1 tiles are on their way
-    static constexpr int SMEM_KV = KW * NST * STAGE;
+    static constexpr int SMEM_KV = GR * NST * STAGE;
     static constexpr int MROW = DPAD * 4 + 16;  // row of the O exchange
-    static constexpr int SMEM_O = NW * 32 * MROW;
+    static constexpr int SMEM_O = KW > 1 ? NW * 32 * MROW : 0;
     static constexpr int SMEM = SMEM_KV > SMEM_O ? SMEM_KV : SMEM_O;
     static constexpr int ROWS = 32 * RW;
     // transfer instructions (64 pieces each) of K (or V) a wave issues per tile
     static constexpr int NI = BN * CPR / 64 / RW;
+    // the scores of the next block are computed beside the softmax of this one: its tile has to be there
+    static constexpr bool PIPE = !F32 && NST > 2;
     static constexpr int WAVES = (SMEM > 72 * 1024 && NW < 8) || (F32 && DPAD > 64) ? 1 : 2;  // per SIMD
+    // f32 quads of a 32-row block in a partial, in the order that the waves hold them
+    static constexpr int QUADS = 8 * DPAD;
 };
 
 // Which column a piece of an LDS row is kept in: piece ^ swizzle(row). 16 columns of 16 bytes are the 64
@@ -160,11 +170,23 @@ __device__ __forceinline__ void write_row4(const TreeArgs& a, int s, int kvh, in
             none ? -INFINITY : m * a.scale + logf(l);
 }
 
-template <typename T, int DPAD, int RW, bool SPLIT>
-__global__ __launch_bounds__((64 * TreeCfg<T, DPAD, RW>::NW),
-                             (TreeCfg<T, DPAD, RW>::WAVES))
+// Inclusive prefix sum over a wave (row shifts by 1, 2, 4, 8, then the last lane of each row of 16 to
+// the next row, and of the first half to the second).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+template <typename T, int DPAD, int RW, int HW, bool SPLIT>
+__global__ __launch_bounds__((64 * TreeCfg<T, DPAD, RW, HW>::NW),
+                             (TreeCfg<T, DPAD, RW, HW>::WAVES))
 void tree_split(TreeKArgs ka) {
-    using C = TreeCfg<T, DPAD, RW>;
+    using C = TreeCfg<T, DPAD, RW, HW>;
     constexpr bool F32 = C::F32;
     constexpr int MB = DPAD / 32;                   // 32-dim blocks of O^T
     constexpr int KS = F32 ? DPAD / 8 : DPAD / 16;  // K pieces a lane reads per 32 keys
@@ -172,81 +194,57 @@ void tree_split(TreeKArgs ka) {
     constexpr int E = 16 / C::EB;                   // elements of a piece
     __shared__ __attribute__((aligned(1024))) uint8_t smem[C::SMEM];
     __shared__ int bt_lds[kTreePages];
-    __shared__ int scan_lds[C::NW + 2];
+    __shared__ int vote_lds[C::NW];
     __shared__ float2 ml_lds[C::NW * 32];
     __shared__ int odd_lds[C::NW];  // this wave took infinities or NaN out of V (2: on any key, 1: behind ctx)
     const TreeArgs& a = ka.a;
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rw = wave % RW, kg = wave / RW;
+    const int rw = wave % RW, gi = wave / RW, kg = gi % C::KW, hd = gi / C::KW;
     const int D = a.head_dim;
     const int logical = xcd_remap(blockIdx.x, gridDim.x);
     const int range = __builtin_amdgcn_readfirstlane((int)ka.row_blocks.div((uint32_t)logical));
     const int rb = logical - range * (int)ka.row_blocks.d;
+    const int units = a.kv_heads / HW;  // of a sequence
 
-    // ---- this workgroup's range of steps [pos, end), and the sequence that holds the first
+    // ---- this workgroup's range of steps [pos, end), and the sequence that holds the first; every wave
+    // for itself, without a barrier
     auto steps_of = [&](int i) {
-        return i < a.n_seqs ? a.kv_heads * ((tree_rows_of(a, i) + C::KT - 1) / C::KT) : 0;
+        return i < a.n_seqs ? units * ((tree_rows_of(a, i) + C::KT - 1) / C::KT) : 0;
     };
-    auto scan = [&](int v, int* sum) {  // inclusive over the workgroup
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(v, o, 64);
-            if (lane >= o) v += up;
-        }
-        __syncthreads();
-        if (lane == 63) scan_lds[wave] = v;
-        __syncthreads();
-        int all = 0, before = 0;
-#pragma unroll
-        for (int w = 0; w < C::NW; ++w) {
-            if (w == wave) before = all;
-            all += scan_lds[w];
-        }
-        *sum = all;
-        return v + before;
-    };
-    int sum0, total;
-    int mine = steps_of(tid);
-    int upto = scan(mine, &sum0);
-    total = sum0;
-    for (int base = NT; base < a.n_seqs; base += NT) {
-        int sum;
-        scan(steps_of(base + tid), &sum);
-        total += sum;
-    }
-    total = __builtin_amdgcn_readfirstlane(total);
+    int mine = steps_of(lane);
+    for (int i = lane + 64; i < a.n_seqs; i += 64) mine += steps_of(i);
+    const int total = __builtin_amdgcn_readlane(wave_scan(mine), 63);
     const int share = max(1, (int)ka.ranges.div((uint32_t)total + ka.ranges.d - 1));
     int64_t pos = (int64_t)range * share;
     const int64_t end = pos + share < total ? pos + share : total;
-    const bool plans = logical == 0;  // writes what tree_combine needs
-    if (pos >= end && !plans) return;
-    for (int base = 0, carry = 0; base < a.n_seqs; base += NT) {
-        int sum = sum0;
-        if (base > 0) {
-            mine = steps_of(base + tid);
-            upto = scan(mine, &sum);
-        }
-        if (plans && base + tid < a.n_seqs) a.plan[base + tid] = carry + upto - mine;
-        if (mine > 0 && carry + upto - mine <= pos && pos < carry + upto) {
-            scan_lds[C::NW] = base + tid;
-            scan_lds[C::NW + 1] = carry + upto - mine;
-        }
-        carry += sum;
-    }
-    if (plans && tid == 0) {
+    const bool plans = logical == 0 && wave == 0;  // writes what tree_combine needs
+    if (plans && lane == 0) {
         a.plan[a.n_seqs] = total;
         a.plan[a.n_seqs + 1] = share;
     }
+    int s = 0, first = 0;  // the sequence, its first step
+    bool found = pos >= end;
+    for (int base = 0, carry = 0; base < a.n_seqs && (plans || !found); base += 64) {
+        const int v = steps_of(base + lane);
+        const int upto = carry + wave_scan(v);
+        if (plans && base + lane < a.n_seqs) a.plan[base + lane] = upto - v;
+        const uint64_t past = __ballot(upto > pos);
+        if (!found && past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            s = base + l;
+            first = __builtin_amdgcn_readlane(upto - v, l);
+            found = true;
+        }
+        carry = __builtin_amdgcn_readlane(upto, 63);
+    }
     if (pos >= end) return;
+    s = __builtin_amdgcn_readfirstlane(s);
     if (lane == 0) odd_lds[wave] = 0;
-    __syncthreads();
-    int s = __builtin_amdgcn_readfirstlane(scan_lds[C::NW]);
-    int first = __builtin_amdgcn_readfirstlane(scan_lds[C::NW + 1]);  // first step of sequence s
 
     // ---- lane constants
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)smem;
-    const int group_base = kg * C::NST * C::STAGE;
+    const int group_base = gi * C::NST * C::STAGE;
     const int n16 = lane & 15;
     // K operand: row lane & 31, piece 2 c + h: the column's XOR takes c by itself
     const int kbase = group_base + (lane & 31) * C::ROWB +
@@ -273,12 +271,12 @@ void tree_split(TreeKArgs ka) {
         for (;; ++s) {
             rows_s = __builtin_amdgcn_readfirstlane(tree_rows_of(a, s));
             steps = (rows_s + C::KT - 1) / C::KT;
-            if (pos < (int64_t)first + (int64_t)steps * a.kv_heads) break;
-            first += steps * a.kv_heads;
+            if (pos < (int64_t)first + (int64_t)steps * units) break;
+            first += steps * units;
         }
         const int in_seq = (int)(pos - first);
-        const int kvh = __builtin_amdgcn_readfirstlane(in_seq / steps);
-        const int st0 = in_seq - kvh * steps;
+        const int unit = __builtin_amdgcn_readfirstlane(in_seq / steps), kvh = unit * HW + hd;
+        const int st0 = in_seq - unit * steps;
         const int st1 = (int)min((int64_t)steps, st0 + (end - pos));
         pos += st1 - st0;
         const int len = __builtin_amdgcn_readfirstlane(a.tree_lens[s]);
@@ -290,8 +288,12 @@ void tree_split(TreeKArgs ka) {
         const int row = r0 + rw * 32 + (lane & 31);
         const int t = ka.grp.div(row), hq = kvh * a.group + row - t * a.group;
         bool row_ok = row < rows_total;
+        const bool live = r0 + rw * 32 < rows_total;  // this wave has rows at all
         const int tok = s * a.max_tokens + t;
         int rope_pos = 0;
+        // the mask of a tree of up to 64 tokens: one word
+        uint64_t mask0 = 0;
+        if (row_ok && a.masks && a.words == 1) mask0 = a.masks[tok];
         if (row_ok && a.rope_table) {
             rope_pos = a.positions ? a.positions[tok] : ctx + t;
             row_ok = rope_pos >= 0 && rope_pos < a.rope_positions;
@@ -350,6 +352,7 @@ void tree_split(TreeKArgs ka) {
             }
         };
 
+        load_q();  // (ahead of the first transfers: behind them it waits for three tiles)
         f32x16_t oacc[MB];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
@@ -379,10 +382,10 @@ void tree_split(TreeKArgs ka) {
             // (a vote of its own: __syncthreads_or goes by the block's three dimensions, registers that
             // are missed later)
             bad = __any(bad);
-            if (lane == 0) scan_lds[wave] = bad;
+            if (lane == 0) vote_lds[wave] = bad;
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < C::NW; ++w) bad |= scan_lds[w] != 0;
+            for (int w = 0; w < C::NW; ++w) bad |= vote_lds[w] != 0;
             bad = __builtin_amdgcn_readfirstlane(bad);
 
             // ---- one tile of this wave's key group into a stage
@@ -459,8 +462,13 @@ void tree_split(TreeKArgs ka) {
                     if (a.masks) {
                         const uint64_t* const m = a.masks + (int64_t)tok * a.words;
                         const int at64 = j0 >= 0 ? j0 >> 6 : 0, sh = j0 & 63;
-                        const uint64_t w0 = row_ok && at64 < a.words ? m[at64] : 0;
-                        const uint64_t w1 = row_ok && j0 >= 0 && at64 + 1 < a.words ? m[at64 + 1] : 0;
+                        uint64_t w0 = mask0, w1 = 0;
+                        if (a.words > 1) {
+                            w0 = row_ok && at64 < a.words ? m[at64] : 0;
+                            w1 = row_ok && j0 >= 0 && at64 + 1 < a.words ? m[at64 + 1] : 0;
+                        } else if (at64 > 0) {
+                            w0 = 0;
+                        }
                         if (j0 >= 0) w = (w0 >> sh) | (sh ? w1 << (64 - sh) : 0);
                         else if (j0 > -32) w = w0 << -j0 | ((1u << -j0) - 1u);
                         else w = 0xffffffffu;
@@ -470,13 +478,13 @@ void tree_split(TreeKArgs ka) {
                     }
                     // keys past the live rows, and on pages that are not there
                     const int left = k_end - key0;
-                    uint32_t live = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+                    uint32_t there = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
                     if (bad) {
                         const int key = min(key0 + (lane & 31), k_end - 1);
                         const int lp = ka.ps.div(key);
-                        live &= (uint32_t)__ballot(bt_lds[lp - p0] >= 0);
+                        there &= (uint32_t)__ballot(bt_lds[lp - p0] >= 0);
                     }
-                    const uint32_t see = ((uint32_t)w & live) >> (4 * h);  // this row sees these keys
+                    const uint32_t see = ((uint32_t)w & there) >> (4 * h);  // this row sees these keys
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (!((see >> (8 * (i / 4) + i % 4)) & 1)) sc[i] = -INFINITY;
@@ -554,7 +562,6 @@ void tree_split(TreeKArgs ka) {
 #pragma unroll
             for (int i = 0; i < C::NST - 1; ++i)
                 if (c0 + i < c1) transfer(c0 + i, i * C::STAGE);
-            if (c0 == st0) load_q();
             int stage = 0;
             auto run = [&](int from, int to, auto masked_c) {
 #pragma unroll 1
@@ -572,58 +579,184 @@ void tree_split(TreeKArgs ka) {
                     const int tile = step * C::KT + kg * C::BN;
 #pragma unroll 1
                     for (int kb = 0; kb < C::BN; kb += 32)
-                        if (!decltype(masked_c)::value || tile + kb < k_end)
+                        if (live && (!decltype(masked_c)::value || tile + kb < k_end))
                             block(tile + kb, stage + kb * C::ROWB, masked_c);
                     stage = stage == (C::NST - 1) * C::STAGE ? 0 : stage + C::STAGE;
                 }
             };
+            // The same for blocks that every row sees, as a pipeline: Q.K^T of the next block is issued
+            // among the softmax of this one (the matrix core runs while the vector unit works), so a
+            // step's transfers have to be complete one step earlier.
+            auto run_pipe = [&](int from, int to) {
+                if constexpr (C::PIPE) {
+                f32x16_t sc;
+                const auto scores = [&](int at, f32x16_t& out) {
+                    const int ka0 = kbase + at;
+                    u32x4_t kf[KS];
+#pragma unroll
+                    for (int c = 0; c < KS; ++c) kf[c] = *(const u32x4_t*)(smem + (ka0 ^ (c << 5)));
+                    f32x16_t x;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < KS; ++c) {
+                        x = Half<T>::mfma32(kf[c], qop[c], x);
+                        if constexpr (SPLIT) x = Half<T>::mfma32(kf[c], qlo[c], x);
+                    }
+                    out = x;
+                };
+#pragma unroll 1
+                for (int step = from; step < to; ++step) {
+                    if (step + C::NST - 2 < c1 - 1) wait_vmcnt<(C::NST - 3) * 2 * C::NI>();
+                    else wait_dma();
+                    __syncthreads();
+                    const int ahead = stage == 0 ? (C::NST - 1) * C::STAGE : stage - C::STAGE;
+                    if (step + C::NST - 1 < c1) transfer(step + C::NST - 1, ahead);
+                    const int next = stage == (C::NST - 1) * C::STAGE ? 0 : stage + C::STAGE;
+                    if (live) {
+                        if (step == from) scores(stage, sc);
+#pragma unroll  // (two blocks: the scores change places without copies)
+                        for (int kb = 0; kb < C::BN; kb += 32) {
+                            const int at = stage + kb * C::ROWB;
+                            // (behind the last block of the run its own scores again, not used)
+                            const int at_next = kb + 32 < C::BN ? at + 32 * C::ROWB : step + 1 < to ? next : at;
+                            f32x16_t sn;
+                            scores(at_next, sn);
+                            u32x4_t vf[2][MB];  // (the second half is read after the first products)
+#pragma unroll
+                            for (int mb = 0; mb < MB; ++mb) vf[0][mb] = tree_v16<DPAD>(smem, vbase + at, 0, mb);
+                            float mt = sc[0];
+#pragma unroll
+                            for (int i = 1; i < 16; ++i) mt = fmaxf(mt, sc[i]);
+                            mt = fmaxf(mt, xor32(mt));
+                            const bool need = mt * c2 > m_run * c2 + 8.0f;
+                            const float m_use = need ? mt : m_run;
+                            const float neg = -m_use * c2;
+                            float ls = 0.0f;
+                            u32x4_t pb[2];
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const float p0 = fast_exp2(fmaf(sc[i], c2, neg));
+                                const float p1 = fast_exp2(fmaf(sc[i + 1], c2, neg));
+                                ls += p0 + p1;
+                                pb[i / 8][i % 8 / 2] = Half<T>::pack(p0, p1);
+                            }
+                            // (here, not behind the branch)
+                            asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(ls));
+                            // issue order: K reads, the maximum, then a product with some of the rest
+                            FA_SG(0x100, KS);
+                            FA_SG(0x402, 14);
+#pragma unroll
+                            for (int i = 0; i < (SPLIT ? 2 : 1) * KS; ++i) {
+                                FA_SG(0x008, 1);
+                                FA_SG(0x100, (SPLIT ? 2 : 4) * MB / KS);
+                                FA_SG(0x402, SPLIT ? 5 : 9);
+                            }
+                            if (__any(need)) {
+                                const float alpha = need ? fast_exp2((m_run - m_use) * c2) : 1.0f;
+                                l_run *= alpha;
+#pragma unroll
+                                for (int mb = 0; mb < MB; ++mb) oacc[mb] *= alpha;
+                                m_run = m_use;
+                            }
+                            l_run += ls;
+                            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int mb = 0; mb < MB; ++mb) vf[1][mb] = tree_v16<DPAD>(smem, vbase + at, 1, mb);
+#pragma unroll
+                            for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+                                for (int mb = 0; mb < MB; ++mb)
+                                    oacc[mb] = Half<T>::mfma32(vf[k2][mb], pb[k2], oacc[mb]);
+                            sc = sn;
+                        }
+                    }
+                    stage = next;
+                }
+                }
+            };
             const int cm = bad ? c0 : max(c0, min(c1, ctx / C::KT));
-            run(c0, cm, std::false_type{});
+            if constexpr (C::PIPE) run_pipe(c0, cm);
+            else run(c0, cm, std::false_type{});
             run(cm, c1, std::true_type{});
             c0 = c1;
         }
 
-        // ---- merge the key groups in LDS and write the rows
+        // ---- finished rows to O and LSE, partial ones to their slot: per 32-row block the quads (four
+        // dims of a row) in the order that the waves hold them, 1 KiB a store
         l_run += xor32(l_run);
+        if (!row_ok) l_run = 0.0f;  // (a token without a position has run with Q = 0: as if it saw nothing)
         int te = tid;
         asm volatile("" : "+v"(te));  // (no address is kept from unit to unit)
         const int le = te & 63, he = le >> 5;
-        // (a token without a position has run with Q = 0: as if it had seen nothing)
-        if (he == 0) ml_lds[wave * 32 + (le & 31)] = make_float2(m_run, row_ok ? l_run : 0.0f);
-        __syncthreads();  // (every stage has been read)
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *(f32x4_t*)(smem + (wave * 32 + (le & 31)) * C::MROW + (32 * mb + 8 * i + 4 * he) * 4) =
-                    f32x4_t{oacc[mb][4 * i], oacc[mb][4 * i + 1], oacc[mb][4 * i + 2], oacc[mb][4 * i + 3]};
-        __syncthreads();
         const bool whole = st0 == 0 && st1 == steps;
         const int64_t slot = 2 * ((int64_t)range * ka.row_blocks.d + rb) + (st0 == 0 ? 1 : 0);
-        constexpr int LPR = DPAD / 4;  // threads a row, four dims each
-        for (int i = te; i < C::ROWS * LPR; i += NT) {
-            const int r = i / LPR, d = 4 * (i % LPR);
-            if (r0 + r >= rows_total || d >= D) continue;
-            float M = -INFINITY, L = 0.0f;
+        if constexpr (C::KW == 1) {
+            const int64_t blk = (slot * HW + hd) * RW + rw;
+            if (live && whole) {
+                if (row < rows_total) {
 #pragma unroll
-            for (int g = 0; g < C::KW; ++g) M = fmaxf(M, ml_lds[g * C::ROWS + r].x);
-            f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+                    for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-            for (int g = 0; g < C::KW; ++g) {
-                const float2 ml = ml_lds[g * C::ROWS + r];
-                if (ml.y == 0.0f) continue;  // (saw nothing)
-                const float w = fast_exp2((ml.x - M) * c2);
-                const f32x4_t x = *(const f32x4_t*)(smem + (g * C::ROWS + r) * C::MROW + 4 * d);
-                L = fmaf(ml.y, w, L);
+                        for (int i = 0; i < 4; ++i) {
+                            const int d = 32 * mb + 8 * i + 4 * he;
+                            if (d < D)
+                                write_row4<T>(a, s, kvh, row, d,
+                                              f32x4_t{oacc[mb][4 * i], oacc[mb][4 * i + 1],
+                                                      oacc[mb][4 * i + 2], oacc[mb][4 * i + 3]},
+                                              m_run, l_run, ka.grp);
+                        }
+                }
+            } else if (live) {
+                f32x4_t* const to = (f32x4_t*)a.part_o + blk * C::QUADS + le;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], w, o[j]);
+                for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        to[(4 * mb + i) * 64] = f32x4_t{oacc[mb][4 * i], oacc[mb][4 * i + 1],
+                                                        oacc[mb][4 * i + 2], oacc[mb][4 * i + 3]};
+                if (he == 0) a.part_ml[blk * 32 + le] = make_float2(m_run, l_run);
             }
-            if (!whole) {
-                *(f32x4_t*)(a.part_o + (slot * C::ROWS + r) * D + d) = o;
-                if (d == 0) a.part_ml[slot * C::ROWS + r] = make_float2(M, L);
-                continue;
+        } else {  // the key groups are merged in LDS
+            if (he == 0) ml_lds[wave * 32 + le] = make_float2(m_run, l_run);
+            __syncthreads();  // (every stage has been read)
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *(f32x4_t*)(smem + (wave * 32 + (le & 31)) * C::MROW + (32 * mb + 8 * i + 4 * he) * 4) =
+                        f32x4_t{oacc[mb][4 * i], oacc[mb][4 * i + 1], oacc[mb][4 * i + 2],
+                                oacc[mb][4 * i + 3]};
+            __syncthreads();
+            for (int i = te; i < HW * RW * C::QUADS; i += NT) {
+                const int blk = i / C::QUADS, q = i % C::QUADS;  // block = head * RW + row block
+                const int r = q & 31, d = q / 64 * 8 + 4 * ((q >> 5) & 1);
+                const int rr = blk % RW * 32 + r, hh = blk / RW;
+                if (r0 + rr >= rows_total || d >= D) continue;
+                float M = -INFINITY, L = 0.0f;
+                const int g0 = hh * C::KW;
+#pragma unroll
+                for (int g = 0; g < C::KW; ++g) M = fmaxf(M, ml_lds[(g0 + g) * C::ROWS + rr].x);
+                f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int g = 0; g < C::KW; ++g) {
+                    const float2 ml = ml_lds[(g0 + g) * C::ROWS + rr];
+                    if (ml.y == 0.0f) continue;  // (saw nothing)
+                    const float w = fast_exp2((ml.x - M) * c2);
+                    const f32x4_t x =
+                        *(const f32x4_t*)(smem + ((g0 + g) * C::ROWS + rr) * C::MROW + 4 * d);
+                    L = fmaf(ml.y, w, L);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], w, o[j]);
+                }
+                if (whole) {
+                    write_row4<T>(a, s, unit * HW + hh, r0 + rr, d, o, M, L, ka.grp);
+                } else {
+                    const int64_t b = slot * (HW * RW) + blk;
+                    ((f32x4_t*)a.part_o)[b * C::QUADS + q] = o;
+                    if (d == 0) a.part_ml[b * 32 + r] = make_float2(M, L);
+                }
             }
-            write_row4<T>(a, s, kvh, r0 + r, d, o, M, L, ka.grp);
         }
     }
     __syncthreads();
@@ -635,183 +768,228 @@ void tree_split(TreeKArgs ka) {
     }
 }
 
-// Merges the partials of the units that several ranges share, and writes the rows past each tree. A wave
-// takes 64 / LPR rows at a time, LPR lanes (four dims each) a row; the partials of a row in their order.
-template <typename T, int LPR>
-__global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rows_block) {
+// Merges the partials of the units that several ranges share, and writes the rows past each tree. One
+// workgroup per 32 rows of a (sequence, kv head): a thread has one row and a quad of dims in each
+// 32 / (DPAD / 32) of it, and merges its partials in their order, several loads ahead.
+template <typename T, int DPAD>
+__global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rw, int hw, int blocks) {
     const TreeArgs& a = ka.a;
-    const int rows_seq = a.max_tokens * a.q_heads;
-    const int64_t i = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    const int s = (int)(i / rows_seq);
-    if (s >= a.n_seqs) return;
-    const int d = 4 * (threadIdx.x % LPR), D = a.head_dim;
-    const int in = (int)(i - (int64_t)s * rows_seq);
-    const int per = a.max_tokens * a.group;
-    const int kvh = in / per, row = in - kvh * per;
-    if (d >= D) return;
+    constexpr int N = DPAD / 32;  // quads of a thread
+    const int D = a.head_dim, tid = threadIdx.x;
+    const int b32 = blockIdx.x % blocks, sh = blockIdx.x / blocks;
+    const int kvh = sh % a.kv_heads, s = sh / a.kv_heads;
+    const int row = b32 * 32 + (tid & 31), rows_all = a.max_tokens * a.group;
     const int rows_s = tree_rows_of(a, s);
     const int len = rows_s ? a.tree_lens[s] : 0;
+    const int d0 = 8 * (tid >> 6) + 4 * ((tid >> 5) & 1);  // dims d0 + 32 n .. + 3
     const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-    if (row >= len * a.group) {
-        write_row4<T>(a, s, kvh, row, d, zero, -INFINITY, 0.0f, ka.grp);
-        return;
+    if (row < rows_all && row >= len * a.group) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (d0 + 32 * n < D) write_row4<T>(a, s, kvh, row, d0 + 32 * n, zero, 0.0f, 0.0f, ka.grp);
     }
+    if (b32 * 32 >= len * a.group) return;
     const int share = a.plan[a.n_seqs + 1];
     const int steps = (rows_s + kt - 1) / kt;
-    const uint32_t u0 = (uint32_t)a.plan[s] + (uint32_t)kvh * (uint32_t)steps;
+    const uint32_t u0 = (uint32_t)a.plan[s] + (uint32_t)(kvh / hw) * (uint32_t)steps;
     const int g0 = (int)(u0 / (uint32_t)share), g1 = (int)((u0 + steps - 1) / (uint32_t)share);
-    const int rb = row / rows_block, r = row - rb * rows_block;
+    const int rb = b32 / rw, in = b32 - rb * rw;
+    const int nrb = (int)ka.row_blocks.d;
     const float c2 = a.scale * kLog2e;
     int odd = 0;
-    if (g0 == g1) {
-        odd = a.odd[(int64_t)g0 * ka.row_blocks.d + rb];
-        if (!odd) return;  // finished by the range that covers it
-    }
     float M = -INFINITY, L = 0.0f;
-    f32x4_t o = zero;
-    if (g0 < g1)
-        for (int g = g0; g <= g1; ++g) {
-            const int64_t slot = 2 * ((int64_t)g * ka.row_blocks.d + rb) + (g == g0 ? 1 : 0);
-            const float2 ml = a.part_ml[slot * rows_block + r];
-            const f32x4_t x = *(const f32x4_t*)(a.part_o + (slot * rows_block + r) * D + d);
-            odd = max(odd, a.odd[(int64_t)g * ka.row_blocks.d + rb]);
-            if (ml.y == 0.0f) continue;
-            const float mx = fmaxf(M, ml.x);
-            const float w0 = L == 0.0f ? 0.0f : fast_exp2((M - mx) * c2);
-            const float w1 = fast_exp2((ml.x - mx) * c2);
-            M = mx;
-            L = fmaf(ml.y, w1, L * w0);
+    f32x4_t o[N];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], w1, o[j] * w0);
+    for (int n = 0; n < N; ++n) o[n] = zero;
+    if (g0 == g1) {
+        odd = a.odd[g0 * nrb + rb];
+        if (!odd) return;  // finished by the range that covers it
+    } else {
+        constexpr int UN = 4;
+        for (int g = g0; g <= g1; g += UN) {
+            float2 ml[UN];
+            f32x4_t x[UN][N];
+            int od[UN];
+#pragma unroll
+            for (int i = 0; i < UN; ++i) {  // (past the end: the last partial again, not counted)
+                const int at = min(g + i, g1);
+                const int64_t blk = ((2 * ((int64_t)at * nrb + rb) + (at == g0 ? 1 : 0)) * hw + kvh % hw) * rw + in;
+                od[i] = a.odd[at * nrb + rb];
+                ml[i] = a.part_ml[blk * 32 + (tid & 31)];
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    x[i][n] = ((const f32x4_t*)a.part_o)[blk * (8 * DPAD) + n * 256 + tid];
+            }
+#pragma unroll
+            for (int i = 0; i < UN; ++i) {
+                odd = max(odd, od[i]);
+                if (g + i > g1 || ml[i].y == 0.0f) continue;
+                const float mx = fmaxf(M, ml[i].x);
+                const float w0 = L == 0.0f ? 0.0f : fast_exp2((M - mx) * c2);
+                const float w1 = fast_exp2((ml[i].x - mx) * c2);
+                M = mx;
+                L = fmaf(ml[i].y, w1, L * w0);
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[n][j] = fmaf(x[i][n][j], w1, o[n][j] * w0);
+            }
         }
-    if (!odd) {
-        write_row4<T>(a, s, kvh, row, d, o, M, L, ka.grp);
-        return;
     }
+    if (row >= len * a.group) return;
+    if (g0 < g1) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (d0 + 32 * n < D) write_row4<T>(a, s, kvh, row, d0 + 32 * n, o[n], M, L, ka.grp);
+    }
+    if (!odd) return;
     // ---- V held infinities or NaN where rows do not see every key: the values that this row sees
     const int ctx = rows_s - len, t = ka.grp.div(row);
     const int hq = kvh * a.group + row - t * a.group;
-    if (g0 == g1) {
-        L = a.lse[((int64_t)s * a.q_heads + hq) * a.max_tokens + t] == -INFINITY ? 0.0f : 1.0f;
-    } else {
-        write_row4<T>(a, s, kvh, row, d, o, M, L, ka.grp);
-    }
+    if (g0 == g1) L = a.lse[((int64_t)s * a.q_heads + hq) * a.max_tokens + t] == -INFINITY ? 0.0f : 1.0f;
     if (L == 0.0f) return;  // (sees nothing)
-    f32x4_t add = zero;
-    for (int key = odd > 1 ? 0 : ctx / kt * kt; key < rows_s; ++key) {
-        const int j = key - ctx;
-        const bool seen = j < 0 ? true
-                          : a.masks
-                              ? (a.masks[((int64_t)s * a.max_tokens + t) * a.words + (j >> 6)] >> (j & 63)) & 1
-                              : j <= t;
-        if (!seen) continue;
-        const int lp = ka.ps.div(key), page = a.block_tables[(int64_t)s * a.max_pages + lp];
-        if ((unsigned)page >= (unsigned)a.physical_pages) continue;
-        const int64_t at = (((int64_t)page * a.page_size + key - lp * a.page_size) * a.kv_heads + kvh) * D + d;
+#pragma unroll 1
+    for (int n = 0; n < N; ++n) {
+        const int d = d0 + 32 * n;
+        if (d >= D) break;
+        f32x4_t add = zero;
+        for (int key = odd > 1 ? 0 : ctx / kt * kt; key < rows_s; ++key) {
+            const int j = key - ctx;
+            const bool seen = j < 0 ? true
+                              : a.masks
+                                  ? (a.masks[((int64_t)s * a.max_tokens + t) * a.words + (j >> 6)] >> (j & 63)) & 1
+                                  : j <= t;
+            if (!seen) continue;
+            const int lp = ka.ps.div(key), page = a.block_tables[(int64_t)s * a.max_pages + lp];
+            if ((unsigned)page >= (unsigned)a.physical_pages) continue;
+            const int64_t at =
+                (((int64_t)page * a.page_size + key - lp * a.page_size) * a.kv_heads + kvh) * D + d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float v;
+                if constexpr (std::is_same<T, float>::value) v = ((const float*)a.v_pool)[at + e];
+                else v = Half<T>::lo(((const uint16_t*)a.v_pool)[at + e]);
+                if (!(fabsf(v) < INFINITY)) add[e] += v;
+            }
+        }
+        const int64_t to = (((int64_t)s * a.max_tokens + t) * a.q_heads + hq) * D + d;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float v;
-            if constexpr (std::is_same<T, float>::value) v = ((const float*)a.v_pool)[at + e];
-            else v = Half<T>::lo(((const uint16_t*)a.v_pool)[at + e]);
-            if (!(fabsf(v) < INFINITY)) add[e] += v;
+            if (add[e] == 0.0f) continue;
+            if constexpr (std::is_same<T, float>::value) ((float*)a.o)[to + e] += add[e];
+            else
+                ((uint16_t*)a.o)[to + e] = (uint16_t)Half<T>::pack(
+                    Half<T>::lo(((const uint16_t*)a.o)[to + e]) + add[e], 0.0f);
         }
     }
-    const int64_t to = (((int64_t)s * a.max_tokens + t) * a.q_heads + hq) * D + d;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (add[e] == 0.0f) continue;
-        if constexpr (std::is_same<T, float>::value) ((float*)a.o)[to + e] += add[e];
-        else
-            ((uint16_t*)a.o)[to + e] = (uint16_t)Half<T>::pack(
-                Half<T>::lo(((const uint16_t*)a.o)[to + e]) + add[e], 0.0f);
-    }
 }
 
-// Rows of a workgroup: as few row blocks of 32 as hold every row of a (sequence, kv head), at most 4;
-// the waves left over are key groups.
-static int tree_row_waves(Dtype dt, const TreeArgs& a) {
+// The shape of a launch. Rows: as few row blocks of 32 as hold every row of a (sequence, kv head), at
+// most 8 (f32: 4). Waves left over take kv heads side by side, whose rows of a token lie next to each
+// other in memory, or key groups where the head count does not divide.
+struct TreeShape {
+    int rw, hw, kt, row_blocks, ranges, threads;
+};
+template <typename T, int DPAD, int RW, int HW>
+static TreeShape shape_of(const TreeArgs& a) {
+    using C = TreeCfg<T, DPAD, RW, HW>;
+    TreeShape s;
+    s.rw = RW;
+    s.hw = HW;
+    s.kt = C::KT;
+    s.row_blocks = (a.max_tokens * a.group + C::ROWS - 1) / C::ROWS;
+    // one round of workgroups: as many a CU as LDS and registers hold
+    const int per_cu = C::NW == 8 || C::SMEM > 72 * 1024 || C::WAVES * 4 / C::NW < 2 ? 1 : 2;
+    s.ranges = std::max(1, per_cu * device_cus() / s.row_blocks);
+    s.threads = 64 * C::NW;
+    return s;
+}
+// Calls f with the row waves and heads of a launch as constants.
+template <typename T, typename F>
+static auto tree_dispatch(const TreeArgs& a, F f) {
+    using std::integral_constant;
+    constexpr bool F32 = std::is_same<T, float>::value;
     const int rows = a.max_tokens * a.group;
-    return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || dt == Dtype::F32 ? 4 : 8;
+    auto go = [&](auto dpad) {
+        constexpr int DP = decltype(dpad)::value;
+        auto run = [&](auto rw, auto hw) { return f(integral_constant<int, DP>{}, rw, hw); };
+        using One = integral_constant<int, 1>;
+        using Two = integral_constant<int, 2>;
+        using Four = integral_constant<int, 4>;
+        if (rows <= 32) {
+            if constexpr (!F32)
+                if (a.kv_heads % 4 == 0) return run(One{}, Four{});
+            return a.kv_heads % 2 == 0 ? run(One{}, Two{}) : run(One{}, One{});
+        }
+        if (rows <= 64) {
+            if constexpr (!F32)
+                if (a.kv_heads % 2 == 0) return run(Two{}, Two{});
+            return run(Two{}, One{});
+        }
+        if constexpr (!F32)
+            if (rows > 128) return run(integral_constant<int, 8>{}, One{});
+        return run(Four{}, One{});
+    };
+    return a.head_dim <= 64 ? go(integral_constant<int, 64>{}) : go(integral_constant<int, 128>{});
 }
-
-// Key ranges of the launch: one round of workgroups, one or (64 to 128 rows) two a CU.
-static void tree_shape(Dtype dt, const TreeArgs& a, int* ranges, int* row_blocks) {
-    const int rw = tree_row_waves(dt, a), rows = 32 * rw;
-    *row_blocks = (a.max_tokens * a.group + rows - 1) / rows;
-    *ranges = std::max(1, (rw == 2 || rw == 4 ? 2 : 1) * device_cus() / *row_blocks);
+template <typename T>
+static TreeShape shape_t(const TreeArgs& a) {
+    return tree_dispatch<T>(a, [&](auto dpad, auto rw, auto hw) {
+        return shape_of<T, decltype(dpad)::value, decltype(rw)::value, decltype(hw)::value>(a);
+    });
+}
+static TreeShape tree_shape(Dtype dt, const TreeArgs& a) {
+    return dt == Dtype::F32 ? shape_t<float>(a) : shape_t<bf16_t>(a);  // (the 16-bit types alike)
 }
 
 size_t tree_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset,
                       size_t* odd_offset) {
-    int ranges, row_blocks;
-    tree_shape(dt, a, &ranges, &row_blocks);
-    const size_t rows = (size_t)2 * ranges * row_blocks * 32 * tree_row_waves(dt, a);
-    *ml_offset = rows * a.head_dim * 4;
+    const TreeShape s = tree_shape(dt, a);
+    const size_t rows = (size_t)2 * s.ranges * s.row_blocks * 32 * s.rw * s.hw;
+    *ml_offset = rows * (a.head_dim <= 64 ? 64 : 128) * 4;
     *plan_offset = *ml_offset + rows * 8;
     *odd_offset = *plan_offset + ((size_t)a.n_seqs + 2) * 4;
-    return *odd_offset + (size_t)ranges * row_blocks * 4;
-}
-
-template <typename T, int DPAD, int RW>
-static void launch_rw(const TreeKArgs& ka, hipStream_t s, unsigned wgs) {
-    using C = TreeCfg<T, DPAD, RW>;
-    if constexpr (!C::F32) {
-        if (ka.a.rope_table) {
-            tree_split<T, DPAD, RW, true><<<wgs, 64 * C::NW, 0, s>>>(ka);
-            return;
-        }
-    }
-    tree_split<T, DPAD, RW, false><<<wgs, 64 * C::NW, 0, s>>>(ka);
-}
-
-template <typename T, int DPAD>
-static void launch_t(const TreeKArgs& ka, hipStream_t s, unsigned grid[3], unsigned* block,
-                     void (*between)(void*), void* user) {
-    const TreeArgs& a = ka.a;
-    grid[0] = (unsigned)(ka.ranges.d * ka.row_blocks.d);
-    grid[1] = grid[2] = 1;
-    constexpr Dtype dt = std::is_same<T, float>::value ? Dtype::F32 : Dtype::BF16;  // (16-bit: alike)
-    const int rw = tree_row_waves(dt, a);
-    int kt = 0;
-    auto run = [&](auto waves) {
-        constexpr int RW = decltype(waves)::value;
-        launch_rw<T, DPAD, RW>(ka, s, grid[0]);
-        kt = TreeCfg<T, DPAD, RW>::KT;
-        *block = 64 * TreeCfg<T, DPAD, RW>::NW;
-    };
-    if (rw == 1) run(std::integral_constant<int, 1>{});
-    else if (rw == 2) run(std::integral_constant<int, 2>{});
-    else if (rw == 4) run(std::integral_constant<int, 4>{});
-    else if constexpr (dt != Dtype::F32) run(std::integral_constant<int, 8>{});
-    if (between) between(user);
-    constexpr int LPR = DPAD / 4;
-    const int64_t rows = (int64_t)a.n_seqs * a.max_tokens * a.q_heads;
-    const unsigned g = (unsigned)((rows + 256 / LPR - 1) / (256 / LPR));
-    tree_combine<T, LPR><<<g, 256, 0, s>>>(ka, kt, 32 * rw);
+    return *odd_offset + (size_t)s.ranges * s.row_blocks * 4;
 }
 
 template <typename T>
-static void launch_d(const TreeKArgs& ka, hipStream_t s, unsigned grid[3], unsigned* block,
+static void launch_t(TreeKArgs& ka, hipStream_t st, unsigned grid[3], unsigned* block, unsigned* rows,
                      void (*between)(void*), void* user) {
-    if (ka.a.head_dim <= 64) launch_t<T, 64>(ka, s, grid, block, between, user);
-    else launch_t<T, 128>(ka, s, grid, block, between, user);
+    const TreeArgs& a = ka.a;
+    const TreeShape s = shape_t<T>(a);
+    ka.ranges = FastDiv((uint32_t)s.ranges);
+    ka.row_blocks = FastDiv((uint32_t)s.row_blocks);
+    grid[0] = (unsigned)(s.ranges * s.row_blocks);
+    grid[1] = grid[2] = 1;
+    *block = (unsigned)s.threads;
+    *rows = (unsigned)(32 * s.rw);
+    tree_dispatch<T>(a, [&](auto dpad, auto rw, auto hw) {
+        constexpr int DP = decltype(dpad)::value, RW = decltype(rw)::value, HW = decltype(hw)::value;
+        if constexpr (!std::is_same<T, float>::value) {
+            if (a.rope_table) {
+                tree_split<T, DP, RW, HW, true><<<grid[0], s.threads, 0, st>>>(ka);
+                return;
+            }
+        }
+        tree_split<T, DP, RW, HW, false><<<grid[0], s.threads, 0, st>>>(ka);
+    });
+    if (between) between(user);
+    const int blocks = (a.max_tokens * a.group + 31) / 32;
+    const unsigned g = (unsigned)((int64_t)a.n_seqs * a.kv_heads * blocks);
+    if (a.head_dim <= 64) tree_combine<T, 64><<<g, 256, 0, st>>>(ka, s.kt, s.rw, s.hw, blocks);
+    else tree_combine<T, 128><<<g, 256, 0, st>>>(ka, s.kt, s.rw, s.hw, blocks);
 }
 
 void launch_tree_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned grid[3],
                            unsigned* block, unsigned* rows, void (*between)(void*), void* user) {
     TreeKArgs ka;
     ka.a = a;
-    int ranges, row_blocks;
-    tree_shape(dt, a, &ranges, &row_blocks);
     ka.ps = SmallDiv((uint32_t)a.page_size);
     ka.grp = SmallDiv((uint32_t)a.group);
-    ka.ranges = FastDiv((uint32_t)ranges);
-    ka.row_blocks = FastDiv((uint32_t)row_blocks);
-    *rows = (unsigned)(32 * tree_row_waves(dt, a));
     switch (dt) {
-        case Dtype::BF16: launch_d<bf16_t>(ka, s, grid, block, between, user); break;
-        case Dtype::F16: launch_d<f16_t>(ka, s, grid, block, between, user); break;
-        default: launch_d<float>(ka, s, grid, block, between, user); break;
+        case Dtype::BF16: launch_t<bf16_t>(ka, s, grid, block, rows, between, user); break;
+        case Dtype::F16: launch_t<f16_t>(ka, s, grid, block, rows, between, user); break;
+        default: launch_t<float>(ka, s, grid, block, rows, between, user); break;
     }
 }
 
