@@ -209,11 +209,10 @@ void tree_split(TreeKArgs ka) {
 
     // ---- this workgroup's range of steps [pos, end), and the sequence that holds the first; every wave
     // for itself, without a barrier
-    auto steps_of = [&](int i) {
-        return i < a.n_seqs ? units * ((tree_rows_of(a, i) + C::KT - 1) / C::KT) : 0;
-    };
-    int mine = steps_of(lane);
-    for (int i = lane + 64; i < a.n_seqs; i += 64) mine += steps_of(i);
+    auto steps_of = [&](int rows) { return units * ((rows + C::KT - 1) / C::KT); };
+    auto rows_of = [&](int i) { return i < a.n_seqs ? tree_rows_of(a, i) : 0; };
+    int mine = steps_of(rows_of(lane));
+    for (int i = lane + 64; i < a.n_seqs; i += 64) mine += steps_of(rows_of(i));
     const int total = __builtin_amdgcn_readlane(wave_scan(mine), 63);
     const int share = max(1, (int)ka.ranges.div((uint32_t)total + ka.ranges.d - 1));
     int64_t pos = (int64_t)range * share;
@@ -223,10 +222,10 @@ void tree_split(TreeKArgs ka) {
         a.plan[a.n_seqs] = total;
         a.plan[a.n_seqs + 1] = share;
     }
-    int s = 0, first = 0;  // the sequence, its first step
+    int s = 0, first = 0, rows_s = 0, len = 0;  // the sequence, its first step, its rows, the drafted ones
     bool found = pos >= end;
     for (int base = 0, carry = 0; base < a.n_seqs && (plans || !found); base += 64) {
-        const int v = steps_of(base + lane);
+        const int rows = rows_of(base + lane), v = steps_of(rows);
         const int upto = carry + wave_scan(v);
         if (plans && base + lane < a.n_seqs) a.plan[base + lane] = upto - v;
         const uint64_t past = __ballot(upto > pos);
@@ -234,6 +233,8 @@ void tree_split(TreeKArgs ka) {
             const int l = __ffsll((unsigned long long)past) - 1;
             s = base + l;
             first = __builtin_amdgcn_readlane(upto - v, l);
+            rows_s = __builtin_amdgcn_readlane(rows, l);
+            len = __builtin_amdgcn_readlane(a.tree_lens[min(base + lane, a.n_seqs - 1)], l);
             found = true;
         }
         carry = __builtin_amdgcn_readlane(upto, 63);
@@ -267,26 +268,25 @@ void tree_split(TreeKArgs ka) {
 
     while (pos < end) {
         // ---- the unit that holds step pos and this range's part of it
-        int rows_s = 0, steps = 0;
-        for (;; ++s) {
+        while (pos >= (int64_t)first + steps_of(rows_s)) {
+            first += steps_of(rows_s);
+            ++s;
             rows_s = __builtin_amdgcn_readfirstlane(tree_rows_of(a, s));
-            steps = (rows_s + C::KT - 1) / C::KT;
-            if (pos < (int64_t)first + (int64_t)steps * units) break;
-            first += steps * units;
+            len = __builtin_amdgcn_readfirstlane(a.tree_lens[s]);
         }
+        const int steps = (rows_s + C::KT - 1) / C::KT;
         const int in_seq = (int)(pos - first);
         const int unit = __builtin_amdgcn_readfirstlane(in_seq / steps), kvh = unit * HW + hd;
         const int st0 = in_seq - unit * steps;
         const int st1 = (int)min((int64_t)steps, st0 + (end - pos));
         pos += st1 - st0;
-        const int len = __builtin_amdgcn_readfirstlane(a.tree_lens[s]);
         const int ctx = rows_s - len;
         const int rows_total = len * a.group, r0 = rb * C::ROWS;
         if (r0 >= rows_total) continue;
 
         // ---- this lane's query row
         const int row = r0 + rw * 32 + (lane & 31);
-        const int t = ka.grp.div(row), hq = kvh * a.group + row - t * a.group;
+        const int t = ka.grp.div(row);
         bool row_ok = row < rows_total;
         const bool live = r0 + rw * 32 < rows_total;  // this wave has rows at all
         const int tok = s * a.max_tokens + t;
@@ -352,7 +352,7 @@ void tree_split(TreeKArgs ka) {
             }
         };
 
-        load_q();  // (ahead of the first transfers: behind them it waits for three tiles)
+        load_q();  // (ahead of the first transfers: behind them it waits for their tiles)
         f32x16_t oacc[MB];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
@@ -768,20 +768,31 @@ void tree_split(TreeKArgs ka) {
     }
 }
 
-// Merges the partials of the units that several ranges share, and writes the rows past each tree. One
-// workgroup per 32 rows of a (sequence, kv head): a thread has one row and a quad of dims in each
-// 32 / (DPAD / 32) of it, and merges its partials in their order, several loads ahead.
-template <typename T, int DPAD>
+// Merges the partials of the units that several ranges share, and writes the rows past each tree. A
+// thread ends with one row and a quad of dims in each of N 32-dim blocks.
+// Not WIDE: a workgroup per 32 rows of a (sequence, kv head), which merges their partials in their order,
+// several loads ahead. WIDE: one per 32 dims of those; its waves take every fourth partial each and are
+// merged in LDS, in their order.
+template <typename T, int DPAD, bool WIDE>
 __global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rw, int hw, int blocks) {
     const TreeArgs& a = ka.a;
-    constexpr int N = DPAD / 32;  // quads of a thread
-    const int D = a.head_dim, tid = threadIdx.x;
-    const int b32 = blockIdx.x % blocks, sh = blockIdx.x / blocks;
+    constexpr int N = WIDE ? 1 : DPAD / 32;
+    constexpr int NQ = WIDE ? 4 : N;      // quads of a thread while merging
+    constexpr int UN = 4;                 // partials on their way
+    constexpr int STEP = WIDE ? 4 : 1;
+    const int D = a.head_dim, tid = threadIdx.x, wave = tid >> 6;
+    int id = blockIdx.x, mb0 = 0;
+    if constexpr (WIDE) {
+        mb0 = id % (DPAD / 32);
+        id /= DPAD / 32;
+    }
+    const int b32 = id % blocks, sh = id / blocks;
     const int kvh = sh % a.kv_heads, s = sh / a.kv_heads;
     const int row = b32 * 32 + (tid & 31), rows_all = a.max_tokens * a.group;
+    const int share = a.plan[a.n_seqs + 1], before = a.plan[s];  // (asked for with the lengths)
     const int rows_s = tree_rows_of(a, s);
     const int len = rows_s ? a.tree_lens[s] : 0;
-    const int d0 = 8 * (tid >> 6) + 4 * ((tid >> 5) & 1);  // dims d0 + 32 n .. + 3
+    const int d0 = 32 * mb0 + 8 * wave + 4 * ((tid >> 5) & 1);  // dims d0 + 32 n .. + 3
     const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
     if (row < rows_all && row >= len * a.group) {
 #pragma unroll
@@ -789,50 +800,74 @@ __global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rw
             if (d0 + 32 * n < D) write_row4<T>(a, s, kvh, row, d0 + 32 * n, zero, 0.0f, 0.0f, ka.grp);
     }
     if (b32 * 32 >= len * a.group) return;
-    const int share = a.plan[a.n_seqs + 1];
     const int steps = (rows_s + kt - 1) / kt;
-    const uint32_t u0 = (uint32_t)a.plan[s] + (uint32_t)(kvh / hw) * (uint32_t)steps;
+    const uint32_t u0 = (uint32_t)before + (uint32_t)(kvh / hw) * (uint32_t)steps;
     const int g0 = (int)(u0 / (uint32_t)share), g1 = (int)((u0 + steps - 1) / (uint32_t)share);
     const int rb = b32 / rw, in = b32 - rb * rw;
     const int nrb = (int)ka.row_blocks.d;
     const float c2 = a.scale * kLog2e;
     int odd = 0;
     float M = -INFINITY, L = 0.0f;
-    f32x4_t o[N];
+    f32x4_t o[NQ];
 #pragma unroll
-    for (int n = 0; n < N; ++n) o[n] = zero;
+    for (int n = 0; n < NQ; ++n) o[n] = zero;
+    // another part (m, l, x) into (M, L, o); l = 0: it saw nothing
+    const auto merge = [&](float2 ml, const f32x4_t (&x)[NQ]) {
+        if (ml.y == 0.0f) return;
+        const float mx = fmaxf(M, ml.x);
+        const float w0 = L == 0.0f ? 0.0f : fast_exp2((M - mx) * c2);
+        const float w1 = fast_exp2((ml.x - mx) * c2);
+        M = mx;
+        L = fmaf(ml.y, w1, L * w0);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][j] = fmaf(x[n][j], w1, o[n][j] * w0);
+    };
     if (g0 == g1) {
         odd = a.odd[g0 * nrb + rb];
         if (!odd) return;  // finished by the range that covers it
     } else {
-        constexpr int UN = 4;
-        for (int g = g0; g <= g1; g += UN) {
+        for (int g = g0 + (WIDE ? wave : 0); g <= g1; g += UN * STEP) {
             float2 ml[UN];
-            f32x4_t x[UN][N];
+            f32x4_t x[UN][NQ];
             int od[UN];
 #pragma unroll
             for (int i = 0; i < UN; ++i) {  // (past the end: the last partial again, not counted)
-                const int at = min(g + i, g1);
+                const int at = min(g + i * STEP, g1);
                 const int64_t blk = ((2 * ((int64_t)at * nrb + rb) + (at == g0 ? 1 : 0)) * hw + kvh % hw) * rw + in;
+                const f32x4_t* const from = (const f32x4_t*)a.part_o + blk * (8 * DPAD);
                 od[i] = a.odd[at * nrb + rb];
                 ml[i] = a.part_ml[blk * 32 + (tid & 31)];
 #pragma unroll
-                for (int n = 0; n < N; ++n)
-                    x[i][n] = ((const f32x4_t*)a.part_o)[blk * (8 * DPAD) + n * 256 + tid];
+                for (int n = 0; n < NQ; ++n)
+                    x[i][n] = WIDE ? from[(4 * mb0 + n) * 64 + (tid & 63)] : from[n * 256 + tid];
             }
 #pragma unroll
             for (int i = 0; i < UN; ++i) {
                 odd = max(odd, od[i]);
-                if (g + i > g1 || ml[i].y == 0.0f) continue;
-                const float mx = fmaxf(M, ml[i].x);
-                const float w0 = L == 0.0f ? 0.0f : fast_exp2((M - mx) * c2);
-                const float w1 = fast_exp2((ml[i].x - mx) * c2);
-                M = mx;
-                L = fmaf(ml[i].y, w1, L * w0);
+                if (g + i * STEP <= g1) merge(ml[i], x[i]);
+            }
+        }
+        if constexpr (WIDE) {
+            __shared__ f32x4_t o_lds[4][NQ][64];
+            __shared__ float2 ml_lds[4][32];
+            __shared__ int odd_lds[4];
+            if ((tid & 63) < 32) ml_lds[wave][tid & 31] = make_float2(M, L);
+            if ((tid & 63) == 0) odd_lds[wave] = odd;
 #pragma unroll
-                for (int n = 0; n < N; ++n)
+            for (int n = 0; n < NQ; ++n) o_lds[wave][n][tid & 63] = o[n];
+            __syncthreads();
+            M = -INFINITY;
+            L = 0.0f;
+            f32x4_t x[NQ];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[n][j] = fmaf(x[i][n][j], w1, o[n][j] * w0);
+            for (int n = 0; n < NQ; ++n) o[n] = x[n] = zero;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                odd = max(odd, odd_lds[w]);
+                x[0] = o_lds[w][wave][tid & 63];
+                merge(ml_lds[w][tid & 31], x);
             }
         }
     }
@@ -975,9 +1010,16 @@ static void launch_t(TreeKArgs& ka, hipStream_t st, unsigned grid[3], unsigned* 
     });
     if (between) between(user);
     const int blocks = (a.max_tokens * a.group + 31) / 32;
-    const unsigned g = (unsigned)((int64_t)a.n_seqs * a.kv_heads * blocks);
-    if (a.head_dim <= 64) tree_combine<T, 64><<<g, 256, 0, st>>>(ka, s.kt, s.rw, s.hw, blocks);
-    else tree_combine<T, 128><<<g, 256, 0, st>>>(ka, s.kt, s.rw, s.hw, blocks);
+    auto combine = [&](auto dpad) {
+        constexpr int DP = decltype(dpad)::value;
+        const unsigned g = (unsigned)((int64_t)a.n_seqs * a.kv_heads * blocks);
+        if (g <= (unsigned)device_cus())
+            tree_combine<T, DP, true><<<g * (DP / 32), 256, 0, st>>>(ka, s.kt, s.rw, s.hw, blocks);
+        else
+            tree_combine<T, DP, false><<<g, 256, 0, st>>>(ka, s.kt, s.rw, s.hw, blocks);
+    };
+    if (a.head_dim <= 64) combine(std::integral_constant<int, 64>{});
+    else combine(std::integral_constant<int, 128>{});
 }
 
 void launch_tree_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned grid[3],
