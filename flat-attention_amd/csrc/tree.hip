@@ -49,7 +49,7 @@ template <typename T, int DPAD, int RW, int HW>
 struct TreeCfg {
     static constexpr bool F32 = std::is_same<T, float>::value;
     static constexpr int EB = F32 ? 4 : 2;
-    static constexpr int NW = RW == 8 ? 8 : F32 && RW < 4 ? 2 : 4;  // waves
+    static constexpr int NW = F32 && RW == 2 ? 2 : RW == 8 ? 8 : 4;  // waves
     static constexpr int GR = NW / RW;                              // groups
     static constexpr int KW = GR / HW;                              // key groups
     static constexpr int BN = !F32 && RW == 8 ? 64 : 32;            // keys of a group's tile
@@ -58,7 +58,11 @@ struct TreeCfg {
     static constexpr int CPR = ROWB / 16;                           // 16-byte pieces of it
     static constexpr int TILE = BN * ROWB;
     static constexpr int STAGE = 2 * TILE;  // K and V of a group
-    static constexpr int NST = F32 || RW < 4 ? 2 : 4;  // stages: NST - 1 tiles are on their way
+    // f32 rows of one block: one stage, whose K is replaced once the scores have it and whose V once P.V
+    // has it, so that LDS holds the tiles of four waves (16 single tokens over 512..4096 keys, Hq32 Hkv8
+    // D128: 92 us; two waves with two stages 120). 16-bit: 218 us against 212 for the 64 tokens above.
+    static constexpr bool ONE = F32 && RW == 1;
+    static constexpr int NST = ONE ? 1 : F32 || RW < 4 ? 2 : 4;  // stages: NST - 1 tiles are on their way
     static constexpr int SMEM_KV = GR * NST * STAGE;
     static constexpr int MROW = DPAD * 4 + 16;  // row of the O exchange
     static constexpr int SMEM_O = KW > 1 ? NW * 32 * MROW : 0;
@@ -83,8 +87,11 @@ __device__ __forceinline__ int swizzle(int row) {
     else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
+// Non-temporal: the cache is read once, or by the row blocks of one range at about the same time. 64 single
+// bf16 tokens over 512..8192 keys (Hq32 Hkv8 D128) 212 against 229 us, 16 drafted tokens for 24 sequences
+// 95 against 105; one sequence of 8192 whose rows were still in the caches 36 against 34.
 __device__ __forceinline__ void global_to_lds16(const void* p, uint32_t lds) {
-    asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(lds));
+    asm volatile("global_load_lds_dwordx4 %0, off nt" : : "v"(p), "{m0}"(lds));
 }
 
 // Division of numbers below 2^31 by a constant of the launch, in 32 bits: with s = ceil(log2 d) and
@@ -388,8 +395,10 @@ void tree_split(TreeKArgs ka) {
             for (int w = 0; w < C::NW; ++w) bad |= vote_lds[w] != 0;
             bad = __builtin_amdgcn_readfirstlane(bad);
 
-            // ---- one tile of this wave's key group into a stage
-            auto transfer = [&](int step, int stage) {
+            constexpr std::true_type yes{};
+            constexpr std::false_type no{};
+            // ---- one tile of this wave's key group into a stage: its K, its V
+            auto transfer = [&](int step, int stage, auto k_c, auto v_c) {
                 const int tile = step * C::KT + kg * C::BN;
                 if (tile >= k_end) return;
                 uint32_t ln = lane, zero;
@@ -410,14 +419,15 @@ void tree_split(TreeKArgs ka) {
                     const uint8_t* const kp = there ? kpool + off : (const uint8_t*)tree_zero;
                     const uint8_t* const vp = there ? vpool + off : (const uint8_t*)tree_zero;
                     const uint32_t dst = lds0 + group_base + stage + (rw * C::NI + i) * 1024;
-                    global_to_lds16(kp, dst);
-                    global_to_lds16(vp, dst + C::TILE);
+                    if constexpr (decltype(k_c)::value) global_to_lds16(kp, dst);
+                    if constexpr (decltype(v_c)::value) global_to_lds16(vp, dst + C::TILE);
                 }
             };
 
             // ---- 32 keys from `key0` at `at` of a stage: scores, softmax, P.V. MASKED: blocks in which
             // some row may not see some key.
-            auto block = [&](int key0, int at, auto masked_c) {
+            // `next` (ONE): the step whose K and V follow into the stage, -1: none.
+            auto block = [&](int key0, int at, auto masked_c, int next) {
                 constexpr bool MASKED = decltype(masked_c)::value;
                 const int ka0 = kbase + at, va0 = vbase + at;
                 f32x16_t sc;
@@ -431,6 +441,11 @@ void tree_split(TreeKArgs ka) {
 #pragma unroll
                     for (int c = 0; c < KH; ++c)
                         kf[c] = *(const u32x4_t*)(smem + (ka0 ^ ((c0k + c) << 5)));
+                    if constexpr (C::ONE)
+                        if (c0k + KH == KS) {
+                            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                            if (next >= 0) transfer(next, 0, yes, no);
+                        }
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int c = 0; c < KH; ++c) {
@@ -517,6 +532,10 @@ void tree_split(TreeKArgs ka) {
                 // bring them to that row. V is taken without them; tree_combine adds what is missing.
                 uint32_t off = 0;
                 if constexpr (F32) {
+                    if constexpr (C::ONE) {
+                        if (next >= 0) wait_vmcnt<C::NI>();  // (K of the next tile may be on its way)
+                        else wait_dma();
+                    }
 #pragma unroll
                     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -529,6 +548,10 @@ void tree_split(TreeKArgs ka) {
                             }
                             oacc[mb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[i], oacc[mb], 0, 0, 0);
                         }
+                    if constexpr (C::ONE) {
+                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                        if (next >= 0) transfer(next, 0, no, yes);
+                    }
                 } else {
 #pragma unroll
                     for (int k2 = 0; k2 < 2; ++k2) {
@@ -561,9 +584,23 @@ void tree_split(TreeKArgs ka) {
             // ---- the steps, NST - 1 transfers ahead: first those whose keys every row sees
 #pragma unroll
             for (int i = 0; i < C::NST - 1; ++i)
-                if (c0 + i < c1) transfer(c0 + i, i * C::STAGE);
+                if (c0 + i < c1) transfer(c0 + i, i * C::STAGE, yes, yes);
+            if constexpr (C::ONE) {
+                transfer(c0, 0, yes, no);
+                transfer(c0, 0, no, yes);
+            }
             int stage = 0;
             auto run = [&](int from, int to, auto masked_c) {
+                if constexpr (C::ONE) {
+#pragma unroll 1
+                    for (int step = from; step < to; ++step) {
+                        const int tile = step * C::KT + kg * C::BN;
+                        if (tile >= k_end) continue;
+                        wait_vmcnt<C::NI>();  // (V may be on its way)
+                        block(tile, 0, masked_c, step + 1 < c1 && tile + C::KT < k_end ? step + 1 : -1);
+                    }
+                    return;
+                }
 #pragma unroll 1
                 for (int step = from; step < to; ++step) {
                     // (transfers complete in order: those of the NST - 2 tiles behind this one may be
@@ -575,12 +612,12 @@ void tree_split(TreeKArgs ka) {
                     if constexpr (RW > 1) __syncthreads();
                     else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     const int ahead = stage == 0 ? (C::NST - 1) * C::STAGE : stage - C::STAGE;
-                    if (step + C::NST - 1 < c1) transfer(step + C::NST - 1, ahead);
+                    if (step + C::NST - 1 < c1) transfer(step + C::NST - 1, ahead, yes, yes);
                     const int tile = step * C::KT + kg * C::BN;
 #pragma unroll 1
                     for (int kb = 0; kb < C::BN; kb += 32)
                         if (live && (!decltype(masked_c)::value || tile + kb < k_end))
-                            block(tile + kb, stage + kb * C::ROWB, masked_c);
+                            block(tile + kb, stage + kb * C::ROWB, masked_c, -1);
                     stage = stage == (C::NST - 1) * C::STAGE ? 0 : stage + C::STAGE;
                 }
             };
@@ -611,7 +648,7 @@ void tree_split(TreeKArgs ka) {
                     else wait_dma();
                     __syncthreads();
                     const int ahead = stage == 0 ? (C::NST - 1) * C::STAGE : stage - C::STAGE;
-                    if (step + C::NST - 1 < c1) transfer(step + C::NST - 1, ahead);
+                    if (step + C::NST - 1 < c1) transfer(step + C::NST - 1, ahead, yes, yes);
                     const int next = stage == (C::NST - 1) * C::STAGE ? 0 : stage + C::STAGE;
                     if (live) {
                         if (step == from) scores(stage, sc);
@@ -952,8 +989,7 @@ static auto tree_dispatch(const TreeArgs& a, F f) {
         using Two = integral_constant<int, 2>;
         using Four = integral_constant<int, 4>;
         if (rows <= 32) {
-            if constexpr (!F32)
-                if (a.kv_heads % 4 == 0) return run(One{}, Four{});
+            if (a.kv_heads % 4 == 0) return run(One{}, Four{});
             return a.kv_heads % 2 == 0 ? run(One{}, Two{}) : run(One{}, One{});
         }
         if (rows <= 64) {
