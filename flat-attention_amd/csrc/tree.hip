@@ -72,7 +72,13 @@ struct TreeCfg {
     static constexpr int NI = BN * CPR / 64 / RW;
     // the scores of the next block are computed beside the softmax of this one: its tile has to be there
     static constexpr bool PIPE = !F32 && NST > 2;
-    static constexpr int WAVES = (SMEM > 72 * 1024 && NW < 8) || (F32 && DPAD > 64) ? 1 : 2;  // per SIMD
+    // waves a SIMD (three at 64 dims and four row blocks: 24 drafted tokens for 16 sequences, Hq32 Hkv8 f16,
+    // 55 us against 57 with two; at two row blocks 45 against 42), and workgroups a CU (with 5 KiB of LDS besides the stages, 160 KiB in all)
+    static constexpr int WAVES = (SMEM > 72 * 1024 && NW < 8) || (F32 && DPAD > 64) ? 1
+                                 : !F32 && DPAD == 64 && RW == 4                   ? 3
+                                                                                   : 2;
+    static constexpr int BY_LDS = 160 / (SMEM / 1024 + 5), BY_WAVES = 4 * WAVES / NW;
+    static constexpr int PER_CU = BY_LDS < BY_WAVES ? BY_LDS : BY_WAVES;
     // f32 quads of a 32-row block in a partial, in the order that the waves hold them
     static constexpr int QUADS = 8 * DPAD;
 };
@@ -971,8 +977,7 @@ static TreeShape shape_of(const TreeArgs& a) {
     s.kt = C::KT;
     s.row_blocks = (a.max_tokens * a.group + C::ROWS - 1) / C::ROWS;
     // one round of workgroups: as many a CU as LDS and registers hold
-    const int per_cu = C::NW == 8 || C::SMEM > 72 * 1024 || C::WAVES * 4 / C::NW < 2 ? 1 : 2;
-    s.ranges = std::max(1, per_cu * device_cus() / s.row_blocks);
+    s.ranges = std::max(1, C::PER_CU * device_cus() / s.row_blocks);
     s.threads = 64 * C::NW;
     return s;
 }
