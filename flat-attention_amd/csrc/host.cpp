@@ -3499,8 +3499,8 @@ int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q,
     const uint64_t n = b->n_seqs, words = (max_tokens + 63) / 64;
     if (q_heads > kI32 || n * max_tokens > kI32 || mul_ov(n * max_tokens, q_heads, &lse) || lse > kI32)
         return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "drafted tokens exceed the i32 index space");
-    // steps of 32 keys or more of every (sequence, kv head), counted in 32 bits
-    if (mul_ov(n * kv_heads, capacity / 32 + 1, &elements) || elements > kI32)
+    // steps of 32 keys or more of every (sequence, kv head), and its start, counted in 32 bits
+    if (mul_ov(n * kv_heads, capacity / 32 + 16, &elements) || elements > kI32)
         return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the i32 index space");
     elements = lse * head_dim;
     fa_packed_layout lay;

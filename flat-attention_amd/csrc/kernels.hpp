@@ -400,8 +400,8 @@ struct TreeArgs {
     int max_pages, page_size, physical_pages;
     float scale;
     // Scratch (tree_workspace): partial O and (m, l) of the units that several key ranges share, and
-    // the plan that the split kernel leaves for the combine: each sequence's first step, the number of
-    // all steps and those of a range.
+    // the plan that the split kernel leaves for the combine: each sequence's place in the split,
+    // the length of a range and what a unit's start counts for.
     float* part_o;
     float2* part_ml;
     int* plan;

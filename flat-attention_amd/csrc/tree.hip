@@ -32,7 +32,7 @@ namespace fa {
 //
 // The lengths are known on the GPU only, so the launch has a fixed number of workgroups; each finds its
 // share by a prefix sum over the sequences: the steps (KT keys) of all (sequence, kv head) units laid
-// end to end are cut into equal ranges. A unit that one range covers is finished there; the others
+// end to end, with a few steps' worth before each for its start, are cut into equal ranges. A unit that one range covers is finished there; the others
 // leave partial (O, m, l), at most two a workgroup, that tree_combine merges in their order.
 
 // Sixteen zero bytes: what rows and dims that do not exist are fetched from.
@@ -42,6 +42,11 @@ __device__ __attribute__((aligned(16))) uint32_t tree_zero[4];
 #define FA_SG(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
 
 constexpr int kTreePages = 1024;  // block-table entries held in LDS at a time
+// Steps that the start of a unit counts for in the split (its table entries, Q, first tile, masked keys and
+// end take as long), but at most half of a range's steps: with few steps a range the split would be uneven.
+// 24 trees of 64 tokens over 512..8192 bf16 keys, Hq32 Hkv8: 198 us with 0, 189 / 182 / 184 / 192 with 3 / 6
+// / 9 / 14; 64 single tokens 212 / 209 / 210 / 213 / 212.
+constexpr int kTreeStart = 6;
 
 // RW row blocks of 32 rows, HW kv heads side by side: NW / RW groups of waves, of which HW KW = NW / RW
 // with KW key groups a head.
@@ -222,23 +227,31 @@ void tree_split(TreeKArgs ka) {
 
     // ---- this workgroup's range of steps [pos, end), and the sequence that holds the first; every wave
     // for itself, without a barrier
-    auto steps_of = [&](int rows) { return units * ((rows + C::KT - 1) / C::KT); };
+    auto steps_of = [&](int rows) { return (rows + C::KT - 1) / C::KT; };
     auto rows_of = [&](int i) { return i < a.n_seqs ? tree_rows_of(a, i) : 0; };
-    int mine = steps_of(rows_of(lane));
-    for (int i = lane + 64; i < a.n_seqs; i += 64) mine += steps_of(rows_of(i));
-    const int total = __builtin_amdgcn_readlane(wave_scan(mine), 63);
+    int mine = 0, count = 0;  // steps, and units that have any
+    for (int i = lane; i < a.n_seqs; i += 64) {
+        const int n = steps_of(rows_of(i));
+        mine += units * n;
+        count += n ? units : 0;
+    }
+    const int n_steps = __builtin_amdgcn_readlane(wave_scan(mine), 63);
+    const int n_units = __builtin_amdgcn_readlane(wave_scan(count), 63);
+    const int ov = min(kTreeStart, (int)ka.ranges.div((uint32_t)n_steps) / 2);
+    const int total = n_steps + n_units * ov;
+    auto length_of = [&](int rows) { return rows ? steps_of(rows) + ov : 0; };  // of a unit
     const int share = max(1, (int)ka.ranges.div((uint32_t)total + ka.ranges.d - 1));
     int64_t pos = (int64_t)range * share;
     const int64_t end = pos + share < total ? pos + share : total;
     const bool plans = logical == 0 && wave == 0;  // writes what tree_combine needs
     if (plans && lane == 0) {
-        a.plan[a.n_seqs] = total;
-        a.plan[a.n_seqs + 1] = share;
+        a.plan[a.n_seqs] = share;
+        a.plan[a.n_seqs + 1] = ov;
     }
     int s = 0, first = 0, rows_s = 0, len = 0;  // the sequence, its first step, its rows, the drafted ones
     bool found = pos >= end;
     for (int base = 0, carry = 0; base < a.n_seqs && (plans || !found); base += 64) {
-        const int rows = rows_of(base + lane), v = steps_of(rows);
+        const int rows = rows_of(base + lane), v = units * length_of(rows);
         const int upto = carry + wave_scan(v);
         if (plans && base + lane < a.n_seqs) a.plan[base + lane] = upto - v;
         const uint64_t past = __ballot(upto > pos);
@@ -281,18 +294,20 @@ void tree_split(TreeKArgs ka) {
 
     while (pos < end) {
         // ---- the unit that holds step pos and this range's part of it
-        while (pos >= (int64_t)first + steps_of(rows_s)) {
-            first += steps_of(rows_s);
+        while (pos >= (int64_t)first + units * length_of(rows_s)) {
+            first += units * length_of(rows_s);
             ++s;
             rows_s = __builtin_amdgcn_readfirstlane(tree_rows_of(a, s));
             len = __builtin_amdgcn_readfirstlane(a.tree_lens[s]);
         }
-        const int steps = (rows_s + C::KT - 1) / C::KT;
+        const int steps = steps_of(rows_s);
         const int in_seq = (int)(pos - first);
-        const int unit = __builtin_amdgcn_readfirstlane(in_seq / steps), kvh = unit * HW + hd;
-        const int st0 = in_seq - unit * steps;
-        const int st1 = (int)min((int64_t)steps, st0 + (end - pos));
-        pos += st1 - st0;
+        const int unit = __builtin_amdgcn_readfirstlane(in_seq / (steps + ov)), kvh = unit * HW + hd;
+        const int from = in_seq - unit * (steps + ov);
+        const int to = (int)min((int64_t)steps + ov, from + (end - pos));
+        pos += to - from;
+        const int st0 = max(0, from - ov), st1 = to - ov;
+        if (st1 <= st0) continue;
         const int ctx = rows_s - len;
         const int rows_total = len * a.group, r0 = rb * C::ROWS;
         if (r0 >= rows_total) continue;
@@ -832,7 +847,7 @@ __global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rw
     const int b32 = id % blocks, sh = id / blocks;
     const int kvh = sh % a.kv_heads, s = sh / a.kv_heads;
     const int row = b32 * 32 + (tid & 31), rows_all = a.max_tokens * a.group;
-    const int share = a.plan[a.n_seqs + 1], before = a.plan[s];  // (asked for with the lengths)
+    const int share = a.plan[a.n_seqs], ov = a.plan[a.n_seqs + 1], before = a.plan[s];  // (asked for with the lengths)
     const int rows_s = tree_rows_of(a, s);
     const int len = rows_s ? a.tree_lens[s] : 0;
     const int d0 = 32 * mb0 + 8 * wave + 4 * ((tid >> 5) & 1);  // dims d0 + 32 n .. + 3
@@ -844,7 +859,7 @@ __global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rw
     }
     if (b32 * 32 >= len * a.group) return;
     const int steps = (rows_s + kt - 1) / kt;
-    const uint32_t u0 = (uint32_t)before + (uint32_t)(kvh / hw) * (uint32_t)steps;
+    const uint32_t u0 = (uint32_t)before + (uint32_t)(kvh / hw) * (uint32_t)(steps + ov) + (uint32_t)ov;
     const int g0 = (int)(u0 / (uint32_t)share), g1 = (int)((u0 + steps - 1) / (uint32_t)share);
     const int rb = b32 / rw, in = b32 - rb * rw;
     const int nrb = (int)ka.row_blocks.d;
