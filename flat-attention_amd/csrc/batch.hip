@@ -88,6 +88,8 @@ __global__ __launch_bounds__(1024) void reserve_plan(ReserveKArgs ka, int fused)
     __shared__ uint64_t sums[16];
     __shared__ ReservePlan plans[1024];
     __shared__ int ctxs[1024];
+    __shared__ int2 backs[1024];  // of an ended sequence: its pages, and how many go on the stack before
+    __shared__ uint64_t ends[16];
     const int tid = threadIdx.x, threads = blockDim.x;
     const int count = min(max(a.free_count[0], 0), a.free_capacity);
     auto kept_of = [&](int s) { return min(max(a.mapped[s], 0), a.max_pages); };
@@ -138,18 +140,29 @@ __global__ __launch_bounds__(1024) void reserve_plan(ReserveKArgs ka, int fused)
                 a.plan[s] = make_int4(p.kept, p.granted, p.first, p.taken);
             }
         }
-        // the pages of ended sequences, one wave a sequence: they are on the stack before any is taken
-        uint64_t ends = __ballot(ended);
-        const int push = (int)((upto >> 32) - (ended ? kept : 0));
-        while (ends) {
-            const int l = __ffsll((unsigned long long)ends) - 1;
-            ends &= ends - 1;
-            const int es = base + (tid & ~63) + l, n = __shfl(kept, l, 64);
-            const int64_t at = (int64_t)count + __shfl(push, l, 64);
-            for (int j = tid & 63; j < n; j += 64)
-                if (at + j < a.free_capacity)
-                    a.free_pages[at + j] = a.block_tables[(int64_t)es * a.max_pages + j];
-        }
+        // the pages of ended sequences, dealt out to the waves: they are on the stack before any is taken
+        if (ended) backs[tid] = make_int2(kept, (int)((upto >> 32) - kept));
+        const uint64_t mine_end = __ballot(ended);
+        if ((tid & 63) == 0) ends[tid >> 6] = mine_end;
+        __syncthreads();
+        int turn = 0;
+        for (int w = 0; w < (threads >> 6); ++w)
+            for (uint64_t left = ends[w]; left; left &= left - 1) {
+                if (turn++ % (threads >> 6) != tid >> 6) continue;
+                const int l = w * 64 + __ffsll((unsigned long long)left) - 1;
+                const int n = backs[l].x;
+                const int64_t at = (int64_t)count + backs[l].y;
+                const int* const row = a.block_tables + (int64_t)(base + l) * a.max_pages;
+                for (int j0 = tid & 63; j0 < n; j0 += 256) {
+                    int page[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) page[i] = row[min(j0 + 64 * i, n - 1)];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (j0 + 64 * i < n && at + j0 + 64 * i < a.free_capacity)
+                            a.free_pages[at + j0 + 64 * i] = page[i];
+                }
+            }
         if (ended) a.ctx_lens[s] = 0;
         carry += total;
     }
@@ -176,7 +189,7 @@ __global__ __launch_bounds__(1024) void reserve_plan(ReserveKArgs ka, int fused)
         fill_sequence(ka, s, plans[s], ctxs[s], avail, 0, a.max_new, tid % lanes, lanes);
 }
 
-constexpr int kFillTokens = 1024;  // slots per workgroup of reserve_fill
+constexpr int kFillTokens = 256;  // slots per workgroup of reserve_fill, one a thread: two loads in a row
 
 __global__ __launch_bounds__(256) void reserve_fill(ReserveKArgs ka, int parts) {
     const int s = blockIdx.x / parts, t0 = blockIdx.x % parts * kFillTokens;
@@ -198,7 +211,8 @@ void launch_reserve(const ReserveArgs& a, hipStream_t s, unsigned grid[3], unsig
     const bool fused = reserve_fused(a.n_seqs, a.max_new);
     const int64_t work = fused ? std::max<int64_t>((int64_t)a.n_seqs * std::min(a.max_new, 64), a.n_seqs)
                                : a.n_seqs;
-    const int threads = work <= 64 ? 64 : work <= 256 && a.n_seqs <= 256 ? 256 : 1024;
+    // (not fused: the waves share the pages of ended sequences)
+    const int threads = fused && work <= 64 ? 64 : fused && work <= 256 ? 256 : 1024;
     reserve_plan<<<1, threads, 0, s>>>(ka, fused ? 1 : 0);
     grid[0] = 1;
     grid[1] = grid[2] = 1;
@@ -221,13 +235,14 @@ void launch_reserve(const ReserveArgs& a, hipStream_t s, unsigned grid[3], unsig
 // LDS, bound by launch and round latency.
 // A parent that is neither -1 nor an earlier token ends in -2, which every descendant inherits: those
 // tokens get an empty mask and position -1.
+template <int W>  // words of a mask
 __global__ __launch_bounds__(1024) void tree_masks(TreeMaskArgs a) {
-    __shared__ uint64_t m[kTreeTokens * (kTreeTokens / 64)];
-    __shared__ int jump[kTreeTokens];
-    const int s = blockIdx.x, tid = threadIdx.x, threads = blockDim.x, W = a.words;
+    __shared__ uint64_t m[64 * W * W];
+    __shared__ int jump[64 * W];
+    const int s = blockIdx.x, tid = threadIdx.x, threads = blockDim.x;
     const int ctx = a.ctx_lens[s], len = a.tree_lens[s];
     const int n = ctx >= 0 && len >= 0 && len <= a.max_tokens ? len : 0;
-    constexpr int kItems = kTreeTokens * (kTreeTokens / 64) / 1024;  // words a thread may hold
+    constexpr int kItems = (64 * W * W + 1023) / 1024;  // words a thread may hold
     for (int t = tid; t < n; t += threads) {
         const int p = a.parents[(int64_t)s * a.max_tokens + t];
         jump[t] = p < -1 || p >= t ? -2 : p;
@@ -288,7 +303,17 @@ __global__ __launch_bounds__(1024) void tree_masks(TreeMaskArgs a) {
 void launch_tree_masks(const TreeMaskArgs& a, hipStream_t s, unsigned grid[3], unsigned* block) {
     const int items = a.max_tokens * a.words;
     const int threads = items >= 1024 ? 1024 : (items + 63) / 64 * 64;
-    tree_masks<<<(unsigned)a.n_seqs, threads, 0, s>>>(a);
+    const unsigned g = (unsigned)a.n_seqs;
+    switch (a.words) {
+        case 1: tree_masks<1><<<g, threads, 0, s>>>(a); break;
+        case 2: tree_masks<2><<<g, threads, 0, s>>>(a); break;
+        case 3: tree_masks<3><<<g, threads, 0, s>>>(a); break;
+        case 4: tree_masks<4><<<g, threads, 0, s>>>(a); break;
+        case 5: tree_masks<5><<<g, threads, 0, s>>>(a); break;
+        case 6: tree_masks<6><<<g, threads, 0, s>>>(a); break;
+        case 7: tree_masks<7><<<g, threads, 0, s>>>(a); break;
+        default: tree_masks<8><<<g, threads, 0, s>>>(a); break;
+    }
     grid[0] = (unsigned)a.n_seqs;
     grid[1] = grid[2] = 1;
     *block = (unsigned)threads;
