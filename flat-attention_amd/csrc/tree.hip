@@ -574,6 +574,30 @@ void tree_split(TreeKArgs ka) {
                         if (next >= 0) transfer(next, 0, no, yes);
                     }
                 } else {
+                    if constexpr (MASKED) {
+                        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+                        u16x2 top = {0, 0};  // largest magnitude, sign off
+#pragma unroll
+                        for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+                            for (int mb = 0; mb < MB; ++mb) {
+                                vf[k2][mb] = tree_v16<DPAD>(smem, va0, k2, mb);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    top = __builtin_elementwise_max(
+                                        top, __builtin_bit_cast(u16x2, vf[k2][mb][j] & 0x7fff7fffu));
+                            }
+                        off = not_finite<T>(__builtin_bit_cast(uint32_t, top));
+                        if (__any(off != 0)) {
+#pragma unroll
+                            for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+                                for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                        vf[k2][mb][j] &= ~not_finite<T>(vf[k2][mb][j]);
+                        }
+                    }
 #pragma unroll
                     for (int k2 = 0; k2 < 2; ++k2) {
                         u32x4_t pb;
@@ -582,19 +606,7 @@ void tree_split(TreeKArgs ka) {
                             pb[j] = Half<T>::pack(sc[8 * k2 + 2 * j], sc[8 * k2 + 2 * j + 1]);
 #pragma unroll
                         for (int mb = 0; mb < MB; ++mb) {
-                            u32x4_t v;
-                            if constexpr (MASKED) {
-                                v = tree_v16<DPAD>(smem, va0, k2, mb);
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const uint32_t x = not_finite<T>(v[j]);
-                                    off |= x;
-                                    v[j] &= ~x;
-                                }
-                            } else {
-                                v = vf[k2][mb];
-                            }
-                            oacc[mb] = Half<T>::mfma32(v, pb, oacc[mb]);
+                            oacc[mb] = Half<T>::mfma32(vf[k2][mb], pb, oacc[mb]);
                         }
                     }
                 }
