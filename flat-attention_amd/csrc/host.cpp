@@ -3269,6 +3269,8 @@ int fa_backward_recompute_mha(fa_ctx* ctx, const void* packed_forward, size_t fo
 // ------------------------------------------------------------------ device-resident batch
 namespace {
 
+constexpr uint64_t kBatchSeqs = 1 << 20;  // sequences of a batch
+
 // Sizes and index ranges of a batch; `tables`: its block tables are used. *capacity: tokens a row holds.
 int check_batch(const fa_paged_batch* b, bool tables, uint64_t* capacity) {
     if (!b) return fail(FA_ERR_NULL_ARGUMENT, "batch is null");
@@ -3276,6 +3278,10 @@ int check_batch(const fa_paged_batch* b, bool tables, uint64_t* capacity) {
         return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
     if (!b->page_size || !b->physical_pages)
         return fail(FA_ERR_PAGED_ZERO_DIMENSION, "paged KV dimensions must be non-zero");
+    // (a launch has below 2^32 threads, here up to 1024 a sequence)
+    if (b->n_seqs > kBatchSeqs)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "%llu sequences exceed the maximum %llu",
+                    (unsigned long long)b->n_seqs, (unsigned long long)kBatchSeqs);
     uint64_t entries, rows;
     if (mul_ov(b->page_size, b->physical_pages, &rows) || rows > kI32 ||
         mul_ov(b->max_pages, b->page_size, capacity) || *capacity > kI32 ||
@@ -3426,7 +3432,7 @@ int fa_paged_append_slots(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* s
     if (!max_new) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
     if (int rc = check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)) return rc;
     if (mul_ov(b->n_seqs, max_new, &rows) || rows > kI32 || mul_ov(rows, row / 16, &pieces) ||
-        pieces > 0xffffffffull)
+        pieces > 0xffffff00ull)
         return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged append exceeds the index space");
     need = rows * row;
     if (int rc = check_buffer("slots", slots, slots_bytes, rows * 4)) return rc;
@@ -3502,6 +3508,9 @@ int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q,
     // steps of 32 keys or more of every (sequence, kv head), and its start, counted in 32 bits
     if (mul_ov(n * kv_heads, capacity / 32 + 16, &elements) || elements > kI32)
         return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the i32 index space");
+    // threads of the combine: 256 for every 32 rows of a (sequence, kv head)
+    if (n * kv_heads * ((max_tokens * (q_heads / kv_heads) + 31) / 32) > 0xffffff)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the launch space");
     elements = lse * head_dim;
     fa_packed_layout lay;
     if (int rc = fa_packed_layout_for(elements, lse, dtype, &lay)) return rc;

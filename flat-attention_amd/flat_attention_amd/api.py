@@ -1151,7 +1151,8 @@ class HipPagedBatch:
                 free_count_out: Optional[DeviceBuffer] = None):
         """Slots for the new tokens of every sequence (fa_paged_reserve_slots). ``mapped`` and
         ``free_count`` are updated in place unless their ``_out`` arrays are given."""
-        mo, fo = mapped_out or mapped, free_count_out or free_count
+        mo = mapped if mapped_out is None else mapped_out
+        fo = free_count if free_count_out is None else free_count_out
         check(lib().fa_paged_reserve_slots(
             self.ctx.handle, self._c, new_lens.ptr, new_lens.nbytes, max_new, mapped.ptr, mo.ptr,
             min(mapped.nbytes, mo.nbytes), free_pages.ptr, free_pages.nbytes, free_count.ptr,
@@ -1205,7 +1206,7 @@ class HipPagedBatch:
                head_dim: int, dtype: int, ctx_lens_out: Optional[DeviceBuffer] = None):
         """Accepted rows into place and the lengths past them (fa_paged_accept), in ``ctx_lens`` unless
         ``ctx_lens_out`` is given."""
-        out = ctx_lens_out or self.ctx_lens
+        out = self.ctx_lens if ctx_lens_out is None else ctx_lens_out
         check(lib().fa_paged_accept(
             self.ctx.handle, self._c, paths.ptr, paths.nbytes, max_accept, accepted.ptr,
             accepted.nbytes, tree_lens.ptr, tree_lens.nbytes, out.ptr, out.nbytes, k_pool.ptr,

@@ -555,7 +555,7 @@ typedef struct fa_paged_batch {
     size_t block_tables_bytes;
     int32_t* ctx_lens;          /* device [n_seqs] live tokens */
     size_t ctx_lens_bytes;
-    uint64_t n_seqs, max_pages, page_size, physical_pages;
+    uint64_t n_seqs, max_pages, page_size, physical_pages; /* n_seqs <= 2^20 */
 } fa_paged_batch;
 
 /* Slots for the new tokens of every sequence, in sequence order. All arrays are device int32:

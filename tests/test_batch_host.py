@@ -159,6 +159,22 @@ def test_other_arguments():
     assert attend(tokens=65, masks=P, masks_bytes=4 * 65 * 2 * 8 - 1) == "BufferTooSmall"
 
 
+def test_launches_stay_within_the_grid():
+    for call in CALLS:
+        assert call(batch(n=(1 << 20) + 1, max_pages=1)) == "IndexSpaceExceeded"
+        assert call(batch(n=1 << 20, max_pages=1)) in ("NullArgument", "BufferTooSmall")
+    # a combine of 2^24 workgroups of 256 threads, and one less
+    for heads in (16, 15):
+        rc = attend(batch(n=1 << 20, max_pages=1), tokens=1, q_heads=heads, kv_heads=heads, head_dim=8,
+                    q_bytes=1 << 62, out_bytes=1 << 62)
+        assert rc == ("IndexSpaceExceeded" if heads == 16 else "NullArgument")
+    # rows of 16 bytes: 2^32 - 256 pieces are the most that an append moves
+    one = dict(kv_heads=2, head_dim=8, src_bytes=1 << 62, slots_bytes=1 << 62)
+    assert append(batch(n=1 << 20, max_pages=1), max_new=2047, **one) == "NullArgument"
+    assert append(batch(n=(1 << 20) - 1, max_pages=1), max_new=2048, **dict(one, kv_heads=3)) \
+        == "IndexSpaceExceeded"
+
+
 def test_python_mirror_names_the_error():
     class Ctx:  # a context that was closed
         handle = None

@@ -109,6 +109,19 @@ def test_reserve_matches_the_model(hip, n, max_new, page, high, short, seed, inp
     _compare(_reserve(hip, table, ctx, new, mapped, free, count, max_new, page, pages, inplace), want)
 
 
+@pytest.mark.parametrize("n", [5, 1500])
+def test_ended_sequences_with_many_pages(hip, n):
+    """Rows of up to 700 pages go back on the stack, and the others take some of them at once."""
+    rng = np.random.default_rng(n)
+    mapped = np.where(rng.random(n) < 0.1, rng.integers(1, 701, n), 1)
+    mapped[1] = 700
+    new = np.where(mapped > 1, -1, 30)
+    table, pages, spare = paged(rng, mapped, 1, width=702, spare=3)
+    free = np.concatenate([spare, np.full(int(mapped.sum()), -5)])
+    args = (table, np.minimum(mapped, 1), new, mapped, free, spare.size, 30, 1, pages)
+    _compare(_reserve(hip, *args, True), model.reserve(*args))
+
+
 def test_reserve_with_arrays_that_hold_nonsense(hip):
     """Negative lengths, mapped counts and free counts out of range, pages outside the pool, a stack too
     short for what comes back: those take no part, nothing else changes."""
@@ -345,6 +358,16 @@ def test_many_sequences(hip, dtype, n, most):
     lens = rng.integers(0, most + 1, n)
     case = Case(hip, dtype, rng.integers(0, 90, n), lens, most, 4, 2, 32, 16, 8)
     case.check()
+
+
+@pytest.mark.parametrize("dtype,most,hq,hkv", [(BF16, 1, 8, 8), (F32, 1, 8, 8), (F16, 9, 8, 4), (BF16, 40, 8, 4),
+                                               (F32, 20, 8, 4), (BF16, 65, 8, 2)])
+def test_long_and_short_sequences_share_the_ranges(hip, dtype, most, hq, hkv):
+    """Enough keys that a range holds several steps: ranges that cover short sequences whole, end in
+    their start, and cut long ones in parts."""
+    rng = np.random.default_rng(most)
+    ctx = np.where(rng.random(40) < 0.5, rng.integers(0, 60, 40), rng.integers(1000, 3200, 40))
+    Case(hip, dtype, ctx, rng.integers(0, most + 1, 40), most, hq, hkv, 64, 16, 12).check()
 
 
 def test_large_scores_and_empty_rows(hip):
