@@ -370,6 +370,36 @@ def test_long_and_short_sequences_share_the_ranges(hip, dtype, most, hq, hkv):
     Case(hip, dtype, ctx, rng.integers(0, most + 1, 40), most, hq, hkv, 64, 16, 12).check()
 
 
+@pytest.mark.parametrize("dtype,ctx,lens,most,hq,hkv,D,page", [
+    (BF16, [70, 9], [5, 2], 5, 8, 8, 8, 16), (F16, [70, 9], [40, 2], 40, 8, 4, 8, 3),
+    (F32, [70, 9], [5, 2], 5, 4, 4, 4, 16), (F32, [140, 9], [40, 1], 40, 4, 2, 4, 1),
+    (BF16, [600], [512], 512, 16, 2, 64, 16), (F32, [100], [300], 300, 8, 2, 64, 16),
+    (BF16, [5000], [512], 512, 1, 1, 128, 1 << 13), (F16, [40, 0], [3, 1], 3, 96, 1, 64, 16)])
+def test_narrow_heads_and_many_rows(hip, dtype, ctx, lens, most, hq, hkv, D, page):
+    Case(hip, dtype, ctx, lens, most, hq, hkv, D, page, 13).check()
+
+
+def test_two_contexts_at_once(hip):
+    """Two contexts of one GPU, their calls in turn and neither waited for: each has its own stream and
+    workspaces, and gets what it gets alone."""
+    other = fa.HipContext(0)
+    try:
+        cases = [Case(c, BF16, [2500, 3, 700], [9, 4, 6], 9, 8, 4, 64, 16, 14 + i)
+                 for i, c in enumerate((hip, other))]
+        alone = [c.check() for c in cases]
+        for _ in range(5):
+            for c in cases:
+                c.out.fill_u32(0x7fc07fc0)
+            for _ in range(4):
+                for c in cases:
+                    c.call(upload=False)
+            for c, (o, lse) in zip(cases, alone):
+                o1, l1 = c.get()
+                assert np.array_equal(o, o1) and np.array_equal(lse, l1)
+    finally:
+        other.close()
+
+
 def test_large_scores_and_empty_rows(hip):
     """Scores of hundreds (the running maximum moves), and a mask that leaves rows nothing."""
     for dtype in (BF16, F16, F32):
