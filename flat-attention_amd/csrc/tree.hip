@@ -17,23 +17,37 @@
 namespace fa {
 
 // Rows of one (sequence, kv head) are flattened as row = t * group + head, so every K/V byte read
-// serves all of them. A workgroup holds 32 RW rows; its waves are RW row blocks times KW key groups.
-// Per 32 keys and wave, the products transposed so that a lane owns one query row:
+// serves all of them. A workgroup holds RW blocks of 32 rows; its waves are RW row blocks times HW kv
+// heads times KW key groups. Per 32 keys and wave, the products transposed so that a lane owns one query
+// row:
 //   S^T[32 keys x 32 rows] = K . Q^T     K from LDS (A operand), Q in registers (B)
 //   P^T = exp2((S - m) scale log2 e)     one lane exchange (lane ^ 32) for the row maximum
 //   O^T[dims x 32 rows]   += V^T . P^T   V read transposed from LDS; the S^T accumulator is the P^T
 //                                        operand as it stands, V's keys are taken in its order
-// K and V rows go straight from memory into LDS, 16 bytes a lane, two stages; the LDS column of a piece
-// is XORed with its row so that both operand reads are free of bank conflicts without padding. Rows
-// that do not exist, and dims past head_dim, are fetched from 16 zero bytes.
+// K and V rows go straight from memory into LDS, 16 bytes a lane, one to three tiles ahead; the LDS column
+// of a piece is XORed with its row so that both operand reads are free of bank conflicts without padding
+// (none counted). Rows that do not exist, and dims past head_dim, are fetched from 16 zero bytes.
 // 16-bit storage: the rotated Q is kept as a 16-bit high part and the rounding of its residual, two
 // MFMAs a step, so that scores and LSE carry f32 accuracy; P is rounded once to the storage type (its
 // sum is taken before), an error of the size of O's own rounding.
 //
 // The lengths are known on the GPU only, so the launch has a fixed number of workgroups; each finds its
 // share by a prefix sum over the sequences: the steps (KT keys) of all (sequence, kv head) units laid
-// end to end, with a few steps' worth before each for its start, are cut into equal ranges. A unit that one range covers is finished there; the others
-// leave partial (O, m, l), at most two a workgroup, that tree_combine merges in their order.
+// end to end, with a few steps' worth before each for its start, are cut into equal ranges. A unit that
+// one range covers is finished there; the others leave partial (O, m, l), at most two a workgroup, that
+// tree_combine merges in their order.
+//
+// What bounds it (both launches, Hq32 Hkv8 D128 bf16, pages of 16 rows, contexts of 512..8192):
+//   64 sequences, one token: 1.16 GB in 195 us, 5.95 TB/s; memory (a copy reaches 5.16 TB/s here, loads
+//     alone 6.75). What is left is each unit's start, while its workgroup does not stream.
+//   24 sequences, 16 / 32 / 64 tokens each: 92 / 103 / 163..178 us (by the box). 64 tokens fill 256 rows: the matrix
+//     core runs 65 % of a step of 64 keys (4850 cycles, 3170 of them MFMA: two waves a SIMD, whose softmax
+//     and products overlap only in part), and a unit's start (its lengths, table entries, Q with its
+//     angles, first tile, masked blocks, end) takes as long as six steps.
+//   One sequence, 5 tokens, 1000 keys, Hq16 Hkv4 D64: 13.1 us, the latency of two launches and of four
+//     dependent loads in the first (lengths; table entries; Q; tile).
+// The simplest kernel of this layout (operands read by each lane from memory, no stages) took 7254, 20521
+// and 205 us for the first, the 64-token and the last of these.
 
 // Sixteen zero bytes: what rows and dims that do not exist are fetched from.
 __device__ __attribute__((aligned(16))) uint32_t tree_zero[4];
@@ -841,8 +855,10 @@ void tree_split(TreeKArgs ka) {
 // Merges the partials of the units that several ranges share, and writes the rows past each tree. A
 // thread ends with one row and a quad of dims in each of N 32-dim blocks.
 // Not WIDE: a workgroup per 32 rows of a (sequence, kv head), which merges their partials in their order,
-// several loads ahead. WIDE: one per 32 dims of those; its waves take every fourth partial each and are
-// merged in LDS, in their order.
+// several loads ahead. WIDE, where those do not fill the chip: one per 32 dims of them; its waves take every
+// fourth partial each and are merged in LDS, in their order (256 ranges, one sequence of 8192 keys, 16 tokens,
+// Hkv8: 14 us against 37; the chain of 5 over 1000 keys 8 against 13; 24 trees of 64 tokens 24 against 15).
+// Partials are f32: of the 24 trees they are 60 MB, 14 us at 4.4 TB/s.
 template <typename T, int DPAD, bool WIDE>
 __global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rw, int hw, int blocks) {
     const TreeArgs& a = ka.a;
@@ -990,8 +1006,12 @@ __global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rw
 }
 
 // The shape of a launch. Rows: as few row blocks of 32 as hold every row of a (sequence, kv head), at
-// most 8 (f32: 4). Waves left over take kv heads side by side, whose rows of a token lie next to each
-// other in memory, or key groups where the head count does not divide.
+// most 8 (f32: 4), since K and V are read once for each 32 RW rows (24 trees of 64 tokens, 256 rows: 175 us
+// with 8 blocks and 64 keys a step, 202 with 4 that read K and V twice). Waves left over take two kv heads
+// side by side and two key groups; the key groups alone where the head count is odd, the heads alone where
+// two groups are left. Four heads / two and two / four key groups: 64 single bf16 tokens over 512..8192 keys
+// 210 / 195 / 194 us, 200 over 16..600 72 / 80 / 100, 8 drafted tokens for 16 sequences of 16 heads 75 / 71 /
+// 75. f32 takes four heads: 16 single tokens 85 us, four key groups 97.
 struct TreeShape {
     int rw, hw, kt, row_blocks, ranges, threads;
 };
@@ -1021,7 +1041,8 @@ static auto tree_dispatch(const TreeArgs& a, F f) {
         using Two = integral_constant<int, 2>;
         using Four = integral_constant<int, 4>;
         if (rows <= 32) {
-            if (a.kv_heads % 4 == 0) return run(One{}, Four{});
+            if constexpr (F32)
+                if (a.kv_heads % 4 == 0) return run(One{}, integral_constant<int, 4>{});
             return a.kv_heads % 2 == 0 ? run(One{}, Two{}) : run(One{}, One{});
         }
         if (rows <= 64) {
