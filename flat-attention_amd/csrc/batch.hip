@@ -24,7 +24,9 @@ namespace fa {
 // sequence whose inclusive sum passes avail gets nothing (nor does any later one that needs a page).
 // A few integers a sequence: bound by the launch and two dependent loads. One workgroup does the
 // prefix sum (a wave scan and one exchange between the waves); it also writes tables and slots where
-// they are few (kReserveFused), otherwise reserve_fill does from the plan it leaves.
+// they are few (reserve_fused), otherwise reserve_fill does from the plan it leaves.
+// One sequence 4.7 us, the smallest a call takes; 256 of up to 2048 tokens, 24 ended, 13.4 (17.8 with four
+// slots a thread and each wave putting back the pages of its own ended sequences).
 
 // What reserve_fill has to know of a sequence: pages that stay, tokens granted (-1: none, 0 tokens),
 // and the exclusive prefix sum of the pages it takes.
@@ -232,7 +234,8 @@ void launch_reserve(const ReserveArgs& a, hipStream_t s, unsigned grid[3], unsig
 // mask_t = the bits of token t and its ancestors, position = ctx + number of ancestors. With p the
 // parent, mask_t = bit t | mask_p(t): log2(depth) rounds of pointer doubling (mask |= mask[jump],
 // jump = jump[jump]) instead of a walk as long as the tree is deep. One workgroup a sequence, masks in
-// LDS, bound by launch and round latency.
+// LDS, bound by launch and round latency: 4 trees of 24 tokens 4.2 us, 192 of 256 6.3 (7.9 with the number
+// of words a variable, which costs a division an item and round).
 // A parent that is neither -1 nor an earlier token ends in -2, which every descendant inherits: those
 // tokens get an empty mask and position -1.
 template <int W>  // words of a mask
@@ -322,7 +325,8 @@ void launch_tree_masks(const TreeMaskArgs& a, hipStream_t s, unsigned grid[3], u
 // ---------------------------------------------------------------------------- append by slot
 //
 // Pool row slots[r] = source row r, K rotated at its position on the way (one rounding to the storage
-// type, after the rotation in f32). Bound by memory: a 16-byte piece of K and one of V per thread.
+// type, after the rotation in f32). Bound by memory: a 16-byte piece of K and one of V per thread; 48
+// sequences of up to 512 bf16 rows of 8 heads of 128 (99 MB): 20.3 us, 4.86 TB/s, a copy's rate 5.16.
 // Rows without a slot, and rows whose position the (cos, sin) table does not have, are left out.
 template <typename T>
 __global__ __launch_bounds__(256) void append_slots(SlotAppendArgs a, FastDiv per_row, FastDiv per_seq,
@@ -389,7 +393,8 @@ void launch_append_slots(Dtype dt, const SlotAppendArgs& a, hipStream_t s, unsig
 // length ctx + accepted. A path is strictly increasing (parents come before children), so path[i] >= i
 // and no row is overwritten before it is read if they are moved in order; a thread moves one 16-byte
 // column of every row, kAcceptRows loads ahead of their stores (a store goes to a row at or before the
-// loads of its round). Bound by latency: the table lookups of all rows at once, then a round of loads.
+// loads of its round). Bound by latency: the table lookups of all rows at once, then a round of loads; 2
+// sequences 4.8 us, 128 with up to 16 rows of 4 KiB (8.4 MB) 4.9.
 // A path that is not strictly increasing inside the tree, or that meets an entry outside the pool,
 // moves nothing and leaves the length. One workgroup a sequence: it reads the length before any thread
 // writes it, so both may be the same array.
