@@ -92,7 +92,8 @@ struct TreeCfg {
     // the scores of the next block are computed beside the softmax of this one: its tile has to be there
     static constexpr bool PIPE = !F32 && NST > 2;
     // waves a SIMD (three at 64 dims and four row blocks: 24 drafted tokens for 16 sequences, Hq32 Hkv8 f16,
-    // 55 us against 57 with two; at two row blocks 45 against 42), and workgroups a CU (with 5 KiB of LDS besides the stages, 160 KiB in all)
+    // 55 us against 57 with two; at two row blocks 45 against 42), and workgroups a CU (with 5 KiB of LDS
+    // besides the stages, 160 KiB in all)
     static constexpr int WAVES = (SMEM > 72 * 1024 && NW < 8) || (F32 && DPAD > 64) ? 1
                                  : !F32 && DPAD == 64 && RW == 4                   ? 3
                                                                                    : 2;
@@ -1042,7 +1043,7 @@ static auto tree_dispatch(const TreeArgs& a, F f) {
         using Four = integral_constant<int, 4>;
         if (rows <= 32) {
             if constexpr (F32)
-                if (a.kv_heads % 4 == 0) return run(One{}, integral_constant<int, 4>{});
+                if (a.kv_heads % 4 == 0) return run(One{}, Four{});
             return a.kv_heads % 2 == 0 ? run(One{}, Two{}) : run(One{}, One{});
         }
         if (rows <= 64) {
