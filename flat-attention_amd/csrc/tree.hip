@@ -40,10 +40,10 @@ namespace fa {
 // What bounds it (both launches, Hq32 Hkv8 D128 bf16, pages of 16 rows, contexts of 512..8192):
 //   64 sequences, one token: 1.16 GB in 195 us, 5.95 TB/s; memory (a copy reaches 5.16 TB/s here, loads
 //     alone 6.75). What is left is each unit's start, while its workgroup does not stream.
-//   24 sequences, 16 / 32 / 64 tokens each: 92 / 103 / 163..178 us (by the box). 64 tokens fill 256 rows: the matrix
-//     core runs 65 % of a step of 64 keys (4850 cycles, 3170 of them MFMA: two waves a SIMD, whose softmax
-//     and products overlap only in part), and a unit's start (its lengths, table entries, Q with its
-//     angles, first tile, masked blocks, end) takes as long as six steps.
+//   24 sequences, 16 / 32 / 64 tokens each: 92 / 103 / 163..178 us (by the box). 64 tokens fill 256
+//     rows: the matrix core runs 65 % of a step of 64 keys (4850 cycles, 3170 of them MFMA: two waves a
+//     SIMD, whose softmax and products overlap only in part), and a unit's start (its lengths, table
+//     entries, Q with its angles, first tile, masked blocks, end) takes as long as six steps.
 //   One sequence, 5 tokens, 1000 keys, Hq16 Hkv4 D64: 13.1 us, the latency of two launches and of four
 //     dependent loads in the first (lengths; table entries; Q; tile).
 // The simplest kernel of this layout (operands read by each lane from memory, no stages) took 7254, 20521
