@@ -25,7 +25,7 @@ namespace fa {
 // A few integers a sequence: bound by the launch and two dependent loads. One workgroup does the
 // prefix sum (a wave scan and one exchange between the waves); it also writes tables and slots where
 // they are few (reserve_fused), otherwise reserve_fill does from the plan it leaves.
-// One sequence 4.7 us, the smallest a call takes; 256 of up to 2048 tokens, 24 ended, 13.4 (17.8 with four
+// One sequence 4.7 us, the smallest a call takes; 256 of up to 2048 tokens, 24 ended, 11.0 (17.8 with four
 // slots a thread and each wave putting back the pages of its own ended sequences).
 
 // What reserve_fill has to know of a sequence: pages that stay, tokens granted (-1: none, 0 tokens),
@@ -52,9 +52,11 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* sums, uint6
     if (lane == 63) sums[wave] = v;
     __syncthreads();
     uint64_t all = 0, before = 0;
-    for (int w = 0; w < waves; ++w) {
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {  // (16 loads at once; those of waves that are not there are dropped)
+        const uint64_t x = sums[w];
         if (w == wave) before = all;
-        all += sums[w];
+        all += w < waves ? x : 0;
     }
     *total = all;
     return v + before;
@@ -147,10 +149,14 @@ __global__ __launch_bounds__(1024) void reserve_plan(ReserveKArgs ka, int fused)
         const uint64_t mine_end = __ballot(ended);
         if ((tid & 63) == 0) ends[tid >> 6] = mine_end;
         __syncthreads();
+        const int waves = threads >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const uint64_t all_ends = ends[tid & (waves - 1)];  // (1, 4 or 16 waves)
         int turn = 0;
-        for (int w = 0; w < (threads >> 6); ++w)
-            for (uint64_t left = ends[w]; left; left &= left - 1) {
-                if (turn++ % (threads >> 6) != tid >> 6) continue;
+        for (int w = 0; w < waves; ++w)
+            for (uint64_t left = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(all_ends >> 32), w) << 32 |
+                                 (uint32_t)__builtin_amdgcn_readlane((int)all_ends, w);
+                 left; left &= left - 1) {
+                if ((turn++ & (waves - 1)) != wave) continue;
                 const int l = w * 64 + __ffsll((unsigned long long)left) - 1;
                 const int n = backs[l].x;
                 const int64_t at = (int64_t)count + backs[l].y;
@@ -178,7 +184,11 @@ __global__ __launch_bounds__(1024) void reserve_plan(ReserveKArgs ka, int fused)
     if ((tid & 63) == 0) sums[tid >> 6] = taken;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < (threads >> 6); ++w) taken = sums[w] > taken ? sums[w] : taken;
+#pragma unroll
+        for (int w = 1; w < 16; ++w) {
+            const uint64_t x = sums[w];
+            if (w < (threads >> 6)) taken = x > taken ? x : taken;
+        }
         a.free_count_out[0] = avail - (int)taken;
         if (!fused) a.plan[a.n_seqs] = make_int4(avail, 0, 0, 0);
     }
@@ -201,10 +211,10 @@ __global__ __launch_bounds__(256) void reserve_fill(ReserveKArgs ka, int parts) 
 }
 
 // One workgroup writes everything up to here: beyond it a second launch over the whole chip. Fused / not
-// (us): 16 sequences of 16 tokens 5.1 / 9.0, 64 of 16 7.7 / 9.3, 64 of 64 9.0 / 9.3, 256 of 16 12.5 / 12.8,
-// 256 of 32 18.0 / 13.0, 1 of 16384 52 / 8.
+// (us): 16 sequences of 16 tokens 5.0 / 8.8, 64 of 16 7.1 / 8.8, 64 of 64 8.6 / 8.9, 256 of 16 10.0 / 10.3,
+// 256 of 32 15.3 / 10.5; 8 of 512 7.9 / 8.0, 1 of 2048 (a sequence has 64 threads) 9.4 / 8.0.
 bool reserve_fused(int n_seqs, int max_new) {
-    return n_seqs <= 1024 && (int64_t)n_seqs * max_new <= 4096;
+    return n_seqs <= 1024 && max_new <= 512 && (int64_t)n_seqs * max_new <= 4096;
 }
 
 void launch_reserve(const ReserveArgs& a, hipStream_t s, unsigned grid[3], unsigned* block,
