@@ -1,0 +1,144 @@
+"""The device-resident batch where its kernels differ: ranges of several steps and units at every padded
+head width, kv heads side by side or alone, non-finite values and pages outside the pool in each of
+those. Models, inputs and tolerances are those of test_gpu_batch.py.
+"""
+import numpy as np
+import pytest
+
+import _batch_model as model
+import flat_attention_amd as fa
+from test_gpu_batch import BF16, F16, F32, HALF_STEP, THETA, Case, i32, load, paged, storage
+
+pytestmark = pytest.mark.gpu
+
+
+# (storage, tokens, q heads, kv heads): one, two, four and eight row blocks, heads alone, in pairs and in
+# fours, one, two and four key groups
+KERNELS = [(BF16, 1, 8, 8), (F16, 3, 9, 3), (BF16, 12, 16, 4), (F16, 14, 9, 3), (BF16, 40, 8, 4), (F16, 65, 8, 2),
+           (F32, 1, 8, 8), (F32, 5, 6, 2), (F32, 3, 9, 3), (F32, 20, 8, 4), (F32, 65, 8, 2)]
+
+
+@pytest.mark.parametrize("D", [80, 128])
+@pytest.mark.parametrize("dtype,most,hq,hkv", KERNELS)
+@pytest.mark.parametrize("rope", [True, False])
+def test_several_steps_and_units_a_range_at_wide_heads(hip, dtype, most, hq, hkv, D, rope):
+    """More steps than there are ranges, several times over, of short and long sequences."""
+    rng = np.random.default_rng(most + D)
+    n = 60
+    ctx = np.where(rng.random(n) < 0.5, rng.integers(0, 60, n), rng.integers(1000, 3200, n))
+    ctx[:4] = [3001, 5, 0, 1999]
+    lens = rng.integers(0, most + 1, n)
+    lens[:4] = [most, most, 1, most]
+    Case(hip, dtype, ctx, lens, most, hq, hkv, D, 16, 31, rope=rope).check(only=[0, 1, 2, 3, 17, 29, 58, 59])
+
+
+def attend_by_head(q, k, v, sees, scale):
+    """model.attend with the rows of a head in one product (every row sees some key)."""
+    T, hq, D = q.shape
+    group, hide = hq // k.shape[1], np.where(sees, 0.0, -np.inf)
+    o, av, lse, size = np.zeros(q.shape), np.zeros(q.shape), np.zeros((hq, T)), np.zeros((hq, T))
+    for h in range(hq):
+        kk, vv = k[:, h // group], v[:, h // group]
+        s = scale * (q[:, h] @ kk.T) + hide
+        m = s.max(1)
+        p = np.exp(s - m[:, None])
+        l = p.sum(1)
+        o[:, h], av[:, h] = p @ vv / l[:, None], p @ np.abs(vv) / l[:, None]
+        lse[h] = m + np.log(l)
+        size[h] = np.where(sees, scale * (np.abs(q[:, h]) @ np.abs(kk).T), 0).max(1)
+    return o, lse, av, size
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D", [8, 80, 128])
+@pytest.mark.parametrize("page", [1, 2])
+def test_a_range_takes_its_table_entries_in_parts(hip, monkeypatch, dtype, D, page):
+    """So many rows that two ranges have all 3012 keys, more than a thousand pages each."""
+    monkeypatch.setattr(model, "attend", attend_by_head)
+    Case(hip, dtype, [2500 * page], [512], 512, 64, 1, D, page, 33).check()
+
+
+@pytest.mark.parametrize("dtype,most,hq,hkv,D", [
+    (BF16, 6, 8, 2, 128), (F16, 30, 8, 4, 80), (BF16, 70, 8, 2, 128), (F16, 5, 9, 3, 128), (F32, 1, 8, 8, 64),
+    (F32, 6, 4, 4, 128), (F32, 30, 4, 2, 80), (F32, 70, 8, 2, 128)])
+def test_pages_outside_the_pool_in_every_form(hip, dtype, most, hq, hkv, D):
+    case = Case(hip, dtype, [300, 90], [most, max(1, most - 1)], most, hq, hkv, D, 16, 34)
+    for s, lp, page in ((0, 2, -1), (0, 11, case.pages), (1, 0, 2147483647), (1, 3, -2147483648)):
+        case.table[s, lp] = page
+    case.batch.block_tables.upload(case.table.astype(np.int32))
+    o, lse = case.run()
+    for s in range(2):
+        c, m = int(case.ctx[s]), int(case.lens[s])
+        keys = np.arange(c + m)
+        there = (case.table[s, keys // 16] >= 0) & (case.table[s, keys // 16] < case.pages)
+        sees = np.ones((m, c + m), bool)
+        sees[:, c:] = case.sees[s, :m, :m]
+        at = np.where(there, case.table[s, keys // 16], 0).astype(np.int64) * 16 + keys % 16
+        eo, el, av, size = model.attend(model.rotate(case.q[s, :m], case.where[s, :m], THETA), case.k[at],
+                                        case.v[at], sees & there, float(np.float32(1) / np.sqrt(np.float32(D))))
+        h = HALF_STEP[dtype]
+        n = c + m
+        ds = size * ((D + 16) * 2.0 ** -24 + (h * h if dtype != F32 else 0))
+        tl = ds + n * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -22 * (np.abs(el) + size)
+        to = h * (np.abs(eo) + av) + (2 * ds.T[..., None] + n * 2.0 ** -23 + 2.0 ** -19) * av + 2.0 ** -25
+        assert (np.abs(lse[s, :, :m] - el) <= tl).all()
+        assert (np.abs(o[s, :m] - eo) <= to).all()
+
+
+@pytest.mark.filterwarnings("ignore:invalid value")
+@pytest.mark.parametrize("dtype,most,hq,hkv,D,ctx", [
+    (BF16, 6, 4, 2, 128, 40), (F16, 40, 8, 2, 128, 500), (BF16, 64, 8, 2, 80, 31), (F16, 33, 16, 2, 128, 2000),
+    (F16, 9, 6, 3, 80, 700), (F32, 6, 4, 4, 64, 900), (F32, 1, 8, 8, 128, 300), (F32, 12, 4, 4, 80, 70),
+    (F32, 20, 4, 2, 128, 333), (F32, 64, 8, 2, 128, 1000)])
+def test_special_values_reach_the_rows_that_see_them_in_every_form(hip, dtype, most, hq, hkv, D, ctx):
+    """NaN and infinities in V of drafted rows and of the last live rows, NaN in K of a drafted one."""
+    args = ([ctx, 5], [most, min(2, most)], most, hq, hkv, D, 16, 35)
+    clean = Case(hip, dtype, *args)
+    o0, l0 = clean.run()
+    case = Case(hip, dtype, *args)
+    group, rows = hq // hkv, case.rows(0, ctx + most)
+    sees = np.ones((most, ctx + most), bool)
+    sees[:, ctx:] = case.sees[0]
+    put = {x: fa.host_storage(np.array([x], np.float32), dtype)[0] for x in (np.nan, np.inf, -np.inf)}
+    spots = {(ctx + most - 1, 0, 3): np.nan, (ctx + most // 2, 0, 3): np.inf, (ctx, 1, D - 1): np.inf,
+             (ctx + most // 3, 1, D - 1): -np.inf, (ctx - 1, hkv - 1, 60): -np.inf, (ctx, 0, 17): -np.inf}
+    vs, want = case.vs.reshape(case.v.shape), np.zeros((most, hq, D))
+    for (key, head, d), x in spots.items():
+        vs[rows[key], head, d] = put[x]
+        want[:, head * group:(head + 1) * group, d] += np.where(sees[:, key], x, 0.0)[:, None]
+    case.upload()
+    o1, l1 = case.run()
+    assert np.array_equal(l1.view(np.uint32), l0.view(np.uint32))
+    hit = want != 0
+    assert hit.any()
+    assert np.array_equal(o1[0][~hit].view(np.uint32), o0[0][~hit].view(np.uint32))
+    assert np.array_equal(o1[1].view(np.uint32), o0[1].view(np.uint32))
+    assert np.array_equal(o1[0][hit], want[hit], equal_nan=True)
+    case.vs[:] = clean.vs
+    key = ctx + most // 2
+    case.ks.reshape(case.k.shape)[rows[key], hkv - 1, D - 2] = put[np.nan]
+    case.upload()
+    o2, l2 = case.run()
+    hit = np.zeros((most, hq), bool)
+    hit[:, (hkv - 1) * group:] = sees[:, key][:, None]
+    assert np.isnan(o2[0][hit]).all() and np.isnan(l2[0].T[hit]).all()
+    assert np.array_equal(o2[0][~hit].view(np.uint32), o0[0][~hit].view(np.uint32))
+    assert np.array_equal(l2[0].T[~hit].view(np.uint32), l0[0].T[~hit].view(np.uint32))
+
+
+@pytest.mark.parametrize("n,most,width,page,hkv,D", [(6, 20, 9, 5, 2, 64), (40, 64, 16, 16, 8, 128), (3, 30, 30, 24, 3, 8)])
+def test_accept_moves_f16_rows_like_the_model(hip, n, most, width, page, hkv, D):
+    rng = np.random.default_rng(most)
+    ctx, lens = rng.integers(0, 60, n), rng.integers(1, most + 1, n)
+    table, pages, _ = paged(rng, ctx + lens, page)
+    accepted = np.array([rng.integers(0, min(l, width) + 1) for l in lens])
+    paths = np.zeros((n, width), np.int64)
+    for s in range(n):
+        paths[s, :accepted[s]] = np.sort(rng.permutation(lens[s])[:accepted[s]])
+    (k, ks), (v, vs) = (storage(rng.standard_normal((pages * page, hkv * D)), F16) for _ in range(2))
+    kb, vb, c = fa.DeviceBuffer.from_array(hip, ks), fa.DeviceBuffer.from_array(hip, vs), i32(hip, ctx)
+    batch = fa.HipPagedBatch(hip, i32(hip, table), c, n, table.shape[1], page, pages)
+    batch.accept(i32(hip, paths), width, i32(hip, accepted), i32(hip, lens), kb, vb, hkv, D, F16)
+    ek, ev, ec = model.accept(k, v, table, ctx, paths, accepted, lens, page, pages, 512)
+    assert np.array_equal(c.download(np.int32, n), ec)
+    assert np.array_equal(load(kb, k.shape, F16), ek) and np.array_equal(load(vb, v.shape, F16), ev)
