@@ -625,8 +625,9 @@ void tree_split(TreeKArgs ka) {
                         }
                     }
                 }
+                // (the larger one of all units and parts of this range)
                 if constexpr (MASKED)
-                    if (__any(off != 0) && lane == 0) odd_lds[wave] = bad ? 2 : 1;
+                    if (__any(off != 0) && lane == 0) odd_lds[wave] = max(odd_lds[wave], bad ? 2 : 1);
             };
 
             // ---- the steps, NST - 1 transfers ahead: first those whose keys every row sees

@@ -142,3 +142,23 @@ def test_accept_moves_f16_rows_like_the_model(hip, n, most, width, page, hkv, D)
     ek, ev, ec = model.accept(k, v, table, ctx, paths, accepted, lens, page, pages, 512)
     assert np.array_equal(c.download(np.int32, n), ec)
     assert np.array_equal(load(kb, k.shape, F16), ek) and np.array_equal(load(vb, v.shape, F16), ev)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("ctx,lens,last,bad,live,drafted", [
+    ([1500], [512], 0, 1000, 1001, 2000), ([100, 100, 40, 40], [512, 512, 500, 490], 1, 20, 5, 400)])
+def test_infinity_beside_a_page_outside_the_pool(hip, dtype, ctx, lens, last, bad, live, drafted):
+    """An infinity that all rows see, among table entries with one outside the pool; behind them in the same range
+    (entries of the same sequence that follow, or another sequence) a drafted row that holds one too."""
+    case = Case(hip, dtype, ctx, lens, 512, 64, 1, 64, 1, 41)
+    vs = case.vs.reshape(case.v.shape)
+    for s, key, d in ((0, live, 3), (last, drafted, 9)):
+        vs[case.rows(s, key + 1)[key], 0, d] = fa.host_storage(np.array([np.inf], np.float32), dtype)[0]
+    case.upload()
+    case.table[0, bad] = case.pages
+    case.batch.block_tables.upload(case.table.astype(np.int32))
+    o, lse = case.run()
+    want = np.zeros(o.shape, bool)
+    want[0, :lens[0], :, 3] = True
+    want[last, case.sees[last, :, drafted - ctx[last]], :, 9] = True
+    assert np.isposinf(o[want]).all() and np.isfinite(o[~want]).all()
