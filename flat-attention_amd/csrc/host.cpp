@@ -3270,6 +3270,9 @@ int fa_backward_recompute_mha(fa_ctx* ctx, const void* packed_forward, size_t fo
 namespace {
 
 constexpr uint64_t kBatchSeqs = 1 << 20;  // sequences of a batch
+// Tokens of a table row, and slots: the kernels round them up to whole steps and step past their end in
+// 32 bits, by less than 1024.
+constexpr uint64_t kBatchIndex = kI32 - 1023;
 
 // Sizes and index ranges of a batch; `tables`: its block tables are used. *capacity: tokens a row holds.
 int check_batch(const fa_paged_batch* b, bool tables, uint64_t* capacity) {
@@ -3284,7 +3287,7 @@ int check_batch(const fa_paged_batch* b, bool tables, uint64_t* capacity) {
                     (unsigned long long)b->n_seqs, (unsigned long long)kBatchSeqs);
     uint64_t entries, rows;
     if (mul_ov(b->page_size, b->physical_pages, &rows) || rows > kI32 ||
-        mul_ov(b->max_pages, b->page_size, capacity) || *capacity > kI32 ||
+        mul_ov(b->max_pages, b->page_size, capacity) || *capacity > kBatchIndex ||
         mul_ov(b->n_seqs, b->max_pages, &entries) || entries > kI32)
         return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the i32 index space");
     if (int rc = check_buffer("context lengths", b->ctx_lens, b->ctx_lens_bytes, b->n_seqs * 4))
@@ -3343,7 +3346,7 @@ int fa_paged_reserve_slots(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* 
     if (int rc = check_batch(b, true, &capacity)) return rc;
     if (!max_new) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
     const uint64_t n = b->n_seqs;
-    if (mul_ov(n, max_new, &n_slots) || n_slots > kI32)
+    if (mul_ov(n, max_new, &n_slots) || n_slots > kBatchIndex)
         return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "slot map exceeds the i32 index space");
     if (int rc = check_buffer("new lengths", new_lens, new_lens_bytes, n * 4)) return rc;
     if (int rc = check_buffer("mapped pages", mapped, mapped_bytes, n * 4)) return rc;

@@ -555,7 +555,8 @@ typedef struct fa_paged_batch {
     size_t block_tables_bytes;
     int32_t* ctx_lens;          /* device [n_seqs] live tokens */
     size_t ctx_lens_bytes;
-    uint64_t n_seqs, max_pages, page_size, physical_pages; /* n_seqs <= 2^20 */
+    /* n_seqs <= 2^20, max_pages * page_size <= 2^31 - 1024 */
+    uint64_t n_seqs, max_pages, page_size, physical_pages;
 } fa_paged_batch;
 
 /* Slots for the new tokens of every sequence, in sequence order. All arrays are device int32:
@@ -572,7 +573,7 @@ typedef struct fa_paged_batch {
  *                       it needs pages and the free ones do not cover it and all sequences before it
  *                       that fit their row. Its pages stay as they were.
  *   slots [n_seqs, max_new]  pool row (page * page_size + offset) of token ctx_lens[s] + t, -1 for
- *                       t >= granted[s] (and on a page id outside the pool)
+ *                       t >= granted[s] (and on a page id outside the pool); n_seqs * max_new <= 2^31 - 1024
  * Lengths of sequences that go on are left for fa_paged_accept or the caller to advance. */
 int fa_paged_reserve_slots(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* new_lens,
                            size_t new_lens_bytes, uint64_t max_new, const int32_t* mapped,

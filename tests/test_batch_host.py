@@ -189,3 +189,17 @@ def test_python_mirror_names_the_error():
         b.tree_masks(Buf, Buf, 1, Buf, Buf)
     assert e.value.variant == "BufferTooSmall"
     assert b.layout(3, 4, 8, fa.DTYPE_BF16).lse_elements == 24
+
+
+def test_lengths_leave_room_for_whole_steps():
+    """The kernels round a length up to whole steps, and step past its end, in 32 bits."""
+    most = (1 << 31) - 1024
+    for call in CALLS:
+        assert call(batch(n=1, max_pages=most, page=1, pages=1)) == "NullArgument"
+        assert "context is null" in L.lib().fa_last_error_message().decode()
+        assert call(batch(n=1, max_pages=most + 1, page=1, pages=1)) == "IndexSpaceExceeded"
+        assert call(batch(n=1, max_pages=1, page=most + 1, pages=1)) == "IndexSpaceExceeded"
+    one = batch(n=1)
+    assert reserve(one, max_new=most) == "NullArgument"
+    assert "context is null" in L.lib().fa_last_error_message().decode()
+    assert reserve(one, max_new=most + 1) == reserve(one, max_new=(1 << 31) - 1) == "IndexSpaceExceeded"
