@@ -1087,14 +1087,38 @@ static TreeShape tree_shape(Dtype dt, const TreeArgs& a) {
     return dt == Dtype::F32 ? shape_t<float>(a) : shape_t<bf16_t>(a);  // (the 16-bit types alike)
 }
 
+// What the partials of a launch take on one CU: rows (with hw heads of rw row blocks), bytes of O, workgroups.
+// The most of any shape that tree_dispatch chooses.
+struct TreeMost {
+    int rows, bytes, groups;
+};
+template <typename T, int DPAD, int RW, int HW>
+static constexpr TreeMost most_of(TreeMost m) {
+    using C = TreeCfg<T, DPAD, RW, HW>;
+    constexpr int rows = C::PER_CU * C::ROWS * HW;
+    return {std::max(m.rows, rows), std::max(m.bytes, rows * DPAD * 4), std::max(m.groups, C::PER_CU)};
+}
+template <int DPAD>
+static constexpr TreeMost most_with(TreeMost m) {
+    m = most_of<bf16_t, DPAD, 1, 1>(most_of<bf16_t, DPAD, 1, 2>(m));
+    m = most_of<bf16_t, DPAD, 2, 1>(most_of<bf16_t, DPAD, 2, 2>(m));
+    m = most_of<bf16_t, DPAD, 4, 1>(most_of<bf16_t, DPAD, 8, 1>(m));
+    m = most_of<float, DPAD, 1, 1>(most_of<float, DPAD, 1, 2>(most_of<float, DPAD, 1, 4>(m)));
+    return most_of<float, DPAD, 2, 1>(most_of<float, DPAD, 4, 1>(m));
+}
+
+// The same partials for every shape and type (69 MB on 256 CUs), so that no later call of up to as many
+// sequences has to allocate: a shape's own need is not monotone in it (65 to 128 16-bit rows of 64 dims have
+// more workgroups than 256 rows, and row blocks that do not divide the workgroups leave some out). A single
+// range, which more row blocks than workgroups have, leaves no partials.
 size_t tree_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset,
                       size_t* odd_offset) {
-    const TreeShape s = tree_shape(dt, a);
-    const size_t rows = (size_t)2 * s.ranges * s.row_blocks * 32 * s.rw * s.hw;
-    *ml_offset = rows * (a.head_dim <= 64 ? 64 : 128) * 4;
-    *plan_offset = *ml_offset + rows * 8;
+    constexpr TreeMost most = most_with<64>(most_with<128>({0, 0, 0}));
+    const size_t cus = (size_t)device_cus();
+    *ml_offset = 2 * cus * most.bytes;
+    *plan_offset = *ml_offset + 2 * cus * most.rows * 8;
     *odd_offset = *plan_offset + ((size_t)a.n_seqs + 2) * 4;
-    return *odd_offset + (size_t)s.ranges * s.row_blocks * 4;
+    return *odd_offset + std::max<size_t>(cus * most.groups, tree_shape(dt, a).row_blocks) * 4;
 }
 
 template <typename T>

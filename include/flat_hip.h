@@ -543,9 +543,11 @@ int fa_paged_append_batched(fa_ctx* ctx, const int32_t* block_tables, uint64_t m
  * without the host: slots are reserved, the drafted rows appended, attended over and the accepted
  * ones moved into place by calls that read every length on the device. No counterpart in the
  * reference, whose tables are host metadata (PagedKvTable src/paged_kv.rs:76). The calls only enqueue
- * kernels (capturable once the context's workspaces and (cos, sin) table are sized, by one earlier
- * call of the same or a larger shape) and give the same results each time. The pool is that of the
- * paged cache and decode: [physical_pages, page_size, kv_heads*head_dim], K stored rotated.
+ * kernels and give the same results each time. They can be captured once the context's workspaces are
+ * sized, by one earlier call of the same or a larger shape of any type, and, where they rotate, its
+ * (cos, sin) table is that of their theta and head_dim, by an earlier call with those and positions as
+ * far. The pool is that of the paged cache and decode: [physical_pages, page_size, kv_heads*head_dim],
+ * K stored rotated.
  *
  * The host cannot check what device arrays hold. A sequence, token, slot or page that does not fit
  * takes no part, as each call says; nothing outside the buffers is read or written. Pools, K/V

@@ -162,3 +162,27 @@ def test_infinity_beside_a_page_outside_the_pool(hip, dtype, ctx, lens, last, ba
     want[0, :lens[0], :, 3] = True
     want[last, case.sees[last, :, drafted - ctx[last]], :, 9] = True
     assert np.isposinf(o[want]).all() and np.isfinite(o[~want]).all()
+
+
+@pytest.mark.parametrize("first,then", [
+    ((F16, 64, 4, 1, 64), (F16, 32, 4, 1, 64)), ((BF16, 192, 4, 1, 128), (BF16, 128, 4, 1, 128)),
+    ((F32, 40, 4, 4, 128), (F32, 8, 4, 4, 128)), ((BF16, 9, 8, 4, 128), (F16, 9, 8, 4, 128))])
+def test_an_earlier_larger_call_sizes_the_workspaces(first, then):
+    """A call captured before its shape has run eagerly, after one larger call on a new context."""
+    ctx = fa.HipContext(0)
+    try:
+        for k, (dtype, most, hq, hkv, D) in enumerate((first, then)):
+            case = Case(ctx, dtype, [300, 20, 7][k:], [most, 3, 5][k:], most, hq, hkv, D, 16, 44)
+            if k == 0:
+                case.check()
+        case.keep = fa.DeviceBuffer.from_array(ctx, case.masks), i32(ctx, case.pos)
+        with ctx.capture() as cap:
+            case.call(upload=False)
+        for _ in range(3):
+            case.out.fill_u32(0x7fc07fc0)
+            cap.graph.launch()
+            o0, l0 = case.get()
+            o1, l1 = case.check()
+            assert np.array_equal(o0, o1) and np.array_equal(l0, l1)
+    finally:
+        ctx.close()
