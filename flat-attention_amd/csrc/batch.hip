@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256) void reserve_fill(ReserveKArgs ka, int parts) 
 // One workgroup writes everything up to here: beyond it a second launch over the whole chip. Fused / not
 // (us): 16 sequences of 16 tokens 5.0 / 8.8, 64 of 16 7.1 / 8.8, 64 of 64 8.6 / 8.9, 256 of 16 10.0 / 10.3,
 // 256 of 32 15.3 / 10.5; 8 of 512 7.9 / 8.0, 1 of 2048 (a sequence has 64 threads) 9.4 / 8.0.
-bool reserve_fused(int n_seqs, int max_new) {
+static bool reserve_fused(int n_seqs, int max_new) {
     return n_seqs <= 1024 && max_new <= 512 && (int64_t)n_seqs * max_new <= 4096;
 }
 

@@ -3360,10 +3360,9 @@ int fa_paged_reserve_slots(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* 
     begin_call(ctx);
     if (int rc = set_device(ctx)) return rc;
     fa::ReserveArgs a{};
-    if (!fa::reserve_fused((int)n, (int)max_new))
-        if (int rc = grow(ctx, &ctx->ws_plan, &ctx->ws_plan_bytes, (n + 1) * sizeof(int4),
-                          (void**)&a.plan))
-            return rc;
+    // (also where one launch does without: a later one of fewer sequences may not)
+    if (int rc = grow(ctx, &ctx->ws_plan, &ctx->ws_plan_bytes, (n + 1) * sizeof(int4), (void**)&a.plan))
+        return rc;
     a.block_tables = b->block_tables;
     a.ctx_lens = b->ctx_lens;
     a.new_lens = new_lens;

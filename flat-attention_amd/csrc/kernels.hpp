@@ -321,7 +321,7 @@ void launch_rotate_rows(Dtype dt, const void* in, void* out, int rows, int heads
 constexpr int kTreeTokens = 512;
 
 // Slots for new tokens from request lengths (all pointers on the device). `plan` is scratch of
-// n_seqs + 1 entries, used where reserve_fused() is false.
+// n_seqs + 1 entries, which calls of two launches use.
 struct ReserveArgs {
     int* block_tables;  // [n_seqs, max_pages]
     int* ctx_lens;      // [n_seqs], zeroed for ended sequences
@@ -336,7 +336,6 @@ struct ReserveArgs {
     int4* plan;
     int n_seqs, max_pages, max_new, page_size, physical_pages, free_capacity;
 };
-bool reserve_fused(int n_seqs, int max_new);
 void launch_reserve(const ReserveArgs& a, hipStream_t s, unsigned grid[3], unsigned* block,
                     unsigned* dispatches);
 

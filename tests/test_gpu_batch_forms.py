@@ -186,3 +186,28 @@ def test_an_earlier_larger_call_sizes_the_workspaces(first, then):
             assert np.array_equal(o0, o1) and np.array_equal(l0, l1)
     finally:
         ctx.close()
+
+
+def test_an_earlier_reservation_sizes_the_plan():
+    """One of more sequences and slots in one launch, then a captured one that takes two."""
+    ctx = fa.HipContext(0)
+    try:
+        for n, max_new in ((100, 40), (7, 570)):
+            page, width, pages = 16, 40, 300
+            table, lens, new = np.full((n, width), -1), np.zeros(n, np.int64), np.full(n, max_new)
+            free = np.arange(pages)
+            state = [i32(ctx, x) for x in (table, lens, new, lens, free, [pages])]
+            t, c, nl, m, f, k = state
+            granted, slots = i32(ctx, np.full(n, 77)), i32(ctx, np.full((n, max_new), 77))
+            batch = fa.HipPagedBatch(ctx, t, c, n, width, page, pages)
+            if n == 100:
+                batch.reserve(nl, max_new, m, f, k, granted, slots)
+        with ctx.capture() as cap:
+            batch.reserve(nl, max_new, m, f, k, granted, slots)
+        cap.graph.launch()
+        want = model.reserve(table, lens, new, lens, free, pages, max_new, page, pages)
+        assert np.array_equal(granted.download(np.int32, n), want["granted"])
+        assert np.array_equal(slots.download(np.int32, n * max_new).reshape(n, max_new), want["slots"])
+        assert k.download(np.int32, 1)[0] == want["count"]
+    finally:
+        ctx.close()
