@@ -29,7 +29,10 @@ namespace fa {
 // (none counted). Rows that do not exist, and dims past head_dim, are fetched from 16 zero bytes.
 // 16-bit storage: the rotated Q is kept as a 16-bit high part and the rounding of its residual, two
 // MFMAs a step, so that scores and LSE carry f32 accuracy; P is rounded once to the storage type (its
-// sum is taken before), an error of the size of O's own rounding.
+// sum is taken before), an error of the size of O's own rounding. f16 has no normal numbers below 2^-14 and
+// nothing below 2^-25: its P is kept 2^7 times as large (at most 2^15, as the running maximum may lag by
+// 2^8), so that a key loses 2^-32 of the largest one's weight at most, and 10^5 small ones beside a large
+// one 2^-15 of O.
 //
 // The lengths are known on the GPU only, so the launch has a fixed number of workgroups; each finds its
 // share by a prefix sum over the sequences: the steps (KT keys) of all (sequence, kv head) units laid
@@ -102,6 +105,14 @@ struct TreeCfg {
     // f32 quads of a 32-row block in a partial, in the order that the waves hold them
     static constexpr int QUADS = 8 * DPAD;
 };
+
+// The power of two by which P and its sum are kept larger.
+template <typename T> constexpr int kTreeLift = std::is_same<T, f16_t>::value ? 7 : 0;
+// What is added to a score's c2-fold before exp2.
+template <typename T>
+__device__ __forceinline__ float exponent_of(float m, float c2) {
+    return kTreeLift<T> ? fmaf(-m, c2, (float)kTreeLift<T>) : -m * c2;
+}
 
 // Which column a piece of an LDS row is kept in: piece ^ swizzle(row). 16 columns of 16 bytes are the 64
 // banks. K is read one row a lane (8 rows at a time have to lie in different columns), V with four rows
@@ -200,7 +211,7 @@ __device__ __forceinline__ void write_row4(const TreeArgs& a, int s, int kvh, in
                                                    Half<T>::pack(o[2] * inv, o[3] * inv)};
     if (d == 0)
         a.lse[((int64_t)s * a.q_heads + hq) * a.max_tokens + t] =
-            none ? -INFINITY : m * a.scale + logf(l);
+            none ? -INFINITY : m * a.scale + logf(l * (1.0f / (1 << kTreeLift<T>)));
 }
 
 // Inclusive prefix sum over a wave (row shifts by 1, 2, 4, 8, then the last lane of each row of 16 to
@@ -556,7 +567,7 @@ void tree_split(TreeKArgs ka) {
                     m_run = m_use;
                 }
                 // (MASKED: maybe no key seen yet)
-                const float neg = MASKED && m_run == -INFINITY ? 0.0f : -m_run * c2;
+                const float neg = MASKED && m_run == -INFINITY ? 0.0f : exponent_of<T>(m_run, c2);
                 float ls = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -717,7 +728,7 @@ void tree_split(TreeKArgs ka) {
                             mt = fmaxf(mt, xor32(mt));
                             const bool need = mt * c2 > m_run * c2 + 8.0f;
                             const float m_use = need ? mt : m_run;
-                            const float neg = -m_use * c2;
+                            const float neg = exponent_of<T>(m_use, c2);
                             float ls = 0.0f;
                             u32x4_t pb[2];
 #pragma unroll

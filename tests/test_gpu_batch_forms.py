@@ -211,3 +211,34 @@ def test_an_earlier_reservation_sizes_the_plan():
         assert k.download(np.int32, 1)[0] == want["count"]
     finally:
         ctx.close()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("most,hq,hkv", [(1, 4, 1), (1, 4, 2), (20, 2, 1), (20, 4, 1), (40, 4, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_small_probabilities_beside_large_ones(hip, dtype, most, hq, hkv, D):
+    """One score in 32 is 17.625 (25.4 powers of two) above the others, and its V is 0, so O is what the small ones
+    add up to. f16: besides its relative rounding each of them may lose half a step of the smallest numbers, 2^-25
+    of the 2^7-fold of the largest probability; their sum is at least that of the large ones, one a run of 32."""
+    n = 1500 + most
+    case = Case(hip, dtype, [1500], [most], most, hq, hkv, D, 16, 43, tree=False, rope=False, scale=1.0)
+    at = case.rows(0, n)
+    q, k, v = np.zeros(case.q.shape), np.zeros(case.k.shape), np.zeros(case.v.shape)
+    q[..., 0] = 1.0
+    k[at[7::32], :, 0] = 17.625
+    v[at] = 1024.0
+    v[at[7::32]] = 0.0
+    (q, qs), (k, case.ks), (v, case.vs) = (storage(x, dtype) for x in (q, k, v))
+    case.bufs[0].upload(qs)
+    case.upload()
+    o, lse = case.run()
+    sees = np.ones((most, n), bool)
+    sees[:, 1500:] = np.tril(np.ones((most, most), bool))
+    eo, el, av, size = model.attend(q[0], k[at], v[at], sees, 1.0)
+    ds = size * (D + 16) * 2.0 ** -24
+    tl = ds + n * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -22 * (np.abs(el) + size)
+    to = HALF_STEP[dtype] * (eo + av) + (2 * ds.T[..., None] + n * 2.0 ** -23 + 2.0 ** -19) * av
+    if dtype == F16:
+        to += 2.0 ** -25 + n * 2.0 ** -32 * 1024 / (1500 // 32)
+    assert (np.abs(lse[0] - el) <= tl).all()
+    assert (np.abs(o[0] - eo) <= to).all()
