@@ -126,7 +126,8 @@ def test_special_values_reach_the_rows_that_see_them_in_every_form(hip, dtype, m
     assert np.array_equal(l2[0].T[~hit].view(np.uint32), l0[0].T[~hit].view(np.uint32))
 
 
-@pytest.mark.parametrize("n,most,width,page,hkv,D", [(6, 20, 9, 5, 2, 64), (40, 64, 16, 16, 8, 128), (3, 30, 30, 24, 3, 8)])
+@pytest.mark.parametrize("n,most,width,page,hkv,D", [(6, 20, 9, 5, 2, 64), (40, 64, 16, 16, 8, 128),
+                                                     (3, 30, 30, 24, 3, 8)])
 def test_accept_moves_f16_rows_like_the_model(hip, n, most, width, page, hkv, D):
     rng = np.random.default_rng(most)
     ctx, lens = rng.integers(0, 60, n), rng.integers(1, most + 1, n)
@@ -242,3 +243,83 @@ def test_many_small_probabilities_beside_large_ones(hip, dtype, most, hq, hkv, D
         to += 2.0 ** -25 + n * 2.0 ** -32 * 1024 / (1500 // 32)
     assert (np.abs(lse[0] - el) <= tl).all()
     assert (np.abs(o[0] - eo) <= to).all()
+
+
+@pytest.mark.parametrize("dtype,page", [(BF16, 16), (F32, 24)])
+def test_pools_of_more_than_four_gib(hip, dtype, page):
+    """The same rows in the first pages of a pool of 5 GiB and in its last: appended, attended and moved alike."""
+    n, most, hq, hkv, D, ctx = 2, 9, 8, 4, 128, 70
+    row = hkv * D * (4 if dtype == F32 else 2)
+    pages = (5 << 30) // (page * row)
+    rng = np.random.default_rng(45)
+    new = {x: rng.standard_normal((n, most, h, D)).astype(np.float32) for x, h in (("q", hq), ("k", hkv), ("v", hkv))}
+    old = [rng.standard_normal((n, ctx, hkv, D)).astype(np.float32) for _ in range(2)]
+    width = -(-(ctx + most) // page)
+    pools = [fa.DeviceBuffer(hip, pages * page * row) for _ in range(2)]
+
+    def put(x):
+        return fa.DeviceBuffer.from_array(hip, fa.host_storage(np.ascontiguousarray(x).ravel(), dtype))
+
+    def through(first):
+        table = first + np.arange(n * width).reshape(width, n).T
+        at = np.arange(ctx + most)
+        rows = table[:, at // page] * page + at % page
+        lens = i32(hip, [ctx] * n)
+        batch = fa.HipPagedBatch(hip, i32(hip, table), lens, n, width, page, pages)
+        batch.append(i32(hip, rows[:, :ctx]), ctx, put(old[0]), put(old[1]), *pools, hkv, D, None, dtype)
+        batch.append(i32(hip, rows[:, ctx:]), most, put(new["k"]), put(new["v"]), *pools, hkv, D, None, dtype)
+        lay = batch.layout(most, hq, D, dtype)
+        out, q = fa.DeviceBuffer(hip, lay.combined_bytes), put(new["q"])
+        results = []
+        for tokens in (most, 3):
+            batch.tree_attention(q, *pools, out, i32(hip, [tokens] * n), most, hq, hkv, D, fa.FlatAttentionConfig(),
+                                 fa.RotaryEmbeddingConfig(THETA), dtype)
+            r = fa.download_attention(out, lay, dtype)
+            results += [r.output, r.lse]
+            if tokens == most:
+                batch.accept(i32(hip, [[0, 4, 8]] * n), 3, i32(hip, [3] * n), i32(hip, [most] * n), *pools, hkv, D,
+                             dtype)
+                results.append(lens.download(np.int32, n))
+        for pool in pools:
+            results.append(np.stack([pool.download(np.uint8, row, int(r) * row) for r in rows[:, ctx:ctx + 3].ravel()]))
+        return results
+
+    low, high = through(0), through(pages - n * width)
+    assert np.isfinite(low[1]).all()
+    for a, b in zip(low, high):
+        assert np.array_equal(a, b)
+
+
+def test_the_most_sequences(hip):
+    """2^20 sequences of one token each: the largest batch."""
+    n, page, D = 1 << 20, 16, 8
+    rng = np.random.default_rng(46)
+    q, k, v = (storage(rng.standard_normal((n, 1, D)).astype(np.float32), BF16) for _ in range(3))
+    pool = [fa.DeviceBuffer(hip, n * page * D * 2) for _ in range(2)]
+    t, c, m, new = (i32(hip, np.full(n, x)) for x in (-1, 0, 0, 1))
+    free, count = i32(hip, np.arange(n)), i32(hip, [n - 5])
+    granted, slots = i32(hip, np.full(n, 77)), i32(hip, np.full(n, 77))
+    batch = fa.HipPagedBatch(hip, t, c, n, 1, page, n)
+    batch.reserve(new, 1, m, free, count, granted, slots)
+    got = np.arange(n) < n - 5
+    assert np.array_equal(granted.download(np.int32, n), got)
+    assert np.array_equal(t.download(np.int32, n), np.where(got, n - 6 - np.arange(n), -1))
+    assert np.array_equal(slots.download(np.int32, n), np.where(got, (n - 6 - np.arange(n)) * page, -1))
+    assert count.download(np.int32, 1)[0] == 0 and np.array_equal(m.download(np.int32, n), got)
+    parents, masks, pos = i32(hip, np.full(n, -1)), fa.DeviceBuffer(hip, n * 8), i32(hip, np.full(n, 77))
+    batch.tree_masks(parents, granted, 1, masks, pos)
+    assert np.array_equal(masks.download(np.uint64, n), got) and np.array_equal(pos.download(np.int32, n), got - 1)
+    qb, kb, vb = (fa.DeviceBuffer.from_array(hip, x[1]) for x in (q, k, v))
+    batch.append(slots, 1, kb, vb, *pool, 1, D, None, BF16)
+    lay = batch.layout(1, 1, D, BF16)
+    out = fa.DeviceBuffer(hip, lay.combined_bytes)
+    batch.tree_attention(qb, *pool, out, granted, 1, 1, 1, D, fa.FlatAttentionConfig(softmax_scale=0.5), None, BF16,
+                         positions=pos, masks=masks)
+    r = fa.download_attention(out, lay, BF16)
+    o = fa.storage_to_f32(r.output, BF16).reshape(n, 1, D)
+    assert np.array_equal(o[got], v[0][got]) and (o[~got] == 0).all() and np.isneginf(r.lse[~got]).all()
+    want = 0.5 * (q[0] * k[0]).sum((1, 2))
+    size = 0.5 * np.abs(q[0] * k[0]).sum((1, 2))
+    assert (np.abs(r.lse - want)[got] <= (size * (D + 16) * 2.0 ** -24 + 2.0 ** -22 * (np.abs(want) + size))[got]).all()
+    batch.accept(i32(hip, np.zeros(n)), 1, granted, granted, *pool, 1, D, BF16)
+    assert np.array_equal(c.download(np.int32, n), got)
