@@ -176,7 +176,8 @@ def test_an_earlier_larger_call_sizes_the_workspaces(first, then):
             case = Case(ctx, dtype, [300, 20, 7][k:], [most, 3, 5][k:], most, hq, hkv, D, 16, 44)
             if k == 0:
                 case.check()
-        case.keep = fa.DeviceBuffer.from_array(ctx, case.masks), i32(ctx, case.pos)
+        # (held here: the graph reads them, and an eager run makes others)
+        held = case.keep = fa.DeviceBuffer.from_array(ctx, case.masks), i32(ctx, case.pos)
         with ctx.capture() as cap:
             case.call(upload=False)
         for _ in range(3):
@@ -185,6 +186,7 @@ def test_an_earlier_larger_call_sizes_the_workspaces(first, then):
             o0, l0 = case.get()
             o1, l1 = case.check()
             assert np.array_equal(o0, o1) and np.array_equal(l0, l1)
+        del held
     finally:
         ctx.close()
 
