@@ -28,8 +28,8 @@ namespace fa {
 // One sequence 4.7 us, the smallest a call takes; 256 of up to 2048 tokens, 24 ended, 11.0 (17.8 with four
 // slots a thread and each wave putting back the pages of its own ended sequences).
 
-// What reserve_fill has to know of a sequence: pages that stay, tokens granted (-1: none, 0 tokens),
-// and the exclusive prefix sum of the pages it takes.
+// What reserve_fill has to know of a sequence: pages that stay, tokens granted, the exclusive prefix sum of
+// the pages taken, and how many it takes.
 struct ReservePlan {
     int kept, granted, first, taken;
 };

@@ -41,14 +41,16 @@ namespace fa {
 // tree_combine merges in their order.
 //
 // What bounds it (both launches, Hq32 Hkv8 D128 bf16, pages of 16 rows, contexts of 512..8192):
-//   64 sequences, one token: 1.16 GB in 195 us, 5.95 TB/s; memory (a copy reaches 5.16 TB/s here, loads
+//   64 sequences, one token: 1.16 GB in 192 us, 6.0 TB/s; memory (a copy reaches 5.16 TB/s here, loads
 //     alone 6.75). What is left is each unit's start, while its workgroup does not stream.
 //   24 sequences, 16 / 32 / 64 tokens each: 92 / 103 / 163..178 us (by the box). 64 tokens fill 256
-//     rows: the matrix core runs 65 % of a step of 64 keys (4850 cycles, 3170 of them MFMA: two waves a
-//     SIMD, whose softmax and products overlap only in part), and a unit's start (its lengths, table
-//     entries, Q with its angles, first tile, masked blocks, end) takes as long as six steps.
-//   One sequence, 5 tokens, 1000 keys, Hq16 Hkv4 D64: 12.8 us, the latency of two launches and of four
-//     dependent loads in the first (lengths; table entries; Q; tile).
+//     rows: the matrix cores are busy 0.47 of the CUs' busy cycles, 0.51 over contexts of 16384 (trees of 32
+//     to 64 tokens leave a fifth of the waves without rows; two waves a SIMD, whose softmax and products
+//     overlap only in part), and a unit's start (its lengths, table entries, Q with its angles, first tile,
+//     masked blocks, end) takes as long as six steps.
+//   One sequence, 5 tokens, 1000 keys, Hq16 Hkv4 D64: 12.9 us, the latency of two launches (8 and 5) and of
+//     four dependent loads in the first (lengths; table entries; Q; tile). Its 32 steps are one range each,
+//     and consecutive ranges run on one XCD, here all on the first.
 // The simplest kernel of this layout (operands read by each lane from memory, no stages) took 7254, 20521
 // and 205 us for the first, the 64-token and the last of these.
 
@@ -62,7 +64,8 @@ constexpr int kTreePages = 1024;  // block-table entries held in LDS at a time
 // Steps that the start of a unit counts for in the split (its table entries, Q, first tile, masked keys and
 // end take as long), but at most half of a range's steps: with few steps a range the split would be uneven.
 // 24 trees of 64 tokens over 512..8192 bf16 keys, Hq32 Hkv8: 198 us with 0, 189 / 182 / 184 / 192 with 3 / 6
-// / 9 / 14; 64 single tokens 212 / 209 / 210 / 213 / 212.
+// / 9 / 14; 64 single tokens 212 / 209 / 210 / 213 / 212. (Measured at these two shapes of 128 dims; other
+// types and row counts, whose steps are shorter or longer, take the same.)
 constexpr int kTreeStart = 6;
 
 // RW row blocks of 32 rows, HW kv heads side by side: NW / RW groups of waves, of which HW KW = NW / RW

@@ -551,7 +551,10 @@ int fa_paged_append_batched(fa_ctx* ctx, const int32_t* block_tables, uint64_t m
  *
  * The host cannot check what device arrays hold. A sequence, token, slot or page that does not fit
  * takes no part, as each call says; nothing outside the buffers is read or written. Pools, K/V
- * sources, Q and outputs start at multiples of 16 bytes (FA_ERR_MISALIGNED). */
+ * sources, Q and outputs start at multiples of 16 bytes (FA_ERR_MISALIGNED); head_dim is a multiple of 8
+ * (f32: of 4), and at most 128 where the call rotates or attends. The context's workspaces hold what a
+ * call leaves for its second launch: a graph captured from one context and launched through another
+ * must not run beside calls or graphs of the first. */
 typedef struct fa_paged_batch {
     int32_t* block_tables;      /* device [n_seqs, max_pages] physical page ids */
     size_t block_tables_bytes;
@@ -568,7 +571,8 @@ typedef struct fa_paged_batch {
  *                       the new counts
  *   free_pages          stack of free page ids, free_count of them from the start (capacity:
  *                       free_pages_bytes / 4); pages come from its end, the last first, and those of
- *                       ended sequences are put on it before any is taken, in sequence order;
+ *                       ended sequences are put on it before any is taken, in sequence order (those
+ *                       that its capacity does not hold are lost);
  *                       free_count_out (may be the same) receives the new count
  *   granted [n_seqs]    new_lens, or 0 for a sequence that got no slots: it ended, it asks for none or
  *                       for more than max_new or its table row can hold, its length is negative, or
@@ -601,7 +605,7 @@ int fa_paged_tree_masks(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t*
  * max_new] (fa_paged_reserve_slots), K rotated at rotary->position_offset + positions[s, t]
  * (positions == NULL: ctx_lens[s] + t) when rotary != NULL. Rows with a slot outside the pool, or a
  * position outside [0, max_pages * page_size) when rotating, are left out; two rows must not share a
- * slot. block_tables are not used (may be null). head_dim: a multiple of 8 (f32: of 4). */
+ * slot. block_tables are not used (may be null). */
 int fa_paged_append_slots(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* slots,
                           size_t slots_bytes, const int32_t* positions, size_t positions_bytes,
                           uint64_t max_new, const void* k_src, const void* v_src,
@@ -619,7 +623,8 @@ int fa_paged_append_slots(fa_ctx* ctx, const fa_paged_batch* batch, const int32_
  * outside [0, max_pages * page_size) when rotating, and all rows of a sequence whose lengths are
  * negative or do not fit max_tokens and its table, get O = 0 and LSE = -inf. Keys on a page id outside
  * the pool are as if masked, and what masked rows and rows past the live ones hold, NaN and
- * infinities too, reaches no result. */
+ * infinities too, reaches no result. A row that sees a K which is not finite may be NaN, and a column in
+ * which it sees an infinite V may be NaN where that key's probability rounds to zero. */
 int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* batch, const void* q, size_t q_bytes,
                             const void* k_pool, const void* v_pool, size_t pool_bytes,
                             void* out_lse, size_t out_bytes, const int32_t* tree_lens,
