@@ -164,6 +164,12 @@ __device__ __forceinline__ void rows16(const uint8_t* ld, int g, float (&l2)[16]
 constexpr int kBwdKeys = 128;     // keys per bwd_dkdv workgroup (32 per wave)
 constexpr int kBwdQueries = 128;  // queries per bwd_dq workgroup (32 per wave)
 constexpr int kBwdTile = 64;      // rows per staged tile (Q/dO in bwd_dkdv, K/V in bwd_dq)
+template <bool WIN> using split_of = std::conditional_t<WIN, WindowSplit, BackwardSplit>;
+// Past the last query that sees a key of key block kb, with a window.
+__device__ __host__ __forceinline__ int window_end(const BackwardArgs& a, int kb) {
+    const int64_t end = (int64_t)(kb + 1) * kBwdKeys - 1 + a.window;
+    return kb * kBwdKeys < a.sinks || end > a.seq ? a.seq : (int)end;
+}
 constexpr uint32_t kOob = 0x7fff0000u;  // transfer offset past every buffer: writes zeros
 
 #define FA_BWD_SG(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
@@ -341,8 +347,10 @@ __global__ __launch_bounds__(256) void bwd_delta(BackwardArgs a, int64_t rows) {
 // Few key blocks (sp.parts > 1): the tiles of a key block are dealt to several workgroups in chunks
 // of sp.chunk; each writes its dK and dV, unscaled, to its slot of sp.part, and the dQ launch adds
 // them up in chunk order (add_partials).
-template <typename T, int DPAD, bool DMA, bool DSO = false>
-__global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, BackwardSplit sp) {
+// WIN (launch_backward_window): position i sees the keys j <= i with i - j < window or j < sinks, so a key
+// block without sinks has the query tiles from its own to the window's end only (WindowSplit).
+template <typename T, int DPAD, bool DMA, bool DSO = false, bool WIN = false>
+__global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, split_of<WIN> sp) {
     using B = Blk<T>;
     using F = typename B::Frag;
     constexpr int ES = B::ES, MB = DPAD / 32;
@@ -370,13 +378,16 @@ __global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, BackwardSplit
     // so the heaviest workgroups dispatch first
     const int bkv = blockIdx.x % nbk;
     int kb, part;
-    sp.coords(blockIdx.x / nbk, (S + kBwdKeys - 1) / kBwdKeys, G, a.causal, kb, part);
+    if constexpr (WIN) sp.coords(blockIdx.x / nbk, kb, part);
+    else sp.coords(blockIdx.x / nbk, (S + kBwdKeys - 1) / kBwdKeys, G, a.causal, kb, part);
     const int b = bkv / a.kv_heads, kvh = bkv - b * a.kv_heads;
     const int k0 = kb * kBwdKeys + wave * 32;
     const int64_t krow0 = (int64_t)bkv * S;
     const int qstart = a.causal ? kb * kBwdKeys : 0;  // a multiple of QT
-    const int nqt = (S - qstart + QT - 1) / QT, all_tiles = G * nqt;
+    const int qend = WIN ? window_end(a, kb) : S;  // past the last query that sees a key of the block
+    const int nqt = (qend - qstart + QT - 1) / QT, all_tiles = G * nqt;
     const int tile0 = part * sp.chunk, ntiles = min(all_tiles - tile0, sp.chunk) + tile0;
+    if (WIN && tile0 >= all_tiles) return;
     const int64_t qhead0 = ((int64_t)b * a.q_heads + (int64_t)kvh * G) * S;  // first row of the group
     auto tile_hq = [&](int j) {  // head of the group and query offset qt of tile j
         const int hh = j / nqt;
@@ -478,14 +489,18 @@ __global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, BackwardSplit
 
     // Probabilities and dS of one sub-block from its S and dP accumulators; `diag`: the
     // sub-block on the causal diagonal (query q0 + kidx(g, t) against key q0 + c).
-    auto softmax = [&](auto diag, const f32x16_t& s, const f32x16_t& dp, const float (&l2)[16],
+    // (q0: the sub-block's first query; used with a window only)
+    auto softmax = [&](auto diag, int q0, const f32x16_t& s, const f32x16_t& dp, const float (&l2)[16],
                        const float (&dl)[16], F& pf, F& df) {
+        (void)q0;
         float pv[16], dsv[16];
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
             float p = fast_exp2(fmaf(s[t], c2, -l2[t]));
-            if constexpr (decltype(diag)::value)
-                if (c > B::kidx(g, t)) p = 0.0f;
+            if constexpr (decltype(diag)::value) {
+                const int back = q0 + B::kidx(g, t) - (k0 + c);  // from the query to the key
+                if (WIN ? back < 0 || (back >= a.window && k0 + c >= a.sinks) : c > B::kidx(g, t)) p = 0.0f;
+            }
             pv[t] = p;
             dsv[t] = p * (dp[t] - dl[t]);
         }
@@ -512,7 +527,13 @@ __global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, BackwardSplit
         const uint32_t ds_goff = DSO ? ds_group_off(hh, qt) : 0u;
         // active sub-blocks [s0, s1): causal skips the ones wholly before the wave's keys
         const int s0 = a.causal ? min(NSUB, max(0, (k0 - qt) >> 5)) : 0;
-        const int s1 = min(NSUB, (S - qt + 31) >> 5);
+        int s1 = min(NSUB, (S - qt + 31) >> 5);
+        if (WIN && k0 >= a.sinks) s1 = min(s1, max(0, (min(S, k0 + 31 + a.window) - qt + 31) >> 5));
+        // whether the sub-block at q0 holds pairs that are not seen
+        auto masked = [&](int q0) {
+            if constexpr (WIN) return q0 < k0 + 31 || (q0 + 31 - k0 >= a.window && k0 + 31 >= a.sinks);
+            else return a.causal && q0 == k0;
+        };
         if constexpr (PIPE) {
             using H = typename B::H;
             constexpr int NS = 4 * MB;  // MFMAs of S+dP, and of dV+dK, per sub-block
@@ -571,13 +592,14 @@ __global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, BackwardSplit
                     load_ld(sb, l2[u], dl[u]);
                     sdp(sb, sacc[u], dacc[u]);
                 }
-                const bool diag = a.causal && qt + 32 * sb == k0;
+                const int q0 = qt + 32 * sb;
+                const bool diag = masked(q0);
                 const bool next = sb + 1 < s1;
                 if (next) {
                     // phase X: S, dP of sb+1 under the softmax of sb
                     auto phase_x = [&](auto dg) {
                         sdp(sb + 1, sacc[u ^ 1], dacc[u ^ 1]);
-                        softmax(dg, sacc[u], dacc[u], l2[u], dl[u], pf, df);
+                        softmax(dg, q0, sacc[u], dacc[u], l2[u], dl[u], pf, df);
                         FA_BWD_SG(0x100, R);
 #pragma unroll
                         for (int i = 0; i < NS; ++i) {
@@ -589,8 +611,8 @@ __global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, BackwardSplit
                     if (diag) phase_x(std::true_type{});
                     else phase_x(std::false_type{});
                 } else {
-                    if (diag) softmax(std::true_type{}, sacc[u], dacc[u], l2[u], dl[u], pf, df);
-                    else softmax(std::false_type{}, sacc[u], dacc[u], l2[u], dl[u], pf, df);
+                    if (diag) softmax(std::true_type{}, q0, sacc[u], dacc[u], l2[u], dl[u], pf, df);
+                    else softmax(std::false_type{}, q0, sacc[u], dacc[u], l2[u], dl[u], pf, df);
                 }
                 // phase Y: dV, dK of sb; (LSE, delta) rows of sb+1
                 dvdk(sb, pf, df);
@@ -621,8 +643,8 @@ __global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, BackwardSplit
                 float l2[16], dl[16];
                 rows16<T>(smem + st + T_LD + sb * 32 * 8, g, l2, dl);
                 F pf, df;
-                if (a.causal && q0 == k0) softmax(std::true_type{}, s, dp, l2, dl, pf, df);
-                else softmax(std::false_type{}, s, dp, l2, dl, pf, df);
+                if (masked(q0)) softmax(std::true_type{}, q0, s, dp, l2, dl, pf, df);
+                else softmax(std::false_type{}, q0, s, dp, l2, dl, pf, df);
                 const uint8_t* tile = smem + st + sb * 32 * RB;
 #pragma unroll
                 for (int m = 0; m < MB; ++m) {
@@ -685,6 +707,31 @@ __global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, BackwardSplit
 // early ones, which under a mask have the most, come first.
 constexpr int kAddRows = 16;
 template <typename T>
+__device__ __forceinline__ void add_partials(const BackwardArgs& a, const WindowSplit& sp, int block) {
+    using B = Blk<T>;
+    const int S = a.seq, D = a.head_dim, units = a.batch * a.kv_heads;
+    const int r0 = block % (kBwdKeys / kAddRows) * kAddRows, at = block / (kBwdKeys / kAddRows);
+    const int kb = at / units, bkv = at - kb * units;
+    const int tiles = a.group * ((window_end(a, kb) - kb * kBwdKeys + sp.tile - 1) / sp.tile);
+    const int n = (tiles + sp.chunk - 1) / sp.chunk;
+    if (n < 2) return;  // written by the workgroup that has all of it
+    const int64_t step = (int64_t)2 * kBwdKeys * D * units;
+    const int count = min(kAddRows, S - kb * kBwdKeys - r0) * D;  // (may be negative: no rows)
+    const int64_t out = ((int64_t)bkv * S + kb * kBwdKeys + r0) * D;
+    const float* const base = sp.part + (int64_t)sp.slot(kb, 0) * step +
+                              (int64_t)bkv * 2 * kBwdKeys * D + r0 * D;
+    for (int e = threadIdx.x; e < count; e += blockDim.x) {
+        float k = 0.0f, v = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            k += base[i * step + e];
+            v += base[i * step + kBwdKeys * D + e];
+        }
+        B::store(a.dk, out + e, k * a.scale);
+        B::store(a.dv, out + e, v);
+    }
+}
+template <typename T>
 __device__ __forceinline__ void add_partials(const BackwardArgs& a, const BackwardSplit& sp,
                                              int block) {
     using B = Blk<T>;
@@ -718,9 +765,9 @@ __device__ __forceinline__ void add_partials(const BackwardArgs& a, const Backwa
 // One workgroup: 128 queries of one (batch, query head), 32 per wave, Q and dO of them in
 // registers; tiles of 64 keys (K, V) of the KV head are swept, DMA double-buffered as above.
 // Two waves per SIMD (16-bit), so the phases of the two waves overlap.
-template <typename T, int DPAD, bool DMA>
+template <typename T, int DPAD, bool DMA, bool WIN = false>
 __global__ __launch_bounds__(256, Blk<T>::ES == 2 ? 2 : 1) void bwd_dq(BackwardArgs a,
-                                                                      BackwardSplit sp, int n_dq) {
+                                                                      split_of<WIN> sp, int n_dq) {
     using B = Blk<T>;
     if ((int)blockIdx.x >= n_dq) {
         add_partials<T>(a, sp, blockIdx.x - n_dq);
@@ -750,7 +797,15 @@ __global__ __launch_bounds__(256, Blk<T>::ES == 2 ? 2 : 1) void bwd_dq(BackwardA
     const int64_t qrow0 = (int64_t)bh * S, krow0 = ((int64_t)b * a.kv_heads + kvh) * S;
     const bool qok = q0 + c < S;
     const int kend = a.causal ? min(S, (qb + 1) * kBwdQueries) : S;
-    const int ntiles = (kend + KT - 1) / KT;
+    // WIN: the tiles between the sinks and the first key that the block's first query sees are left out
+    int before = 0, skip = 0;
+    if constexpr (WIN) {
+        const int low = max(0, qb * kBwdQueries + 1 - a.window) / KT;
+        before = (min(a.sinks, low * KT) + KT - 1) / KT;
+        skip = low - before;
+    }
+    const int ntiles = (kend + KT - 1) / KT - skip;
+    auto tile_at = [&](int m) { return WIN && m >= before ? m + skip : m; };
     const bool vec = DMA || a.vec;
 
     uint32_t doff[DMA ? KI : 1];
@@ -789,16 +844,16 @@ __global__ __launch_bounds__(256, Blk<T>::ES == 2 ? 2 : 1) void bwd_dq(BackwardA
     if constexpr (ES == 2) ops.init(lane);
 
     if constexpr (DMA) {
-        dma_tile(0, 0);
+        dma_tile(tile_at(0), 0);
         wait_dma();
         __syncthreads();
     }
     for (int j = 0; j < ntiles; ++j) {
-        const int kt = j * KT;
+        const int kt = tile_at(j) * KT;
         int st = 0;
         if constexpr (DMA) {
             st = (j & 1) * STAGE;
-            if (j + 1 < ntiles) dma_tile(j + 1, STAGE - st);
+            if (j + 1 < ntiles) dma_tile(tile_at(j + 1), STAGE - st);
         } else {
             const int nv = min(KT, S - kt);
             __syncthreads();
@@ -812,6 +867,7 @@ __global__ __launch_bounds__(256, Blk<T>::ES == 2 ? 2 : 1) void bwd_dq(BackwardA
             const int kk0 = kt + sub * 32;
             if (kk0 >= S) break;
             if (a.causal && kk0 > q0 + 31) continue;  // every key of the block is masked
+            if (WIN && q0 - kk0 - 31 >= a.window && kk0 >= a.sinks) continue;
             f32x16_t s = (f32x16_t)0.0f, dp = (f32x16_t)0.0f;
             const uint8_t* tk = smem + st + sub * 32 * RB;
             if constexpr (ES == 2) {
@@ -832,13 +888,16 @@ __global__ __launch_bounds__(256, Blk<T>::ES == 2 ? 2 : 1) void bwd_dq(BackwardA
                 }
             }
             // register t: key kk0 + kidx(g, t), query q0 + c
-            const bool mask = (a.causal && kk0 + 31 > q0) || kk0 + 31 >= S;
+            const bool mask = (a.causal && kk0 + 31 > q0) || kk0 + 31 >= S ||
+                              (WIN && q0 + 31 - kk0 >= a.window && kk0 + 31 >= a.sinks);
             float dsv[16];
 #pragma unroll
             for (int t = 0; t < 16; ++t) {
                 float p = fast_exp2(fmaf(s[t], c2, -l2));
                 const int key = kk0 + B::kidx(g, t);
-                if (mask && (key >= S || (a.causal && key > q0 + c))) p = 0.0f;
+                if (mask && (key >= S || (a.causal && key > q0 + c) ||
+                             (WIN && q0 + c - key >= a.window && key >= a.sinks)))
+                    p = 0.0f;
                 dsv[t] = p * (dp[t] - dl);
             }
             const F df = B::pack(dsv);
@@ -1214,6 +1273,67 @@ void launch_backward(Dtype dt, const BackwardArgs& a, const BackwardSplit& sp, h
         case Dtype::F32: launch_dims<float>(a, sp, s, a64_out); break;
         case Dtype::F16: launch_dims<f16_t>(a, sp, s, a64_out); break;
         case Dtype::BF16: launch_dims<bf16_t>(a, sp, s, a64_out); break;
+    }
+}
+
+// ------------------------------------------------------------------ sliding windows
+// Key blocks without sinks have about window / 128 + 1 tiles a query head, those with sinks all queries
+// behind them, so the latter are dealt to several workgroups (and both where they leave CUs idle): a chunk
+// is an even share of the tiles for each CU, but no more than a block without sinks has.
+WindowSplit window_split(Dtype dt, const BackwardArgs& a, uint64_t limit) {
+    WindowSplit sp{};
+    sp.tile = dt == Dtype::F32 ? 64 : 128;
+    const int nkb = (a.seq + kBwdKeys - 1) / kBwdKeys;
+    sp.sink_blocks = (std::min(a.sinks, a.seq) + kBwdKeys - 1) / kBwdKeys;
+    auto tiles = [&](int kb) {
+        return (int64_t)a.group * ((window_end(a, kb) - kb * kBwdKeys + sp.tile - 1) / sp.tile);
+    };
+    int64_t all = 0;
+    for (int kb = 0; kb < nkb; ++kb) all += tiles(kb);
+    const int64_t units = (int64_t)a.batch * a.kv_heads, cus = device_cus();
+    const int64_t most = sp.sink_blocks < nkb ? tiles(sp.sink_blocks) : tiles(0);
+    const int64_t even = std::max<int64_t>((all * units + cus - 1) / cus, 4);
+    sp.blocks = nkb;
+    // (longer chunks where the partials would take more than `limit`: many sinks over a long sequence)
+    for (int64_t chunk = std::min(most, even);; chunk *= 2) {
+        sp.chunk = (int)std::min<int64_t>(chunk, tiles(0));
+        sp.sink_parts = (int)((tiles(0) + sp.chunk - 1) / sp.chunk);
+        sp.parts = sp.sink_blocks < nkb ? (int)((most + sp.chunk - 1) / sp.chunk) : 0;
+        // partials: of the sink blocks, and of the others where these have several parts too
+        sp.bytes = (uint64_t)(sp.parts > 1         ? sp.workgroups()
+                              : sp.sink_parts > 1 ? sp.sink_blocks * sp.sink_parts
+                                                  : 0) *
+                   units * 2 * kBwdKeys * a.head_dim * 4;
+        if (sp.bytes <= limit) break;
+    }
+    return sp;
+}
+
+template <typename T, int DPAD>
+static void launch_window(const BackwardArgs& a, const WindowSplit& sp, hipStream_t s) {
+    const unsigned units = (unsigned)(a.batch * a.kv_heads);
+    hipLaunchKernelGGL((bwd_dkdv<T, DPAD, true, false, true>), dim3(sp.workgroups() * units), dim3(256),
+                       0, s, a, sp);
+    const int n_dq = (a.seq + kBwdQueries - 1) / kBwdQueries * a.batch * a.q_heads;
+    const unsigned split = sp.parts > 1 ? sp.blocks : sp.sink_parts > 1 ? sp.sink_blocks : 0;
+    const unsigned n_add = split * units * (kBwdKeys / kAddRows);
+    hipLaunchKernelGGL((bwd_dq<T, DPAD, true, true>), dim3(n_dq + n_add), dim3(256), 0, s, a, sp, n_dq);
+}
+
+template <typename T>
+static void launch_window_dims(const BackwardArgs& a, const WindowSplit& sp, hipStream_t s) {
+    const int64_t rows = (int64_t)a.batch * a.q_heads * a.seq;
+    hipLaunchKernelGGL((bwd_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a, rows);
+    if (a.head_dim <= 32) launch_window<T, 32>(a, sp, s);
+    else if (a.head_dim <= 64) launch_window<T, 64>(a, sp, s);
+    else launch_window<T, 128>(a, sp, s);
+}
+
+void launch_backward_window(Dtype dt, const BackwardArgs& a, const WindowSplit& sp, hipStream_t s) {
+    switch (dt) {
+        case Dtype::F32: launch_window_dims<float>(a, sp, s); break;
+        case Dtype::F16: launch_window_dims<f16_t>(a, sp, s); break;
+        case Dtype::BF16: launch_window_dims<bf16_t>(a, sp, s); break;
     }
 }
 

@@ -1123,6 +1123,39 @@ int run_prefill(fa_ctx* ctx, PrefillJob& j) {
     return enqueue_prefill(ctx, r);
 }
 
+int check_aligned(const char* name, const void* p) {
+    if ((uintptr_t)p % 16)
+        return fail(FA_ERR_MISALIGNED, "buffer %s does not start at a multiple of 16 bytes", name);
+    return FA_OK;
+}
+
+int check_window(const fa_window* w) {
+    if (!w) return fail(FA_ERR_NULL_ARGUMENT, "window is null");
+    if (!w->window) return fail(FA_ERR_ZERO_DIMENSION, "the window must hold at least one position");
+    return FA_OK;
+}
+
+// What the contiguous window calls take: causal, rows of whole 16-byte pieces, one (batch, head) slice within
+// 32-bit offsets.
+int check_window_shape(const fa_grouped_shape* sh, const fa_config* cfg, const fa_window* w, int dtype) {
+    if (int rc = check_window(w)) return rc;
+    if (!cfg || !cfg->causal)
+        return fail(FA_ERR_CAUSAL_VISIBILITY_MISMATCH, "a sliding window needs causal attention");
+    if (sh->head_dim % 8)
+        return fail(FA_ERR_UNSUPPORTED_HEAD_DIM,
+                    "head_dim %llu is not a multiple of 8, required for a sliding window",
+                    (unsigned long long)sh->head_dim);
+    if (sh->seq_len * sh->head_dim * (uint64_t)elem_bytes(dtype) > (uint64_t)INT32_MAX)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED,
+                    "one K/V slice spans %llu bytes; sliding windows address at most 2 GiB",
+                    (unsigned long long)(sh->seq_len * sh->head_dim * (uint64_t)elem_bytes(dtype)));
+    // (a launch has below 2^32 threads, here up to 16 a row)
+    if (sh->batch * sh->q_heads * sh->seq_len > 0xffffff0ull)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "%llu query rows exceed the launch space",
+                    (unsigned long long)(sh->batch * sh->q_heads * sh->seq_len));
+    return FA_OK;
+}
+
 int validate_grouped(uint64_t b, uint64_t hq, uint64_t hkv, uint64_t s, uint64_t d) {
     if (!b || !hq || !hkv || !s || !d)
         return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
@@ -1233,6 +1266,54 @@ int fa_forward_gqa_rope(fa_ctx* ctx, const void* q, size_t q_bytes, const void* 
     begin_call(ctx);
     if (int rc = set_device(ctx)) return rc;
     if (int rc = run_prefill(ctx, j)) return rc;
+    return ok();
+}
+
+int fa_forward_gqa_window(fa_ctx* ctx, const void* q, size_t q_bytes, const void* k, const void* v,
+                          size_t kv_bytes, void* out_lse, size_t out_bytes, const fa_grouped_shape* sh,
+                          const fa_config* cfg, const fa_window* window, const fa_rotary* rot,
+                          int dtype) {
+    PrefillJob j;
+    int rc = build_gqa_job(ctx, q, q_bytes, k, v, kv_bytes, out_lse, out_bytes, sh, cfg, rot, dtype, j,
+                           nullptr);
+    // (a null context is reported after the other arguments)
+    if (rc && !(rc == FA_ERR_NULL_ARGUMENT && !ctx && sh && q && k && v && out_lse)) return rc;
+    if (int w = check_window_shape(sh, cfg, window, dtype)) return w;
+    const struct { const char* name; const void* p; } aligned[] = {{"Q", q}, {"K", k}, {"V", v}, {"O|LSE", out_lse}};
+    for (const auto& t : aligned)
+        if (int w = check_aligned(t.name, t.p)) return w;
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int w = set_device(ctx)) return w;
+    fa::PrefillArgs& a = j.a;
+    a.window = (int)std::min<uint64_t>(window->window, sh->seq_len);
+    a.sinks = (int)std::min<uint64_t>(window->sinks, sh->seq_len);
+    unsigned dispatches = 1;
+    if (j.rope) {
+        if (int w = ensure_rope(ctx, j.theta, sh->head_dim, j.max_pos, &a.rope_table)) return w;
+        void* ws = nullptr;
+        if (int w = ensure_ws(ctx, j.kv_bytes, &ws)) return w;
+        begin_span(ctx);
+        fa::launch_rotate_rows(j.dt, a.k, ws, (int)j.k_rows, (int)j.k_heads, a.head_dim,
+                               (int64_t)j.k_period, a.rope_table, a.kv_rope_offset, ctx->stream);
+        end_span(ctx, FA_KERNEL_ROPE_ROTATE);
+        HIP_TRY(hipGetLastError());
+        a.k = ws;
+        a.rope_k = 0;
+        a.rope_rows = (int)j.max_pos;
+        ++dispatches;
+    }
+    unsigned grid[3], block, rows, keys;
+    const int kid = prefill_kernel_id(dtype, j.rope);
+    begin_span(ctx);
+    fa::launch_prefill_window(j.dt, a, ctx->stream, grid, &block, &rows, &keys);
+    end_span(ctx, kid);
+    HIP_TRY(hipGetLastError());
+    char name[64];
+    snprintf(name, sizeof name, "%sprefill_%s<%s> (window)", j.rope ? "rotate_rows + " : "",
+             dtype == FA_DTYPE_F32 ? (rows == 32 ? "f32_groups" : "mfma_f32") : "mfma16",
+             dtype_name(dtype));
+    record(ctx, kid, name, rows, keys, grid, block, dispatches, 1, nullptr);
     return ok();
 }
 
@@ -3230,6 +3311,69 @@ int fa_backward_grouped(fa_ctx* ctx, const void* q, const void* k, const void* v
     return ok();
 }
 
+int fa_backward_gqa_window(fa_ctx* ctx, const void* q, const void* k, const void* v,
+                           const void* d_out, const void* out, const float* lse, void* dq, void* dk,
+                           void* dv, const fa_grouped_shape* sh, const fa_config* cfg,
+                           const fa_window* window, int dtype) {
+    fa_backward_layout lay;
+    if (int rc = fa_backward_grouped_layout(sh, dtype, &lay)) return rc;
+    if (int rc = validate_grouped(sh->batch, sh->q_heads, sh->kv_heads, sh->seq_len, sh->head_dim))
+        return rc;
+    if (int rc = check_head_dim(sh->head_dim, dtype)) return rc;
+    const struct { const char* name; const void* p; } ptrs[] = {
+        {"Q", q}, {"K", k}, {"V", v}, {"dO", d_out}, {"O", out}, {"LSE", lse}, {"dQ", dq}, {"dK", dk}, {"dV", dv}};
+    for (const auto& t : ptrs)
+        if (!t.p) return fail(FA_ERR_NULL_ARGUMENT, "backward tensor pointer is null");
+    float scale;
+    if (int rc = resolve_scale(cfg, sh->head_dim, &scale)) return rc;
+    if (int rc = check_window_shape(sh, cfg, window, dtype)) return rc;
+    for (const auto& t : ptrs)
+        if (t.p != (const void*)lse)
+            if (int rc = check_aligned(t.name, t.p)) return rc;
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int rc = set_device(ctx)) return rc;
+    void* delta = nullptr;
+    if (int rc = grow(ctx, &ctx->ws_delta, &ctx->ws_delta_bytes, lay.lse_elements * 8, &delta))
+        return rc;
+    fa::BackwardArgs a{};
+    a.q = q; a.k = k; a.v = v; a.dout = d_out; a.o = out; a.lse = lse;
+    a.dq = dq; a.dk = dk; a.dv = dv;
+    a.ld = (float2*)delta;
+    a.batch = (int)sh->batch;
+    a.q_heads = (int)sh->q_heads;
+    a.kv_heads = (int)sh->kv_heads;
+    a.group = (int)(sh->q_heads / sh->kv_heads);
+    a.seq = (int)sh->seq_len;
+    a.head_dim = (int)sh->head_dim;
+    a.causal = a.vec = a.dma = 1;
+    a.scale = scale;
+    a.window = (int)std::min<uint64_t>(window->window, sh->seq_len);
+    a.sinks = (int)std::min<uint64_t>(window->sinks, sh->seq_len);
+    fa::WindowSplit sp = fa::window_split((Dtype)dtype, a, fa::kBackwardPartialBytes);
+    if (sp.bytes) {
+        size_t bytes = (size_t)1 << 20;  // (a power of two, as in fa_backward_grouped)
+        while (bytes < sp.bytes) bytes *= 2;
+        void* part = nullptr;
+        if (grow(ctx, &ctx->ws_part, &ctx->ws_part_bytes, bytes, &part) != FA_OK) {
+            // no memory, or the stream is captured: the split that the workspace of earlier calls holds
+            (void)hipGetLastError();
+            sp = fa::window_split((Dtype)dtype, a, ctx->ws_part_bytes);
+            part = ctx->ws_part;
+        }
+        sp.part = (float*)part;
+    }
+    begin_span(ctx);
+    fa::launch_backward_window((Dtype)dtype, a, sp, ctx->stream);
+    end_span(ctx, FA_KERNEL_BACKWARD_RECOMPUTE);
+    HIP_TRY(hipGetLastError());
+    const unsigned grid[3] = {(unsigned)(sp.workgroups() * a.batch * a.kv_heads), 1, 1};
+    char name[64];
+    snprintf(name, sizeof name, "bwd_delta + bwd_dkdv + bwd_dq<%s> (window)", dtype_name(dtype));
+    record(ctx, FA_KERNEL_BACKWARD_RECOMPUTE, name, (uint32_t)sp.tile, 64, grid, 256, 3, 1, nullptr);
+    return ok();
+}
+
 int fa_backward_grouped_recompute(fa_ctx* ctx, const void* packed_forward, size_t forward_bytes,
                                   void* packed_grads, size_t grads_bytes,
                                   const fa_grouped_shape* sh, const fa_config* cfg, int dtype) {
@@ -3298,12 +3442,6 @@ int check_batch(const fa_paged_batch* b, bool tables, uint64_t* capacity) {
     return FA_OK;
 }
 
-int check_aligned(const char* name, const void* p) {
-    if ((uintptr_t)p % 16)
-        return fail(FA_ERR_MISALIGNED, "buffer %s does not start at a multiple of 16 bytes", name);
-    return FA_OK;
-}
-
 // Heads, storage and pools of a batch; *row: bytes of a pool row.
 int check_pools(const fa_paged_batch* b, const void* k_pool, const void* v_pool, size_t pool_bytes,
                 uint64_t kv_heads, uint64_t head_dim, int dtype, uint64_t* row) {
@@ -3330,6 +3468,256 @@ int check_tree_tokens(uint64_t max_tokens) {
         return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "%llu drafted tokens exceed the maximum %d",
                     (unsigned long long)max_tokens, fa::kTreeTokens);
     return FA_OK;
+}
+
+// Heads and row of a 4-bit pool.
+int check_fp4_row(uint64_t kv_heads, uint64_t head_dim) {
+    if (!kv_heads || !head_dim)
+        return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
+    if (head_dim % 32 || head_dim > kMaxHeadDim)
+        return fail(FA_ERR_UNSUPPORTED_HEAD_DIM,
+                    "head_dim %llu is not a multiple of 32 up to %llu, required for 4-bit rows",
+                    (unsigned long long)head_dim, (unsigned long long)kMaxHeadDim);
+    if (kv_heads > kI32 / 4 / head_dim)
+        return fail(FA_ERR_SHAPE_OVERFLOW, "attention shape overflows the address space");
+    return FA_OK;
+}
+
+int check_fp4_pools(const fa_paged_batch* b, const void* k_pool, const void* v_pool, size_t pool_bytes,
+                    uint64_t kv_heads, uint64_t head_dim, int dtype, uint64_t* row) {
+    if (int rc = check_dtype(dtype)) return rc;
+    if (int rc = check_fp4_row(kv_heads, head_dim)) return rc;
+    *row = (uint64_t)fa::fp4_row_bytes((int)kv_heads, (int)head_dim);
+    const uint64_t need = b->page_size * b->physical_pages * *row;  // (below 2^31 rows of 2^29 bytes)
+    if (int rc = check_buffer("K pool", k_pool, pool_bytes, need)) return rc;
+    if (int rc = check_buffer("V pool", v_pool, pool_bytes, need)) return rc;
+    if (int rc = check_aligned("K pool", k_pool)) return rc;
+    return check_aligned("V pool", v_pool);
+}
+
+enum class Rows { kAppend, kAppendFp4, kReadFp4 };
+// Rows [n_seqs, max_new, kv_heads*head_dim] of `dtype` to their slots of pools of `dtype` or of 4-bit
+// rows, or (kReadFp4) from them.
+int move_rows(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* slots, size_t slots_bytes,
+              const int32_t* positions, size_t positions_bytes, uint64_t max_new, const void* k_src,
+              const void* v_src, size_t src_bytes, void* k_pool, void* v_pool, size_t pool_bytes,
+              uint64_t kv_heads, uint64_t head_dim, const fa_rotary* rot, int dtype, Rows what) {
+    uint64_t capacity, row, rows, pieces, need;
+    const bool fp4 = what != Rows::kAppend;
+    if (int rc = check_batch(b, false, &capacity)) return rc;
+    if (!max_new) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
+    if (int rc = fp4 ? check_fp4_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)
+                     : check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row))
+        return rc;
+    if (fp4) row = kv_heads * head_dim * elem_bytes(dtype);  // (of the source)
+    if (mul_ov(b->n_seqs, max_new, &rows) || rows > kI32 || mul_ov(rows, row / 16, &pieces) ||
+        pieces > 0xffffff00ull)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged append exceeds the index space");
+    need = rows * row;
+    if (int rc = check_buffer("slots", slots, slots_bytes, rows * 4)) return rc;
+    if (positions)
+        if (int rc = check_buffer("positions", positions, positions_bytes, rows * 4)) return rc;
+    if (int rc = check_buffer("K", k_src, src_bytes, need)) return rc;
+    if (int rc = check_buffer("V", v_src, src_bytes, need)) return rc;
+    if (int rc = check_aligned("K", k_src)) return rc;
+    if (int rc = check_aligned("V", v_src)) return rc;
+    if (rot) {
+        if (head_dim > kMaxHeadDim)  // (the table's frequencies travel in the kernel arguments)
+            return fail(FA_ERR_UNSUPPORTED_HEAD_DIM, "head_dim %llu exceeds maximum %llu",
+                        (unsigned long long)head_dim, (unsigned long long)kMaxHeadDim);
+        if (int rc = check_rotary(rot->theta, rot->position_offset, head_dim, capacity)) return rc;
+    }
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int rc = set_device(ctx)) return rc;
+    fa::SlotAppendArgs a{};
+    if (rot)
+        if (int rc = ensure_rope(ctx, rot->theta, head_dim, rot->position_offset + capacity,
+                                 &a.rope_table))
+            return rc;
+    a.k_src = k_src;
+    a.v_src = v_src;
+    a.k_pool = k_pool;
+    a.v_pool = v_pool;
+    a.slots = slots;
+    a.positions = positions;
+    a.ctx_lens = b->ctx_lens;
+    a.rope_positions = (int64_t)capacity;
+    a.rope_offset = rot ? (int)rot->position_offset : 0;
+    a.n_rows = (int)rows;
+    a.max_new = (int)max_new;
+    a.pool_rows = (int)(b->page_size * b->physical_pages);
+    a.kv_heads = (int)kv_heads;
+    a.head_dim = (int)head_dim;
+    unsigned grid[3];
+    begin_span(ctx);
+    (what == Rows::kAppend      ? fa::launch_append_slots
+     : what == Rows::kAppendFp4 ? fa::launch_append_fp4
+                                : fa::launch_read_fp4)((Dtype)dtype, a, ctx->stream, grid);
+    end_span(ctx, FA_KERNEL_PAGED_APPEND);
+    HIP_TRY(hipGetLastError());
+    record(ctx, FA_KERNEL_PAGED_APPEND,
+           what == Rows::kAppend ? "append_slots" : what == Rows::kAppendFp4 ? "append_fp4" : "read_fp4", 0, (uint32_t)b->page_size, grid, 256, 1, 1,
+           nullptr);
+    return ok();
+}
+
+// Attention of new tokens over the cache: by masks, as chains, or with a window (null: none); over pools
+// of `dtype` or (fp4) of 4-bit rows.
+int batch_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q, size_t q_bytes,
+                    const void* k_pool, const void* v_pool, size_t pool_bytes, void* out_lse,
+                    size_t out_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                    const int32_t* positions, size_t positions_bytes, const uint64_t* masks,
+                    size_t masks_bytes, uint64_t max_tokens, uint64_t q_heads, uint64_t kv_heads,
+                    uint64_t head_dim, const fa_config* cfg, const fa_window* window,
+                    const fa_rotary* rot, int dtype, bool fp4) {
+    uint64_t capacity, row, lse, elements;
+    if (window) {
+        if (int rc = check_window(window)) return rc;
+        if (masks)
+            return fail(FA_ERR_CAUSAL_VISIBILITY_MISMATCH, "a window and masks exclude each other");
+    }
+    if (int rc = check_batch(b, true, &capacity)) return rc;
+    if (int rc = check_tree_tokens(max_tokens)) return rc;
+    if (!q_heads) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
+    if (int rc = fp4 ? check_fp4_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)
+                     : check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row))
+        return rc;
+    if (q_heads % kv_heads)
+        return fail(FA_ERR_INVALID_HEAD_GROUPING,
+                    "q_heads (%llu) must be exactly divisible by kv_heads (%llu)",
+                    (unsigned long long)q_heads, (unsigned long long)kv_heads);
+    if (int rc = check_head_dim(head_dim, dtype)) return rc;
+    float scale;
+    if (int rc = resolve_scale(cfg, head_dim, &scale)) return rc;
+    if (rot)
+        if (int rc = check_rotary(rot->theta, rot->position_offset, head_dim, capacity)) return rc;
+    const uint64_t n = b->n_seqs, words = (max_tokens + 63) / 64;
+    if (q_heads > kI32 || n * max_tokens > kI32 || mul_ov(n * max_tokens, q_heads, &lse) || lse > kI32)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "drafted tokens exceed the i32 index space");
+    // steps of 32 keys or more of every (sequence, kv head), and its start, counted in 32 bits
+    if (mul_ov(n * kv_heads, capacity / 32 + 16, &elements) || elements > kI32)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the i32 index space");
+    // threads of the combine: 256 for every 32 rows of a (sequence, kv head), fp4: up to four times as many
+    if (n * kv_heads * ((max_tokens * (q_heads / kv_heads) + 31) / 32) > (fp4 ? 0x3fffffu : 0xffffffu))
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the launch space");
+    elements = lse * head_dim;
+    fa_packed_layout lay;
+    if (int rc = fa_packed_layout_for(elements, lse, dtype, &lay)) return rc;
+    if (int rc = check_buffer("Q", q, q_bytes, elements * elem_bytes(dtype))) return rc;
+    if (int rc = check_buffer("O|LSE", out_lse, out_bytes, lay.combined_bytes)) return rc;
+    if (int rc = check_aligned("Q", q)) return rc;
+    if (int rc = check_aligned("O|LSE", out_lse)) return rc;
+    if (int rc = check_buffer("tree lengths", tree_lens, tree_lens_bytes, n * 4)) return rc;
+    if (positions)
+        if (int rc = check_buffer("positions", positions, positions_bytes, n * max_tokens * 4)) return rc;
+    if (masks)
+        if (int rc = check_buffer("masks", masks, masks_bytes, n * max_tokens * words * 8)) return rc;
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int rc = set_device(ctx)) return rc;
+    fa::TreeArgs a{};
+    if (rot)
+        if (int rc = ensure_rope(ctx, rot->theta, head_dim, rot->position_offset + capacity,
+                                 &a.rope_table))
+            return rc;
+    a.q = q;
+    a.k_pool = k_pool;
+    a.v_pool = v_pool;
+    a.o = out_lse;
+    a.lse = (float*)((uint8_t*)out_lse + lay.lse_byte_offset);
+    a.block_tables = b->block_tables;
+    a.ctx_lens = b->ctx_lens;
+    a.tree_lens = tree_lens;
+    a.positions = positions;
+    a.masks = masks;
+    a.rope_positions = (int)capacity;
+    a.rope_offset = rot ? (int)rot->position_offset : 0;
+    a.n_seqs = (int)n;
+    a.max_tokens = (int)max_tokens;
+    a.words = (int)words;
+    a.q_heads = (int)q_heads;
+    a.kv_heads = (int)kv_heads;
+    a.group = (int)(q_heads / kv_heads);
+    a.head_dim = (int)head_dim;
+    a.max_pages = (int)b->max_pages;
+    a.page_size = (int)b->page_size;
+    a.physical_pages = (int)b->physical_pages;
+    a.window = window ? (int)std::min<uint64_t>(window->window, capacity) : 0;
+    a.sinks = window ? (int)std::min<uint64_t>(window->sinks, capacity) : 0;
+    a.scale = scale;
+    size_t ml_offset, plan_offset, odd_offset = 0;
+    const size_t bytes = fp4 ? fa::fp4_workspace((Dtype)dtype, a, &ml_offset, &plan_offset)
+                             : fa::tree_workspace((Dtype)dtype, a, &ml_offset, &plan_offset, &odd_offset);
+    void* ws = nullptr;
+    if (int rc = grow(ctx, &ctx->ws_tree, &ctx->ws_tree_bytes, bytes, &ws)) return rc;
+    a.part_o = (float*)ws;
+    a.part_ml = (float2*)((uint8_t*)ws + ml_offset);
+    a.plan = (int*)((uint8_t*)ws + plan_offset);
+    a.odd = (int*)((uint8_t*)ws + odd_offset);
+    unsigned grid[3], block, q_rows;
+    begin_span(ctx);
+    (fp4 ? fa::launch_fp4_attention : fa::launch_tree_attention)(
+        (Dtype)dtype, a, ctx->stream, grid, &block, &q_rows,
+        [](void* c) {
+            end_span((fa_ctx*)c, FA_KERNEL_TREE_ATTENTION);
+            begin_span((fa_ctx*)c);
+        },
+        ctx);
+    end_span(ctx, FA_KERNEL_TREE_COMBINE);
+    HIP_TRY(hipGetLastError());
+    record(ctx, FA_KERNEL_TREE_ATTENTION,
+           fp4 ? "fp4_split + fp4_combine" : window ? "tree_split (window) + tree_combine"
+                                                    : "tree_split + tree_combine",
+           q_rows, 32, grid, block, 2, 1, nullptr);
+    return ok();
+}
+
+int accept_rows(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* paths,
+                size_t paths_bytes, uint64_t max_accept, const int32_t* accepted,
+                size_t accepted_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                int32_t* ctx_lens_out, size_t ctx_lens_out_bytes, void* k_pool, void* v_pool,
+                size_t pool_bytes, uint64_t kv_heads, uint64_t head_dim, int dtype, bool fp4) {
+    uint64_t capacity, row, cells;
+    if (int rc = check_batch(b, true, &capacity)) return rc;
+    if (int rc = check_tree_tokens(max_accept)) return rc;
+    if (int rc = fp4 ? check_fp4_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)
+                     : check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row))
+        return rc;
+    const uint64_t n = b->n_seqs;
+    if (mul_ov(n, max_accept, &cells) || cells > kI32)
+        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "accepted paths exceed the i32 index space");
+    if (int rc = check_buffer("paths", paths, paths_bytes, cells * 4)) return rc;
+    if (int rc = check_buffer("accepted", accepted, accepted_bytes, n * 4)) return rc;
+    if (int rc = check_buffer("tree lengths", tree_lens, tree_lens_bytes, n * 4)) return rc;
+    if (int rc = check_buffer("context lengths out", ctx_lens_out, ctx_lens_out_bytes, n * 4)) return rc;
+    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
+    begin_call(ctx);
+    if (int rc = set_device(ctx)) return rc;
+    fa::AcceptArgs a{};
+    a.block_tables = b->block_tables;
+    a.ctx_lens = b->ctx_lens;
+    a.ctx_lens_out = ctx_lens_out;
+    a.paths = paths;
+    a.accepted = accepted;
+    a.tree_lens = tree_lens;
+    a.k_pool = k_pool;
+    a.v_pool = v_pool;
+    a.n_seqs = (int)n;
+    a.max_pages = (int)b->max_pages;
+    a.page_size = (int)b->page_size;
+    a.physical_pages = (int)b->physical_pages;
+    a.max_tokens = fa::kTreeTokens;
+    a.max_accept = (int)max_accept;
+    a.row_pieces = (int)(row / 16);
+    unsigned grid[3], block;
+    begin_span(ctx);
+    fa::launch_accept(a, ctx->stream, grid, &block);
+    end_span(ctx, FA_KERNEL_PAGED_ACCEPT);
+    HIP_TRY(hipGetLastError());
+    record(ctx, FA_KERNEL_PAGED_ACCEPT, "accept_rows", (uint32_t)max_accept, (uint32_t)b->page_size,
+           grid, block, 1, 1, nullptr);
+    return ok();
 }
 
 }  // namespace
@@ -3429,57 +3817,34 @@ int fa_paged_append_slots(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* s
                           uint64_t max_new, const void* k_src, const void* v_src,
                           size_t src_bytes, void* k_pool, void* v_pool, size_t pool_bytes,
                           uint64_t kv_heads, uint64_t head_dim, const fa_rotary* rot, int dtype) {
-    uint64_t capacity, row, rows, pieces, need;
-    if (int rc = check_batch(b, false, &capacity)) return rc;
-    if (!max_new) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
-    if (int rc = check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)) return rc;
-    if (mul_ov(b->n_seqs, max_new, &rows) || rows > kI32 || mul_ov(rows, row / 16, &pieces) ||
-        pieces > 0xffffff00ull)
-        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged append exceeds the index space");
-    need = rows * row;
-    if (int rc = check_buffer("slots", slots, slots_bytes, rows * 4)) return rc;
-    if (positions)
-        if (int rc = check_buffer("positions", positions, positions_bytes, rows * 4)) return rc;
-    if (int rc = check_buffer("K", k_src, src_bytes, need)) return rc;
-    if (int rc = check_buffer("V", v_src, src_bytes, need)) return rc;
-    if (int rc = check_aligned("K", k_src)) return rc;
-    if (int rc = check_aligned("V", v_src)) return rc;
-    if (rot) {
-        if (head_dim > kMaxHeadDim)  // (the table's frequencies travel in the kernel arguments)
-            return fail(FA_ERR_UNSUPPORTED_HEAD_DIM, "head_dim %llu exceeds maximum %llu",
-                        (unsigned long long)head_dim, (unsigned long long)kMaxHeadDim);
-        if (int rc = check_rotary(rot->theta, rot->position_offset, head_dim, capacity)) return rc;
-    }
-    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
-    begin_call(ctx);
-    if (int rc = set_device(ctx)) return rc;
-    fa::SlotAppendArgs a{};
-    if (rot)
-        if (int rc = ensure_rope(ctx, rot->theta, head_dim, rot->position_offset + capacity,
-                                 &a.rope_table))
-            return rc;
-    a.k_src = k_src;
-    a.v_src = v_src;
-    a.k_pool = k_pool;
-    a.v_pool = v_pool;
-    a.slots = slots;
-    a.positions = positions;
-    a.ctx_lens = b->ctx_lens;
-    a.rope_positions = (int64_t)capacity;
-    a.rope_offset = rot ? (int)rot->position_offset : 0;
-    a.n_rows = (int)rows;
-    a.max_new = (int)max_new;
-    a.pool_rows = (int)(b->page_size * b->physical_pages);
-    a.kv_heads = (int)kv_heads;
-    a.head_dim = (int)head_dim;
-    unsigned grid[3];
-    begin_span(ctx);
-    fa::launch_append_slots((Dtype)dtype, a, ctx->stream, grid);
-    end_span(ctx, FA_KERNEL_PAGED_APPEND);
-    HIP_TRY(hipGetLastError());
-    record(ctx, FA_KERNEL_PAGED_APPEND, "append_slots", 0, (uint32_t)b->page_size, grid, 256, 1, 1,
-           nullptr);
+    return move_rows(ctx, b, slots, slots_bytes, positions, positions_bytes, max_new, k_src, v_src,
+                     src_bytes, k_pool, v_pool, pool_bytes, kv_heads, head_dim, rot, dtype, Rows::kAppend);
+}
+
+int fa_fp4_row_bytes(uint64_t kv_heads, uint64_t head_dim, uint64_t* out) {
+    if (!out) return fail(FA_ERR_NULL_ARGUMENT, "null argument");
+    if (int rc = check_fp4_row(kv_heads, head_dim)) return rc;
+    *out = (uint64_t)fa::fp4_row_bytes((int)kv_heads, (int)head_dim);
     return ok();
+}
+
+int fa_paged_append_slots_fp4(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* slots,
+                              size_t slots_bytes, const int32_t* positions, size_t positions_bytes,
+                              uint64_t max_new, const void* k_src, const void* v_src,
+                              size_t src_bytes, void* k_pool, void* v_pool, size_t pool_bytes,
+                              uint64_t kv_heads, uint64_t head_dim, const fa_rotary* rot, int dtype) {
+    return move_rows(ctx, b, slots, slots_bytes, positions, positions_bytes, max_new, k_src, v_src,
+                     src_bytes, k_pool, v_pool, pool_bytes, kv_heads, head_dim, rot, dtype,
+                     Rows::kAppendFp4);
+}
+
+int fa_paged_read_slots_fp4(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* slots,
+                            size_t slots_bytes, uint64_t max_new, const void* k_pool,
+                            const void* v_pool, size_t pool_bytes, void* k_out, void* v_out,
+                            size_t out_bytes, uint64_t kv_heads, uint64_t head_dim, int dtype) {
+    return move_rows(ctx, b, slots, slots_bytes, nullptr, 0, max_new, k_out, v_out, out_bytes,
+                     (void*)k_pool, (void*)v_pool, pool_bytes, kv_heads, head_dim, nullptr, dtype,
+                     Rows::kReadFp4);
 }
 
 int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q, size_t q_bytes,
@@ -3490,93 +3855,34 @@ int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q,
                             uint64_t max_tokens, uint64_t q_heads, uint64_t kv_heads,
                             uint64_t head_dim, const fa_config* cfg, const fa_rotary* rot,
                             int dtype) {
-    uint64_t capacity, row, lse, elements;
-    if (int rc = check_batch(b, true, &capacity)) return rc;
-    if (int rc = check_tree_tokens(max_tokens)) return rc;
-    if (!q_heads) return fail(FA_ERR_ZERO_DIMENSION, "attention dimensions must all be non-zero");
-    if (int rc = check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)) return rc;
-    if (q_heads % kv_heads)
-        return fail(FA_ERR_INVALID_HEAD_GROUPING,
-                    "q_heads (%llu) must be exactly divisible by kv_heads (%llu)",
-                    (unsigned long long)q_heads, (unsigned long long)kv_heads);
-    if (int rc = check_head_dim(head_dim, dtype)) return rc;
-    float scale;
-    if (int rc = resolve_scale(cfg, head_dim, &scale)) return rc;
-    if (rot)
-        if (int rc = check_rotary(rot->theta, rot->position_offset, head_dim, capacity)) return rc;
-    const uint64_t n = b->n_seqs, words = (max_tokens + 63) / 64;
-    if (q_heads > kI32 || n * max_tokens > kI32 || mul_ov(n * max_tokens, q_heads, &lse) || lse > kI32)
-        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "drafted tokens exceed the i32 index space");
-    // steps of 32 keys or more of every (sequence, kv head), and its start, counted in 32 bits
-    if (mul_ov(n * kv_heads, capacity / 32 + 16, &elements) || elements > kI32)
-        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the i32 index space");
-    // threads of the combine: 256 for every 32 rows of a (sequence, kv head)
-    if (n * kv_heads * ((max_tokens * (q_heads / kv_heads) + 31) / 32) > 0xffffff)
-        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "paged batch exceeds the launch space");
-    elements = lse * head_dim;
-    fa_packed_layout lay;
-    if (int rc = fa_packed_layout_for(elements, lse, dtype, &lay)) return rc;
-    if (int rc = check_buffer("Q", q, q_bytes, elements * elem_bytes(dtype))) return rc;
-    if (int rc = check_buffer("O|LSE", out_lse, out_bytes, lay.combined_bytes)) return rc;
-    if (int rc = check_aligned("Q", q)) return rc;
-    if (int rc = check_aligned("O|LSE", out_lse)) return rc;
-    if (int rc = check_buffer("tree lengths", tree_lens, tree_lens_bytes, n * 4)) return rc;
-    if (positions)
-        if (int rc = check_buffer("positions", positions, positions_bytes, n * max_tokens * 4)) return rc;
-    if (masks)
-        if (int rc = check_buffer("masks", masks, masks_bytes, n * max_tokens * words * 8)) return rc;
-    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
-    begin_call(ctx);
-    if (int rc = set_device(ctx)) return rc;
-    fa::TreeArgs a{};
-    if (rot)
-        if (int rc = ensure_rope(ctx, rot->theta, head_dim, rot->position_offset + capacity,
-                                 &a.rope_table))
-            return rc;
-    a.q = q;
-    a.k_pool = k_pool;
-    a.v_pool = v_pool;
-    a.o = out_lse;
-    a.lse = (float*)((uint8_t*)out_lse + lay.lse_byte_offset);
-    a.block_tables = b->block_tables;
-    a.ctx_lens = b->ctx_lens;
-    a.tree_lens = tree_lens;
-    a.positions = positions;
-    a.masks = masks;
-    a.rope_positions = (int)capacity;
-    a.rope_offset = rot ? (int)rot->position_offset : 0;
-    a.n_seqs = (int)n;
-    a.max_tokens = (int)max_tokens;
-    a.words = (int)words;
-    a.q_heads = (int)q_heads;
-    a.kv_heads = (int)kv_heads;
-    a.group = (int)(q_heads / kv_heads);
-    a.head_dim = (int)head_dim;
-    a.max_pages = (int)b->max_pages;
-    a.page_size = (int)b->page_size;
-    a.physical_pages = (int)b->physical_pages;
-    a.scale = scale;
-    size_t ml_offset, plan_offset, odd_offset;
-    const size_t bytes = fa::tree_workspace((Dtype)dtype, a, &ml_offset, &plan_offset, &odd_offset);
-    void* ws = nullptr;
-    if (int rc = grow(ctx, &ctx->ws_tree, &ctx->ws_tree_bytes, bytes, &ws)) return rc;
-    a.part_o = (float*)ws;
-    a.part_ml = (float2*)((uint8_t*)ws + ml_offset);
-    a.plan = (int*)((uint8_t*)ws + plan_offset);
-    a.odd = (int*)((uint8_t*)ws + odd_offset);
-    unsigned grid[3], block, q_rows;
-    begin_span(ctx);
-    fa::launch_tree_attention((Dtype)dtype, a, ctx->stream, grid, &block, &q_rows,
-                              [](void* c) {
-                                  end_span((fa_ctx*)c, FA_KERNEL_TREE_ATTENTION);
-                                  begin_span((fa_ctx*)c);
-                              },
-                              ctx);
-    end_span(ctx, FA_KERNEL_TREE_COMBINE);
-    HIP_TRY(hipGetLastError());
-    record(ctx, FA_KERNEL_TREE_ATTENTION, "tree_split + tree_combine", q_rows, 32, grid, block, 2, 1,
-           nullptr);
-    return ok();
+    return batch_attention(ctx, b, q, q_bytes, k_pool, v_pool, pool_bytes, out_lse, out_bytes,
+                           tree_lens, tree_lens_bytes, positions, positions_bytes, masks, masks_bytes,
+                           max_tokens, q_heads, kv_heads, head_dim, cfg, nullptr, rot, dtype, false);
+}
+
+int fa_paged_window_attention(fa_ctx* ctx, const fa_paged_batch* b, const void* q, size_t q_bytes,
+                              const void* k_pool, const void* v_pool, size_t pool_bytes,
+                              void* out_lse, size_t out_bytes, const int32_t* new_lens,
+                              size_t new_lens_bytes, const int32_t* positions,
+                              size_t positions_bytes, uint64_t max_tokens, uint64_t q_heads,
+                              uint64_t kv_heads, uint64_t head_dim, const fa_config* cfg,
+                              const fa_window* window, const fa_rotary* rot, int dtype) {
+    if (!window) return fail(FA_ERR_NULL_ARGUMENT, "window is null");
+    return batch_attention(ctx, b, q, q_bytes, k_pool, v_pool, pool_bytes, out_lse, out_bytes,
+                           new_lens, new_lens_bytes, positions, positions_bytes, nullptr, 0,
+                           max_tokens, q_heads, kv_heads, head_dim, cfg, window, rot, dtype, false);
+}
+
+int fa_paged_attention_fp4(fa_ctx* ctx, const fa_paged_batch* b, const void* q, size_t q_bytes,
+                           const void* k_pool, const void* v_pool, size_t pool_bytes, void* out_lse,
+                           size_t out_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                           const int32_t* positions, size_t positions_bytes, const uint64_t* masks,
+                           size_t masks_bytes, uint64_t max_tokens, uint64_t q_heads,
+                           uint64_t kv_heads, uint64_t head_dim, const fa_config* cfg,
+                           const fa_window* window, const fa_rotary* rot, int dtype) {
+    return batch_attention(ctx, b, q, q_bytes, k_pool, v_pool, pool_bytes, out_lse, out_bytes,
+                           tree_lens, tree_lens_bytes, positions, positions_bytes, masks, masks_bytes,
+                           max_tokens, q_heads, kv_heads, head_dim, cfg, window, rot, dtype, true);
 }
 
 int fa_paged_accept(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* paths,
@@ -3584,44 +3890,19 @@ int fa_paged_accept(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* paths,
                     size_t accepted_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
                     int32_t* ctx_lens_out, size_t ctx_lens_out_bytes, void* k_pool, void* v_pool,
                     size_t pool_bytes, uint64_t kv_heads, uint64_t head_dim, int dtype) {
-    uint64_t capacity, row, cells;
-    if (int rc = check_batch(b, true, &capacity)) return rc;
-    if (int rc = check_tree_tokens(max_accept)) return rc;
-    if (int rc = check_pools(b, k_pool, v_pool, pool_bytes, kv_heads, head_dim, dtype, &row)) return rc;
-    const uint64_t n = b->n_seqs;
-    if (mul_ov(n, max_accept, &cells) || cells > kI32)
-        return fail(FA_ERR_INDEX_SPACE_EXCEEDED, "accepted paths exceed the i32 index space");
-    if (int rc = check_buffer("paths", paths, paths_bytes, cells * 4)) return rc;
-    if (int rc = check_buffer("accepted", accepted, accepted_bytes, n * 4)) return rc;
-    if (int rc = check_buffer("tree lengths", tree_lens, tree_lens_bytes, n * 4)) return rc;
-    if (int rc = check_buffer("context lengths out", ctx_lens_out, ctx_lens_out_bytes, n * 4)) return rc;
-    if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
-    begin_call(ctx);
-    if (int rc = set_device(ctx)) return rc;
-    fa::AcceptArgs a{};
-    a.block_tables = b->block_tables;
-    a.ctx_lens = b->ctx_lens;
-    a.ctx_lens_out = ctx_lens_out;
-    a.paths = paths;
-    a.accepted = accepted;
-    a.tree_lens = tree_lens;
-    a.k_pool = k_pool;
-    a.v_pool = v_pool;
-    a.n_seqs = (int)n;
-    a.max_pages = (int)b->max_pages;
-    a.page_size = (int)b->page_size;
-    a.physical_pages = (int)b->physical_pages;
-    a.max_tokens = fa::kTreeTokens;
-    a.max_accept = (int)max_accept;
-    a.row_pieces = (int)(row / 16);
-    unsigned grid[3], block;
-    begin_span(ctx);
-    fa::launch_accept(a, ctx->stream, grid, &block);
-    end_span(ctx, FA_KERNEL_PAGED_ACCEPT);
-    HIP_TRY(hipGetLastError());
-    record(ctx, FA_KERNEL_PAGED_ACCEPT, "accept_rows", (uint32_t)max_accept, (uint32_t)b->page_size,
-           grid, block, 1, 1, nullptr);
-    return ok();
+    return accept_rows(ctx, b, paths, paths_bytes, max_accept, accepted, accepted_bytes, tree_lens,
+                       tree_lens_bytes, ctx_lens_out, ctx_lens_out_bytes, k_pool, v_pool, pool_bytes,
+                       kv_heads, head_dim, dtype, false);
+}
+
+int fa_paged_accept_fp4(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* paths,
+                        size_t paths_bytes, uint64_t max_accept, const int32_t* accepted,
+                        size_t accepted_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                        int32_t* ctx_lens_out, size_t ctx_lens_out_bytes, void* k_pool, void* v_pool,
+                        size_t pool_bytes, uint64_t kv_heads, uint64_t head_dim) {
+    return accept_rows(ctx, b, paths, paths_bytes, max_accept, accepted, accepted_bytes, tree_lens,
+                       tree_lens_bytes, ctx_lens_out, ctx_lens_out_bytes, k_pool, v_pool, pool_bytes,
+                       kv_heads, head_dim, FA_DTYPE_F32, true);
 }
 
 }  // extern "C"

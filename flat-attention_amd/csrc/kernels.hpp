@@ -61,6 +61,8 @@ struct PrefillArgs {
     // f32 kernel; null: none), so that a span brackets the kernel alone, as a profiler's dispatch
     // timestamps do.
     hipEvent_t ev_start, ev_stop;
+    // launch_prefill_window: position i sees the keys j <= i with i - j < window or j < sinks.
+    int window, sinks;
 };
 
 // The assembly prefill (64 query rows per wave, code object loaded per device): bf16, Q rotated
@@ -86,6 +88,11 @@ void launch_prefill(Dtype dt, bool paged, const PrefillArgs& a, hipStream_t s,
 // The grid, workgroup size and query rows per workgroup launch_prefill uses for `a` (host only).
 void prefill_geometry(Dtype dt, bool paged, const PrefillArgs& a, unsigned grid[3],
                       unsigned* block, unsigned* rows);
+
+// The same over a sliding window (contiguous rows of a multiple of 8 dims, 16-byte aligned, q_len == kv_len,
+// causal, K not rotated here). *rows, *keys: query rows of a workgroup, keys of a tile.
+void launch_prefill_window(Dtype dt, const PrefillArgs& a, hipStream_t s, unsigned grid[3],
+                           unsigned* block, unsigned* rows, unsigned* keys);
 
 // Paged q_len=1 decode, split-K over the context of every sequence.
 struct DecodeArgs {
@@ -161,6 +168,8 @@ struct BackwardArgs {
     // where it is the faster one, or always (kA64Never ...).
     // It reads `ld` as two f32 arrays of batch*q_heads*seq rows, -LSE / scale then -delta.
     int a64;
+    // launch_backward_window: position i sees the keys j <= i with i - j < window or j < sinks.
+    int window, sinks;
 };
 // How a dK/dV launch splits the query blocks that see a key block: `parts` chunks of `chunk` blocks
 // of 32 queries, each chunk's dK and dV in a workspace of `bytes` (`part`) when there are several.
@@ -262,6 +271,32 @@ void launch_backward_f32(const BackwardArgs& a, const BackwardSplit& sp, hipStre
 // tells whether the assembly dK/dV kernel ran.
 void launch_backward(Dtype dt, const BackwardArgs& a, const BackwardSplit& sp, hipStream_t s,
                      bool* a64_out = nullptr);
+
+// The same over a sliding window (a.dma, causal; three launches, no dS). The dK/dV launch has workgroups of
+// `chunk` tiles (of `tile` queries of a head): sink_parts for each of the key blocks with sinks, which come
+// first, then `parts` for each of the others; a workgroup's index is the slot of its partials, for the blocks
+// that have several (`part`, of `bytes`; the (batch, kv head) units of an index lie side by side).
+struct WindowSplit {
+    float* part;
+    int tile, chunk, blocks, sink_blocks, sink_parts, parts;
+    uint64_t bytes;
+    __host__ __device__ int workgroups() const {
+        return sink_blocks * sink_parts + (blocks - sink_blocks) * parts;
+    }
+    __host__ __device__ int slot(int kb, int p) const {
+        return kb < sink_blocks ? kb * sink_parts + p
+                                : sink_blocks * sink_parts + (kb - sink_blocks) * parts + p;
+    }
+    __device__ void coords(int idx, int& kb, int& p) const {
+        const int first = sink_blocks * sink_parts, n = idx < first ? sink_parts : parts;
+        const int i = idx < first ? idx : idx - first;
+        kb = i / n + (idx < first ? 0 : sink_blocks);
+        p = i % n;
+    }
+};
+// The split whose partials take at most `limit` bytes, `part` still to be set when bytes > 0.
+WindowSplit window_split(Dtype dt, const BackwardArgs& a, uint64_t limit);
+void launch_backward_window(Dtype dt, const BackwardArgs& a, const WindowSplit& sp, hipStream_t s);
 
 // The assembly dK/dV kernel (gen_bwd_a64.py): bf16 or f16, head_dim 128, seq a multiple of 128, dS
 // stored, 16-byte aligned tensors, 32-bit offsets; its module loaded on the current device.
@@ -380,7 +415,8 @@ struct AcceptArgs {
 };
 void launch_accept(const AcceptArgs& a, hipStream_t s, unsigned grid[3], unsigned* block);
 
-// Attention of drafted tokens over the paged cache, lengths and tables on the device.
+// Attention of drafted tokens over the paged cache, lengths and tables on the device. window > 0 (no
+// masks): token t, at row i = ctx_lens + t, sees the rows j <= i with i - j < window or j < sinks.
 struct TreeArgs {
     const void* q;  // [n_seqs, max_tokens, q_heads*head_dim]
     const void* k_pool;
@@ -397,6 +433,7 @@ struct TreeArgs {
     int rope_offset;
     int n_seqs, max_tokens, words, q_heads, kv_heads, group, head_dim;
     int max_pages, page_size, physical_pages;
+    int window, sinks;
     float scale;
     // Scratch (tree_workspace): partial O and (m, l) of the units that several key ranges share, and
     // the plan that the split kernel leaves for the combine: each sequence's place in the split,
@@ -413,5 +450,19 @@ size_t tree_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* pl
 // rows of a workgroup.
 void launch_tree_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned grid[3],
                            unsigned* block, unsigned* rows, void (*between)(void*), void* user);
+
+// A pool row of 4-bit floats: the codes of all heads, then their scales, up to a multiple of 16 bytes.
+__host__ __device__ inline int fp4_row_bytes(int kv_heads, int head_dim) {
+    const int codes = kv_heads * head_dim / 2;
+    return (codes + codes / 16 + 15) / 16 * 16;
+}
+// Rows to slots as launch_append_slots, into pools of 4-bit rows; and slots to rows of k_src, v_src's
+// layout (zeros for slots outside the pool), `a.k_src`, `a.v_src` being written then.
+void launch_append_fp4(Dtype dt, const SlotAppendArgs& a, hipStream_t s, unsigned grid[3]);
+void launch_read_fp4(Dtype dt, const SlotAppendArgs& a, hipStream_t s, unsigned grid[3]);
+// Attention as launch_tree_attention over pools of 4-bit rows; `dt` is Q's and O's type.
+size_t fp4_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset);
+void launch_fp4_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned grid[3],
+                          unsigned* block, unsigned* rows, void (*between)(void*), void* user);
 
 }  // namespace fa

@@ -128,6 +128,21 @@ __device__ __forceinline__ void block_coords(const PrefillKArgs& ka, int bid, in
     qb = __builtin_amdgcn_readfirstlane(qb);
 }
 
+// Which tiles of BN keys a block whose first query position is `first` leaves out of a window: `skip`
+// behind the first `before`, which hold the sinks.
+template <int BN>
+struct WindowTiles {
+    int before, skip;
+    __device__ __forceinline__ WindowTiles(const PrefillArgs& a, int first) {
+        const int low = max(0, first + 1 - a.window) / BN;  // tile of the first key it sees
+        before = (min(a.sinks, low * BN) + BN - 1) / BN;
+        skip = low - before;
+    }
+};
+// The power of two by which a window's f16 probabilities and their sum are kept larger: f16 has nothing
+// below 2^-25, and the sum, which is taken before the rounding, would hold what the product with V lost.
+template <typename T> constexpr float kWinLift = std::is_same<T, f16_t>::value ? 7.0f : 0.0f;
+
 // Running-max slack (log2 units) tolerated before O is rescaled: probabilities stay <= 2^8.
 constexpr float kRescaleLog2 = 8.0f;
 
@@ -196,10 +211,15 @@ __host__ __device__ constexpr bool prefill_pingpong(int pmode, bool ropek) {
 // the workgroup's waves form KW groups of RW = NW / KW waves on the same 32 RW rows; group k runs
 // the tiles k, k + KW, ... with an LDS region and a running (m, l, O) of its own, and the groups'
 // results are merged in LDS at the end.
+// WIN (launch_prefill_window): the tiles between the sinks and the first key that the block's first
+// position sees are left out; tiles are counted without them and tile_at() gives the place of one. A row
+// may see nothing of its first tiles. The row sum takes the probabilities before they are rounded, so that
+// LSE has f32 accuracy, and f16 ones are kept 2^7 times as large (WinLift).
 template <typename T, int DPAD, int PMODE, bool ROPEK, bool FULLD, int NW, bool SPLIT = false,
-          int KW = 1>
+          int KW = 1, bool WIN = false>
 __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(PrefillKArgs ka) {
     static_assert(!SPLIT || (ROPEK && NW == 4), "split scores need the in-kernel K rotation");
+    static_assert(!WIN || (PMODE == kContig && !ROPEK && !SPLIT && NW == 8), "contiguous, rotated K");
     using H = Half<T>;
     const PrefillArgs& a = ka.a;
     constexpr int RW = NW / KW;             // waves (of 32 rows) side by side
@@ -291,12 +311,16 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
     const int t_min = (int)ka.grp.div((uint32_t)r0w);
     int n_keys = kv_len_;
     if (a.causal) n_keys = min(n_keys, causal_off_ + t_max + 1);
-    const int n_tiles = __builtin_amdgcn_readfirstlane((n_keys + BN - 1) / BN);
+    const WindowTiles<BN> wt(a, (int)ka.grp.div((uint32_t)r0));
+    auto tile_at = [&](int m) { return WIN && m >= wt.before ? m + wt.skip : m; };
+    const int n_tiles =
+        __builtin_amdgcn_readfirstlane((n_keys + BN - 1) / BN - (WIN ? wt.skip : 0));
     const int cpos_min = causal_off_ + t_min;
     int n_keys_blk = kv_len_;
     if (a.causal)
         n_keys_blk = min(n_keys_blk, causal_off_ + min(q_len_ - 1, (int)ka.grp.div((uint32_t)(r0 + BM - 1))) + 1);
-    const int n_blk = __builtin_amdgcn_readfirstlane((n_keys_blk + BN - 1) / BN);
+    const int n_blk =
+        __builtin_amdgcn_readfirstlane((n_keys_blk + BN - 1) / BN - (WIN ? wt.skip : 0));
     (void)n_blk;
 
     // ---- Q^T operand, rotated in registers: lane holds Q[row][16ks + 8g .. +8]. The ping-pong
@@ -571,11 +595,16 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
     auto softmax_max = [&](f32x16_t (&sacc)[2], int tile, auto masked) {
         if constexpr (decltype(masked)::value) {
             const int lim = (a.causal ? min(kv_len_ - 1, cpos) : kv_len_ - 1) - tile * BN - 8 * g;
+            const int sinks = a.sinks - tile * BN - 8 * g;
+            (void)sinks;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (32 * kb + 16 * (i >> 3) + (i & 7) > lim) sacc[kb][i] = -INFINITY;
+                for (int i = 0; i < 16; ++i) {
+                    const int key = 32 * kb + 16 * (i >> 3) + (i & 7);
+                    if (WIN ? key > lim || (key < lim - a.window + 1 && key >= sinks) : key > lim)
+                        sacc[kb][i] = -INFINITY;
+                }
         }
         // row = this lane's query; partner lane ^ 32 holds the other keys. Four partial
         // chains keep the max and sum dependency chains short.
@@ -602,7 +631,10 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
     // ---- probabilities, row sum and the P^T operands (16 keys each)
     auto softmax_exp = [&](f32x16_t (&sacc)[2], u32x4_t (&pop)[4]) {
         // (a later key group's first tiles may hold no key that this row sees: m_run = -inf)
-        const float neg = KW > 1 && m_run == -INFINITY ? 0.0f : -m_run * c2;
+        constexpr float lift = WIN ? kWinLift<T> : 0.0f;
+        const float neg = (KW > 1 || WIN) && m_run == -INFINITY ? 0.0f
+                          : lift != 0.0f                        ? fmaf(-m_run, c2, lift)
+                                                                : -m_run * c2;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -620,7 +652,11 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
 #pragma unroll
         for (int s2 = 0; s2 < 4; ++s2)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) ls[j] = H::sum2(pop[s2][j], ls[j]);
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (WIN) ls[j] += sacc[s2 >> 1][(s2 & 1) * 8 + 2 * j] +
+                                            sacc[s2 >> 1][(s2 & 1) * 8 + 2 * j + 1];
+                else ls[j] = H::sum2(pop[s2][j], ls[j]);
+            }
         l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
     };
 
@@ -673,6 +709,13 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
     int n_full = kv_len_ / BN;
     if (a.causal) n_full = min(n_full, (cpos_min + 1) / BN);
     n_full = __builtin_amdgcn_readfirstlane(n_full);
+    // (WIN: those from first_full on, which the last row's window reaches)
+    int first_full = 0;
+    if constexpr (WIN) {
+        n_full -= wt.skip;
+        first_full = __builtin_amdgcn_readfirstlane(
+            (max(0, causal_off_ + t_max - a.window + 1) + BN - 1) / BN - wt.skip);
+    }
     using NoMask = std::integral_constant<bool, false>;
     using Mask = std::integral_constant<bool, true>;
 
@@ -765,8 +808,8 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
                 }
             };
             auto softmax_phase = [&](int m) {
-                if (m < n_full) softmax_max(sacc, m, NoMask{});
-                else softmax_max(sacc, m, Mask{});
+                if (m < n_full && (!WIN || m >= first_full)) softmax_max(sacc, m, NoMask{});
+                else softmax_max(sacc, tile_at(m), Mask{});
                 rescale_o();
                 softmax_exp(sacc, pop);
             };
@@ -783,8 +826,8 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
             auto start_dma = [&](int m) {
                 if (!xfer) return;
                 if constexpr (DMA) {
-                    if (m + 1 < n_blk) dma_k(m + 1, ((m + 1) & 1) * STAGE);
-                    if (m < n_blk) dma_v(m, (m & 1) * STAGE);
+                    if (m + 1 < n_blk) dma_k(tile_at(m + 1), ((m + 1) & 1) * STAGE);
+                    if (m < n_blk) dma_v(tile_at(m), (m & 1) * STAGE);
                 } else {
                     if (m + 1 < n_blk) load_one(m + 1, kb8, kreg);
                     if (m < n_blk) load_one(m, vb8, vreg);
@@ -807,7 +850,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
                 __syncthreads();
             };
             if constexpr (DMA) {
-                if (n_blk > 0 && xfer) dma_k(0, 0);
+                if (n_blk > 0 && xfer) dma_k(tile_at(0), 0);
                 load_q();
                 wait_dma();
             } else {
@@ -882,19 +925,19 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
         const int gbase = kg * NST * STAGE;
         static_assert(KW > 1, "one group takes the ping-pong loop");
         const int n_steps = (n_tiles + KW - 1) / KW;
-        if (kg < n_tiles) dma_tile(kg, gbase);
+        if (kg < n_tiles) dma_tile(tile_at(kg), gbase);
         wait_dma();
         __syncthreads();
         auto tile_step = [&](int i, auto masked) {
             const int tile = kg + KW * i;
             st_r = gbase + (i & 1) * STAGE;
             st_k = st_v = st_r;
-            if (tile + KW < n_tiles) dma_tile(tile + KW, gbase + STAGE - (i & 1) * STAGE);
+            if (tile + KW < n_tiles) dma_tile(tile_at(tile + KW), gbase + STAGE - (i & 1) * STAGE);
             if (tile < n_tiles) {
                 f32x16_t sacc[2];
                 u32x4_t pop[4];
                 compute_s(sacc, std::true_type{}, no_hook);
-                softmax_max(sacc, tile, masked);
+                softmax_max(sacc, tile_at(tile), masked);
                 rescale_o();
                 softmax_exp(sacc, pop);
                 compute_pv(pop, no_hook);
@@ -903,6 +946,8 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
             __syncthreads();
         };
         int i = 0;
+        if constexpr (WIN)
+            for (; i < n_steps && kg + KW * i < first_full; ++i) tile_step(i, Mask{});
         for (; i < (n_full - kg + KW - 1) / KW; ++i) tile_step(i, NoMask{});
         for (; i < n_steps; ++i) tile_step(i, Mask{});
         }
@@ -918,7 +963,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
             load_one(tile, kb8, kreg);
             load_v(tile);
         };
-        if (n_steps > 0) load_tile(min(kg, n_tiles - 1));
+        if (n_steps > 0) load_tile(tile_at(min(kg, n_tiles - 1)));
         for (int i = 0; i < n_steps; ++i) {
             const int tile = kg + KW * i;
             st_w = st_r = gbase + (NST == 2 ? (i & 1) * STAGE : 0);
@@ -928,12 +973,12 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
             store_v();
             __syncthreads();
             if (tile < n_tiles) {
-                load_tile(min(tile + KW, n_tiles - 1));
+                load_tile(tile_at(min(tile + KW, n_tiles - 1)));
                 f32x16_t sacc[2];
                 u32x4_t pop[4];
                 compute_s(sacc, std::true_type{}, no_hook);
-                if (tile < n_full) softmax_max(sacc, tile, NoMask{});
-                else softmax_max(sacc, tile, Mask{});
+                if (tile < n_full && (!WIN || tile >= first_full)) softmax_max(sacc, tile, NoMask{});
+                else softmax_max(sacc, tile_at(tile), Mask{});
                 rescale_o();
                 softmax_exp(sacc, pop);
                 compute_pv(pop, no_hook);
@@ -1003,7 +1048,8 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
         const float w =
             (m_run == -INFINITY ? 0.0f : fast_exp2((m_run - mx) * c2)) * (1.0f / l_all);
         if (kg == 0 && g == 0 && row_ok)
-            a.lse[(int64_t)b * a.lse_sb + (int64_t)hq * a.lse_sh + t] = mx * a.scale + logf(l_all);
+            a.lse[(int64_t)b * a.lse_sb + (int64_t)hq * a.lse_sh + t] =
+                mx * a.scale + logf(WIN ? l_all * fast_exp2(-kWinLift<T>) : l_all);
         __syncthreads();
         uint8_t* const dst = smem + (kg * BM + wave * 32 + (lane & 31)) * MROW + 16 * g;
 #pragma unroll
@@ -1074,7 +1120,8 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
     }
     if (row_ok) {
         if (g == 0)
-            a.lse[(int64_t)b * a.lse_sb + (int64_t)hq * a.lse_sh + t] = m_run * a.scale + logf(l_tot);
+            a.lse[(int64_t)b * a.lse_sb + (int64_t)hq * a.lse_sh + t] =
+                m_run * a.scale + logf(WIN ? l_tot * fast_exp2(-kWinLift<T>) : l_tot);
     }
     pad_rows();
 }
@@ -1088,7 +1135,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT ? 1 : 2) void prefill_mfma16(Prefill
 // tile's products); K rows are padded by one 16-byte slot so each lane reads four K operands
 // per 16-byte LDS read without bank conflicts. Otherwise tiles are staged through registers
 // (paged pools, K rotated on load, other head dims), K rows at an odd stride.
-template <int DPAD, bool PAGED, bool DMA = false>
+template <int DPAD, bool PAGED, bool DMA = false, bool WIN = false>
 __global__ __launch_bounds__(256, DMA ? 2 : 1) void prefill_mfma_f32(PrefillKArgs ka) {
     static_assert(!(DMA && PAGED), "transfers need contiguous K/V");
     const PrefillArgs& a = ka.a;
@@ -1147,7 +1194,9 @@ __global__ __launch_bounds__(256, DMA ? 2 : 1) void prefill_mfma_f32(PrefillKArg
     const int t_min = (int)ka.grp.div((uint32_t)r0);
     int n_keys = kv_len_;
     if (a.causal) n_keys = min(n_keys, causal_off_ + t_max + 1);
-    const int n_tiles = (n_keys + BN - 1) / BN;
+    const WindowTiles<BN> wt(a, t_min);
+    auto tile_at = [&](int m) { return WIN && m >= wt.before ? m + wt.skip : m; };
+    const int n_tiles = (n_keys + BN - 1) / BN - (WIN ? wt.skip : 0);
     const int cpos_min = causal_off_ + t_min;
 
     // Q operand: qv[ks] = Q[row][g*HALFD + ks] (rotated)
@@ -1229,16 +1278,26 @@ __global__ __launch_bounds__(256, DMA ? 2 : 1) void prefill_mfma_f32(PrefillKArg
     constexpr int PASSES = BN / RPP;
 
     if constexpr (DMA) {
-        if (n_tiles > 0) dma_tile(0, 0);
+        if (n_tiles > 0) dma_tile(tile_at(0), 0);
         wait_dma();
         __syncthreads();
     }
-    for (int tile = 0; tile < n_tiles; ++tile) {
+    // WIN: tiles that start in [open_at, open_at + open_span] need no mask (none: a start past every tile)
+    unsigned open_at = 0x7fffffff, open_span = 0;
+    if constexpr (WIN) {
+        const int from = max(0, causal_off_ + t_max - a.window + 1), to = cpos_min - BN + 1;
+        if (to >= from) {
+            open_at = from;
+            open_span = to - from;
+        }
+    }
+    for (int m = 0; m < n_tiles; ++m) {
+        const int tile = tile_at(m);
         const float* kst = k_lds;  // this tile's K and V rows in LDS
         const float* vst = v_lds;
         if constexpr (DMA) {
-            const int st = (tile & 1) * STAGE;
-            if (tile + 1 < n_tiles) dma_tile(tile + 1, STAGE - st);
+            const int st = (m & 1) * STAGE;
+            if (m + 1 < n_tiles) dma_tile(tile_at(m + 1), STAGE - st);
             kst = (const float*)(smem + st);
             vst = (const float*)(smem + st + KREG);
         } else {
@@ -1318,14 +1377,15 @@ __global__ __launch_bounds__(256, DMA ? 2 : 1) void prefill_mfma_f32(PrefillKArg
         // the maxima: with two, the compiler's wait states held along the longer way only (14 of 18).
         // (Waiting here instead: B4 H16 S2048 D128 causal 641 -> 650 us.)
         const int open_end = a.causal ? min(kv_len_ - 1, cpos_min) : kv_len_ - 1;
-        if (tile_end - 1 > open_end) {
+        if (WIN ? (unsigned)(tile_end - BN) - open_at > open_span : tile_end - 1 > open_end) {
             const int lim = a.causal ? min(kv_len_ - 1, cpos) : kv_len_ - 1;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int key = tile * BN + 32 * kb + 8 * (i >> 2) + 4 * g + (i & 3);
-                    if (key > lim) sacc[kb][i] = -INFINITY;
+                    if (WIN ? key > lim || (lim - key >= a.window && key >= a.sinks) : key > lim)
+                        sacc[kb][i] = -INFINITY;
                 }
         }
 
@@ -1339,14 +1399,15 @@ __global__ __launch_bounds__(256, DMA ? 2 : 1) void prefill_mfma_f32(PrefillKArg
             const bool need = mt * c2 > m_run * c2 + kRescaleLog2;
             if (__any(need)) {
                 const float m_use = need ? mt : m_run;
-                const float alpha = fast_exp2((m_run - m_use) * c2);
+                // (WIN: a row may not have seen a key yet)
+                const float alpha = !WIN || need ? fast_exp2((m_run - m_use) * c2) : 1.0f;
                 l_run *= alpha;
 #pragma unroll
                 for (int mb = 0; mb < MB; ++mb) oacc[mb] *= alpha;
                 m_run = m_use;
             }
         }
-        const float neg = -m_run * c2;
+        const float neg = WIN && m_run == -INFINITY ? 0.0f : -m_run * c2;
         float lsum = 0.0f;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -1401,7 +1462,7 @@ __global__ __launch_bounds__(256, DMA ? 2 : 1) void prefill_mfma_f32(PrefillKArg
 // memory into registers: K rows of the next tile and V columns of the next 32 dims are loaded
 // under the products. Same mapping as prefill_mfma_f32 (lane group g: k-index g of every step).
 // Contiguous K/V that is not rotated here, 16-byte aligned rows, head_dim % 4 == 0.
-template <int DPAD, int NW, bool FULL>
+template <int DPAD, int NW, bool FULL, bool WIN = false>
 __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void prefill_f32_groups(PrefillKArgs ka) {
     const PrefillArgs& a = ka.a;
     constexpr int HALFD = DPAD / 2, MB = DPAD / 32, NV = HALFD / 4;
@@ -1441,10 +1502,14 @@ __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void prefill_f32_grou
     const int t_min = (int)ka.grp.div((uint32_t)r0);
     int n_keys = kv_len_;
     if (a.causal) n_keys = min(n_keys, causal_off_ + t_max + 1);
-    const int n_tiles = __builtin_amdgcn_readfirstlane((n_keys + 31) / 32);
+    const WindowTiles<32> wt(a, t_min);
+    auto tile_at = [&](int m) { return WIN && m >= wt.before ? m + wt.skip : m; };
+    const int n_tiles = __builtin_amdgcn_readfirstlane((n_keys + 31) / 32 - (WIN ? wt.skip : 0));
     // last key that this lane's row sees, first key that some row of the block does not
     const int lim = a.causal ? min(kv_len_ - 1, causal_off_ + t) : kv_len_ - 1;
     const int clear = a.causal ? min(kv_len_, causal_off_ + t_min + 1) : kv_len_;
+    // (WIN: the first key that every row's window reaches)
+    const int near = WIN ? max(0, causal_off_ + t_max - a.window + 1) : 0;
 
     const int row_bytes = (int)a.k_ss * 4;
     const int64_t head = ((int64_t)b * a.k_sb + (int64_t)kvh * a.k_sh) * 4;
@@ -1471,7 +1536,7 @@ __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void prefill_f32_grou
             vc[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
                 rs, 4 * g * row_bytes + c * 4, (8 * (i >> 2) + (i & 3)) * row_bytes + mb * 128, 0));
     };
-    if (wave < n_tiles) load_k(wave);
+    if (wave < n_tiles) load_k(tile_at(wave));
 
     f32x4_t qv[NV];
     {
@@ -1504,7 +1569,8 @@ __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void prefill_f32_grou
     for (int mb = 0; mb < MB; ++mb) oacc[mb] = (f32x16_t)0.0f;
     float m_run = -INFINITY, l_run = 0.0f;
     const float c2 = a.scale * kLog2e;
-    for (int tile = wave; tile < n_tiles; tile += NW) {
+    for (int m = wave; m < n_tiles; m += NW) {
+        const int tile = tile_at(m);
         f32x16_t s = (f32x16_t)0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -1516,10 +1582,12 @@ __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void prefill_f32_grou
         float vc[16];
         load_v(rv, 0, vc);
         __builtin_amdgcn_sched_barrier(0);
-        if (tile * 32 + 32 > clear) {
+        if (WIN ? tile * 32 + 32 > clear || tile * 32 < near : tile * 32 + 32 > clear) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (tile * 32 + 8 * (i >> 2) + 4 * g + (i & 3) > lim) s[i] = -INFINITY;
+            for (int i = 0; i < 16; ++i) {
+                const int key = tile * 32 + 8 * (i >> 2) + 4 * g + (i & 3);
+                if (WIN ? key > lim || (lim - key >= a.window && key >= a.sinks) : key > lim) s[i] = -INFINITY;
+            }
         }
         float mt = s[0];
 #pragma unroll
@@ -1543,7 +1611,7 @@ __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void prefill_f32_grou
             lsum += s[i];
         }
         l_run += lsum;
-        if (tile + NW < n_tiles) load_k(tile + NW);
+        if (m + NW < n_tiles) load_k(tile_at(m + NW));
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
             float vm[16];
@@ -1869,6 +1937,64 @@ void launch_prefill(Dtype dt, bool paged, const PrefillArgs& a, hipStream_t s, u
             else launch32<false>(ka, dpad, g, s);
             break;
     }
+}
+
+// ------------------------------------------------------------------ sliding windows
+template <typename T, int DPAD, bool FULLD>
+static void launch_window16(const PrefillKArgs& ka, int kw, dim3 grid, hipStream_t s) {
+    if (kw == 4)
+        prefill_mfma16<T, DPAD, kContig, false, FULLD, 8, false, 4, true><<<grid, 512, 0, s>>>(ka);
+    else if (kw == 2)
+        prefill_mfma16<T, DPAD, kContig, false, FULLD, 8, false, 2, true><<<grid, 512, 0, s>>>(ka);
+    else
+        prefill_mfma16<T, DPAD, kContig, false, FULLD, 8, false, 1, true><<<grid, 512, 0, s>>>(ka);
+}
+template <int DPAD, int NW, bool FULLD>
+static void launch_window32(const PrefillKArgs& ka, bool groups, dim3 grid, hipStream_t s) {
+    if (groups) prefill_f32_groups<DPAD, NW, FULLD, true><<<grid, 64 * NW, 0, s>>>(ka);
+    else prefill_mfma_f32<DPAD, false, true, true><<<grid, 256, 0, s>>>(ka);
+}
+
+void launch_prefill_window(Dtype dt, const PrefillArgs& a, hipStream_t s, unsigned grid[3],
+                           unsigned* block, unsigned* rows, unsigned* keys) {
+    PrefillKArgs ka;
+    ka.a = a;
+    const bool f32 = dt == Dtype::F32;
+    const int64_t cus = device_cus(), units = (int64_t)a.batch * a.kv_heads;
+    const int64_t n_rows = (int64_t)a.q_len * a.group;
+    auto blocks = [&](int64_t bm) { return units * ((n_rows + bm - 1) / bm); };
+    int kw = 0;
+    if (f32) {
+        kw = blocks(32) <= 2 * cus;
+        *rows = kw ? 32 : 128;
+        *block = kw && a.head_dim <= 64 ? 512 : 256;
+        *keys = 32;
+    } else {
+        kw = blocks(64) <= cus ? 4 : blocks(128) <= cus ? 2 : 1;
+        *rows = (unsigned)(256 / kw);
+        *block = 512;
+        *keys = 64;
+    }
+    grid[0] = (unsigned)blocks(*rows);
+    grid[1] = grid[2] = 1;
+    ka.set_grid(grid[0], *rows);
+    const dim3 g(grid[0]);
+    auto go = [&](auto dpad, auto full) {
+        constexpr int DP = decltype(dpad)::value;
+        constexpr bool FULLD = decltype(full)::value;
+        switch (dt) {
+            case Dtype::BF16: launch_window16<bf16_t, DP, FULLD>(ka, kw, g, s); break;
+            case Dtype::F16: launch_window16<f16_t, DP, FULLD>(ka, kw, g, s); break;
+            default: launch_window32<DP, DP == 128 ? 4 : 8, FULLD>(ka, kw != 0, g, s); break;
+        }
+    };
+    auto dims = [&](auto dpad) {
+        if (a.head_dim == decltype(dpad)::value) go(dpad, std::true_type{});
+        else go(dpad, std::false_type{});
+    };
+    if (a.head_dim <= 32) dims(std::integral_constant<int, 32>{});
+    else if (a.head_dim <= 64) dims(std::integral_constant<int, 64>{});
+    else dims(std::integral_constant<int, 128>{});
 }
 
 }  // namespace fa

@@ -11,8 +11,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "common.hpp"
-#include "kernels.hpp"
+#include "tree.hpp"
 
 namespace fa {
 
@@ -134,32 +133,11 @@ __device__ __forceinline__ void global_to_lds16(const void* p, uint32_t lds) {
     asm volatile("global_load_lds_dwordx4 %0, off nt" : : "v"(p), "{m0}"(lds));
 }
 
-// Division of numbers below 2^31 by a constant of the launch, in 32 bits: with s = ceil(log2 d) and
-// m = floor(2^(31 + s) / d) + 1, m d - 2^(31 + s) <= 2^s, so n m / 2^(31 + s) is off by less than 1 / d.
-struct SmallDiv {
-    uint32_t m, s;
-    __host__ SmallDiv() : m(0), s(0) {}
-    __host__ explicit SmallDiv(uint32_t d) {
-        for (s = 0; (1ull << s) < d; ++s) {
-        }
-        m = (uint32_t)((1ull << (31 + s)) / d + 1);
-    }
-    __device__ __forceinline__ int div(int n) const { return (int)(__umulhi((uint32_t)n << 1, m) >> s); }
-};
-
 struct TreeKArgs {
     TreeArgs a;
     SmallDiv ps, grp;
     FastDiv ranges, row_blocks;
 };
-
-// Live rows of a sequence, drafted ones included; 0: it has no part in this call.
-__device__ __forceinline__ int tree_rows_of(const TreeArgs& a, int s) {
-    const int ctx = a.ctx_lens[s], len = a.tree_lens[s];
-    const bool ok = ctx >= 0 && len > 0 && len <= a.max_tokens &&
-                    (int64_t)ctx + len <= (int64_t)a.max_pages * a.page_size;
-    return ok ? ctx + len : 0;
-}
 
 // Bits of a word's values (one f32, two 16-bit) that are infinite or NaN.
 template <typename T>
@@ -217,19 +195,7 @@ __device__ __forceinline__ void write_row4(const TreeArgs& a, int s, int kvh, in
             none ? -INFINITY : m * a.scale + logf(l * (1.0f / (1 << kTreeLift<T>)));
 }
 
-// Inclusive prefix sum over a wave (row shifts by 1, 2, 4, 8, then the last lane of each row of 16 to
-// the next row, and of the first half to the second).
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-    return v;
-}
-
-template <typename T, int DPAD, int RW, int HW, bool SPLIT>
+template <typename T, int DPAD, int RW, int HW, bool SPLIT, bool WIN = false>
 __global__ __launch_bounds__((64 * TreeCfg<T, DPAD, RW, HW>::NW),
                              (TreeCfg<T, DPAD, RW, HW>::WAVES))
 void tree_split(TreeKArgs ka) {
@@ -256,11 +222,16 @@ void tree_split(TreeKArgs ka) {
 
     // ---- this workgroup's range of steps [pos, end), and the sequence that holds the first; every wave
     // for itself, without a barrier
-    auto steps_of = [&](int rows) { return (rows + C::KT - 1) / C::KT; };
+    auto steps_of = [&](int rows, int len) {
+        int n = (rows + C::KT - 1) / C::KT, before;
+        if constexpr (WIN) n -= tree_skip(a, rows, len, C::KT, &before);
+        return n;
+    };
     auto rows_of = [&](int i) { return i < a.n_seqs ? tree_rows_of(a, i) : 0; };
+    auto len_of = [&](int i) { return WIN ? a.tree_lens[min(i, a.n_seqs - 1)] : 0; };
     int mine = 0, count = 0;  // steps, and units that have any
     for (int i = lane; i < a.n_seqs; i += 64) {
-        const int n = steps_of(rows_of(i));
+        const int n = steps_of(rows_of(i), len_of(i));
         mine += units * n;
         count += n ? units : 0;
     }
@@ -268,7 +239,7 @@ void tree_split(TreeKArgs ka) {
     const int n_units = __builtin_amdgcn_readlane(wave_scan(count), 63);
     const int ov = min(kTreeStart, (int)ka.ranges.div((uint32_t)n_steps) / 2);
     const int total = n_steps + n_units * ov;
-    auto length_of = [&](int rows) { return rows ? steps_of(rows) + ov : 0; };  // of a unit
+    auto length_of = [&](int rows, int len) { return rows ? steps_of(rows, len) + ov : 0; };  // of a unit
     const int share = max(1, (int)ka.ranges.div((uint32_t)total + ka.ranges.d - 1));
     int64_t pos = (int64_t)range * share;
     const int64_t end = pos + share < total ? pos + share : total;
@@ -280,7 +251,7 @@ void tree_split(TreeKArgs ka) {
     int s = 0, first = 0, rows_s = 0, len = 0;  // the sequence, its first step, its rows, the drafted ones
     bool found = pos >= end;
     for (int base = 0, carry = 0; base < a.n_seqs && (plans || !found); base += 64) {
-        const int rows = rows_of(base + lane), v = units * length_of(rows);
+        const int rows = rows_of(base + lane), v = units * length_of(rows, len_of(base + lane));
         const int upto = carry + wave_scan(v);
         if (plans && base + lane < a.n_seqs) a.plan[base + lane] = upto - v;
         const uint64_t past = __ballot(upto > pos);
@@ -323,13 +294,13 @@ void tree_split(TreeKArgs ka) {
 
     while (pos < end) {
         // ---- the unit that holds step pos and this range's part of it
-        while (pos >= (int64_t)first + units * length_of(rows_s)) {
-            first += units * length_of(rows_s);
+        while (pos >= (int64_t)first + units * length_of(rows_s, len)) {
+            first += units * length_of(rows_s, len);
             ++s;
             rows_s = __builtin_amdgcn_readfirstlane(tree_rows_of(a, s));
             len = __builtin_amdgcn_readfirstlane(a.tree_lens[s]);
         }
-        const int steps = steps_of(rows_s);
+        const int steps = steps_of(rows_s, len);
         const int in_seq = (int)(pos - first);
         const int unit = __builtin_amdgcn_readfirstlane(in_seq / (steps + ov)), kvh = unit * HW + hd;
         const int from = in_seq - unit * (steps + ov);
@@ -420,12 +391,17 @@ void tree_split(TreeKArgs ka) {
         const uint8_t* const vpool = (const uint8_t*)a.v_pool + (int64_t)kvh * D * C::EB;
         const int* const table = a.block_tables + (int64_t)s * a.max_pages;
 
-        for (int c0 = st0; c0 < st1;) {
+        // (WIN: behind the first `before` steps `skip` are left out, and a part of the loop ends there)
+        int before = 0, skip = 0;
+        if constexpr (WIN) skip = tree_skip(a, rows_s, len, C::KT, &before);
+        for (int at0 = st0; at0 < st1;) {
+            const int shift = WIN && at0 >= before ? skip : 0, c0 = at0 + shift;
+            const int part = WIN && at0 < before && skip > 0 ? min(st1, before) : st1 + shift;
             // ---- table entries of as many steps as they cover: first pool row of each page, -1 where
             // the id lies outside the pool
             const int p0 = ka.ps.div(c0 * C::KT);
             const int64_t reach = ((int64_t)p0 + kTreePages) * page_size;  // keys below are covered
-            const int c1 = (int)min((int64_t)st1, max((int64_t)c0 + 1, reach / C::KT));
+            const int c1 = (int)min((int64_t)part, max((int64_t)c0 + 1, reach / C::KT));
             const int k_end = min(c1 * C::KT, rows_s);
             const int n_pages = ka.ps.div(k_end - 1) - p0 + 1;
             bool bad = false;
@@ -523,24 +499,10 @@ void tree_split(TreeKArgs ka) {
                 if constexpr (MASKED) {
                     wait_mfma32<F32>(sc);
                     const int j0 = key0 - ctx;  // drafted token of the first key
-                    uint64_t w;
-                    if (a.masks) {
-                        const uint64_t* const m = a.masks + (int64_t)tok * a.words;
-                        const int at64 = j0 >= 0 ? j0 >> 6 : 0, sh = j0 & 63;
-                        uint64_t w0 = mask0, w1 = 0;
-                        if (a.words > 1) {
-                            w0 = row_ok && at64 < a.words ? m[at64] : 0;
-                            w1 = row_ok && j0 >= 0 && at64 + 1 < a.words ? m[at64 + 1] : 0;
-                        } else if (at64 > 0) {
-                            w0 = 0;
-                        }
-                        if (j0 >= 0) w = (w0 >> sh) | (sh ? w1 << (64 - sh) : 0);
-                        else if (j0 > -32) w = w0 << -j0 | ((1u << -j0) - 1u);
-                        else w = 0xffffffffu;
-                    } else {
-                        const int last = t - j0;  // keys 0..last
-                        w = last >= 31 ? 0xffffffffu : last >= 0 ? (2u << last) - 1u : 0u;
-                    }
+                    uint32_t w;
+                    if constexpr (WIN) w = window_word(a, ctx + t, key0);
+                    else if (a.masks) w = mask_word(a, row_ok, tok, mask0, j0);
+                    else w = causal_word(t, j0);
                     // keys past the live rows, and on pages that are not there
                     const int left = k_end - key0;
                     uint32_t there = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
@@ -549,7 +511,7 @@ void tree_split(TreeKArgs ka) {
                         const int lp = ka.ps.div(key);
                         there &= (uint32_t)__ballot(bt_lds[lp - p0] >= 0);
                     }
-                    const uint32_t see = ((uint32_t)w & there) >> (4 * h);  // this row sees these keys
+                    const uint32_t see = (w & there) >> (4 * h);  // this row sees these keys
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (!((see >> (8 * (i / 4) + i % 4)) & 1)) sc[i] = -INFINITY;
@@ -641,7 +603,7 @@ void tree_split(TreeKArgs ka) {
                 }
                 // (the larger one of all units and parts of this range)
                 if constexpr (MASKED)
-                    if (__any(off != 0) && lane == 0) odd_lds[wave] = max(odd_lds[wave], bad ? 2 : 1);
+                    if (__any(off != 0) && lane == 0) odd_lds[wave] = max(odd_lds[wave], WIN || bad ? 2 : 1);
             };
 
             // ---- the steps, NST - 1 transfers ahead: first those whose keys every row sees
@@ -775,11 +737,19 @@ void tree_split(TreeKArgs ka) {
                 }
                 }
             };
-            const int cm = bad ? c0 : max(c0, min(c1, ctx / C::KT));
-            if constexpr (C::PIPE) run_pipe(c0, cm);
+            int cm = bad ? c0 : max(c0, min(c1, ctx / C::KT));
+            if constexpr (WIN) {
+                // steps before ca hold keys that the last token's window does not reach (or sinks)
+                const int reached = (max(0, rows_s - a.window) + C::KT - 1) / C::KT;
+                const int ca = bad ? c1 : max(c0, min(c1, reached));
+                run(c0, ca, std::true_type{});
+                cm = max(ca, cm);
+                if constexpr (C::PIPE) run_pipe(ca, cm);
+                else run(ca, cm, std::false_type{});
+            } else if constexpr (C::PIPE) run_pipe(c0, cm);
             else run(c0, cm, std::false_type{});
             run(cm, c1, std::true_type{});
-            c0 = c1;
+            at0 = c1 - shift;
         }
 
         // ---- finished rows to O and LSE, partial ones to their slot: per 32-row block the quads (four
@@ -921,7 +891,8 @@ __global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rw
             if (d0 + 32 * n < D) write_row4<T>(a, s, kvh, row, d0 + 32 * n, zero, 0.0f, 0.0f, ka.grp);
     }
     if (b32 * 32 >= len * a.group) return;
-    const int steps = (rows_s + kt - 1) / kt;
+    int before_skip, steps = (rows_s + kt - 1) / kt;
+    if (a.window) steps -= tree_skip(a, rows_s, len, kt, &before_skip);
     const uint32_t u0 = (uint32_t)before + (uint32_t)(kvh / hw) * (uint32_t)(steps + ov) + (uint32_t)ov;
     const int g0 = (int)(u0 / (uint32_t)share), g1 = (int)((u0 + steps - 1) / (uint32_t)share);
     const int rb = b32 / rw, in = b32 - rb * rw;
@@ -1011,7 +982,8 @@ __global__ __launch_bounds__(256) void tree_combine(TreeKArgs ka, int kt, int rw
         f32x4_t add = zero;
         for (int key = odd > 1 ? 0 : ctx / kt * kt; key < rows_s; ++key) {
             const int j = key - ctx;
-            const bool seen = j < 0 ? true
+            const bool seen = a.window ? j <= t && (t - j < a.window || key < a.sinks)
+                              : j < 0  ? true
                               : a.masks
                                   ? (a.masks[((int64_t)s * a.max_tokens + t) * a.words + (j >> 6)] >> (j & 63)) & 1
                                   : j <= t;
@@ -1148,13 +1120,18 @@ static void launch_t(TreeKArgs& ka, hipStream_t st, unsigned grid[3], unsigned* 
     *rows = (unsigned)(32 * s.rw);
     tree_dispatch<T>(a, [&](auto dpad, auto rw, auto hw) {
         constexpr int DP = decltype(dpad)::value, RW = decltype(rw)::value, HW = decltype(hw)::value;
-        if constexpr (!std::is_same<T, float>::value) {
-            if (a.rope_table) {
-                tree_split<T, DP, RW, HW, true><<<grid[0], s.threads, 0, st>>>(ka);
-                return;
+        const auto split = [&](auto win) {
+            constexpr bool WIN = decltype(win)::value;
+            if constexpr (!std::is_same<T, float>::value) {
+                if (a.rope_table) {
+                    tree_split<T, DP, RW, HW, true, WIN><<<grid[0], s.threads, 0, st>>>(ka);
+                    return;
+                }
             }
-        }
-        tree_split<T, DP, RW, HW, false><<<grid[0], s.threads, 0, st>>>(ka);
+            tree_split<T, DP, RW, HW, false, WIN><<<grid[0], s.threads, 0, st>>>(ka);
+        };
+        if (a.window) split(std::true_type{});
+        else split(std::false_type{});
     });
     if (between) between(user);
     const int blocks = (a.max_tokens * a.group + 31) / 32;

@@ -8,7 +8,7 @@ and fails loudly when it has not been built.
 
 from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, LIB_PATH, FlatHipError, lib)
 from .api import (AsymmetricGroupedAttentionShape, AsymmetricRotaryEmbeddingConfig,
-                  AttentionShape, DeviceBuffer, FlatAttentionConfig, FlatAttentionOutput,
+                  AttentionShape, AttentionWindow, DeviceBuffer, FlatAttentionConfig, FlatAttentionOutput,
                   GroupedAttentionShape, HipAsymmetricProjectionPipeline,
                   HipChunkedProjectionPrefillPipeline, HipContext, HipFlatAttention, HipGraph,
                   HipPagedBatch, HipPagedDecodePipeline,
@@ -24,7 +24,7 @@ from .api import (AsymmetricGroupedAttentionShape, AsymmetricRotaryEmbeddingConf
                   grouped_backward_layout, pack_grouped_backward_recompute_inputs,
                   HipBackwardRecomputePipeline, pack_backward_recompute_inputs,
                   bf16_bits_to_f32, download_attention,
-                  f32_to_bf16_bits, host_storage, packed_layout, paged_append_batched,
+                  f32_to_bf16_bits, fp4_row_bytes, host_storage, packed_layout, paged_append_batched,
                   paged_decode_noalloc,
                   storage_np_dtype, storage_to_f32)
 

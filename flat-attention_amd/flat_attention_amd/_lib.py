@@ -68,6 +68,10 @@ class RotaryC(ctypes.Structure):
     _fields_ = [("theta", F32), ("position_offset", U64)]
 
 
+class WindowC(ctypes.Structure):
+    _fields_ = [("window", U64), ("sinks", U64)]
+
+
 class VariableSequenceC(ctypes.Structure):
     _fields_ = [("active_query_len", U64), ("active_kv_len", U64),
                 ("query_position_offset", U64), ("query_rope_position_offset", U64)]
@@ -225,6 +229,23 @@ PROTOTYPES = {
                                       SZ, VP, SZ, U64, U64, U64, U64, P(ConfigC), P(RotaryC), INT]),
     "fa_paged_accept": (INT, [VP, P(PagedBatchC), VP, SZ, U64, VP, SZ, VP, SZ, VP, SZ, VP, VP, SZ,
                               U64, U64, INT]),
+    "fa_forward_gqa_window": (INT, [VP, VP, SZ, VP, VP, SZ, VP, SZ, P(GroupedShapeC), P(ConfigC),
+                                    P(WindowC), P(RotaryC), INT]),
+    "fa_backward_gqa_window": (INT, [VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, P(GroupedShapeC),
+                                     P(ConfigC), P(WindowC), INT]),
+    "fa_paged_window_attention": (INT, [VP, P(PagedBatchC), VP, SZ, VP, VP, SZ, VP, SZ, VP, SZ, VP,
+                                        SZ, U64, U64, U64, U64, P(ConfigC), P(WindowC), P(RotaryC),
+                                        INT]),
+    "fa_fp4_row_bytes": (INT, [U64, U64, P(U64)]),
+    "fa_paged_append_slots_fp4": (INT, [VP, P(PagedBatchC), VP, SZ, VP, SZ, U64, VP, VP, SZ, VP, VP,
+                                        SZ, U64, U64, P(RotaryC), INT]),
+    "fa_paged_read_slots_fp4": (INT, [VP, P(PagedBatchC), VP, SZ, U64, VP, VP, SZ, VP, VP, SZ, U64,
+                                      U64, INT]),
+    "fa_paged_attention_fp4": (INT, [VP, P(PagedBatchC), VP, SZ, VP, VP, SZ, VP, SZ, VP, SZ, VP,
+                                     SZ, VP, SZ, U64, U64, U64, U64, P(ConfigC), P(WindowC),
+                                     P(RotaryC), INT]),
+    "fa_paged_accept_fp4": (INT, [VP, P(PagedBatchC), VP, SZ, U64, VP, SZ, VP, SZ, VP, SZ, VP, VP, SZ,
+                                  U64, U64]),
     "fa_last_telemetry": (INT, [VP, P(TelemetryC)]),
     "fa_forward_gqa_rope_telemetry": (INT, [VP, P(GroupedShapeC), P(ConfigC), P(RotaryC), INT,
                                             P(TelemetryC)]),

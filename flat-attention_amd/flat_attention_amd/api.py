@@ -116,6 +116,16 @@ class RotaryEmbeddingConfig:
 
 
 @dataclass(frozen=True)
+class AttentionWindow:
+    """fa_window: position i sees the keys j <= i with i - j < window, and those with j < sinks."""
+    window: int
+    sinks: int = 0
+
+    def c(self):
+        return L.WindowC(self.window, self.sinks)
+
+
+@dataclass(frozen=True)
 class AsymmetricRotaryEmbeddingConfig:
     """AsymmetricRotaryEmbeddingConfig src/projection_asymmetric.rs:19."""
     theta: float
@@ -523,6 +533,20 @@ class HipRotaryGroupedAttention:
                                         min(k.nbytes, v.nbytes), out.ptr, out.nbytes,
                                         ctypes.byref(shape.c()), ctypes.byref(config.c()), rot,
                                         self.dtype))
+        return out
+
+    def forward_window(self, q, k, v, shape: GroupedAttentionShape, config: FlatAttentionConfig,
+                       window: AttentionWindow, rotary: Optional[RotaryEmbeddingConfig] = None,
+                       out: Optional[DeviceBuffer] = None) -> DeviceBuffer:
+        """Causal attention with a sliding window and sinks (fa_forward_gqa_window; no reference
+        counterpart), otherwise as forward_resident."""
+        lay = self.layout(shape)
+        out = out or DeviceBuffer(self.ctx, lay.combined_bytes)
+        rot = ctypes.byref(rotary.c()) if rotary is not None else None
+        check(lib().fa_forward_gqa_window(self.ctx.handle, q.ptr, q.nbytes, k.ptr, v.ptr,
+                                          min(k.nbytes, v.nbytes), out.ptr, out.nbytes,
+                                          ctypes.byref(shape.c()), ctypes.byref(config.c()),
+                                          ctypes.byref(window.c()), rot, self.dtype))
         return out
 
     def prepare(self, q, k, v, out, shape: GroupedAttentionShape, config: FlatAttentionConfig,
@@ -1213,6 +1237,80 @@ class HipPagedBatch:
             v_pool.ptr, min(k_pool.nbytes, v_pool.nbytes), kv_heads, head_dim, dtype))
 
 
+    def window_attention(self, q: DeviceBuffer, k_pool: DeviceBuffer, v_pool: DeviceBuffer,
+                         out_and_lse: DeviceBuffer, new_lens: DeviceBuffer, max_tokens: int,
+                         q_heads: int, kv_heads: int, head_dim: int, config: FlatAttentionConfig,
+                         window: AttentionWindow, rotary: Optional[RotaryEmbeddingConfig],
+                         dtype: int, positions: Optional[DeviceBuffer] = None):
+        """Attention of new tokens over the cache with a sliding window and sinks
+        (fa_paged_window_attention); the output's layout is that of tree_attention."""
+        check(lib().fa_paged_window_attention(
+            self.ctx.handle, self._c, q.ptr, q.nbytes, k_pool.ptr, v_pool.ptr,
+            min(k_pool.nbytes, v_pool.nbytes), out_and_lse.ptr, out_and_lse.nbytes, new_lens.ptr,
+            new_lens.nbytes, positions.ptr if positions is not None else None,
+            positions.nbytes if positions is not None else 0, max_tokens, q_heads, kv_heads,
+            head_dim, config.c(), window.c(), rotary.c() if rotary is not None else None, dtype))
+
+    # ---- the pools in 4 bits a value: rows of fp4_row_bytes(kv_heads, head_dim) bytes
+
+    def append_fp4(self, slots: DeviceBuffer, max_new: int, k_src: DeviceBuffer, v_src: DeviceBuffer,
+                   k_pool: DeviceBuffer, v_pool: DeviceBuffer, kv_heads: int, head_dim: int,
+                   rotary: Optional[RotaryEmbeddingConfig], dtype: int,
+                   positions: Optional[DeviceBuffer] = None):
+        """New rows to their slots in 4 bits, K rotated on the way (fa_paged_append_slots_fp4)."""
+        check(lib().fa_paged_append_slots_fp4(
+            self.ctx.handle, self._c, slots.ptr, slots.nbytes,
+            positions.ptr if positions is not None else None,
+            positions.nbytes if positions is not None else 0, max_new, k_src.ptr, v_src.ptr,
+            min(k_src.nbytes, v_src.nbytes), k_pool.ptr, v_pool.ptr,
+            min(k_pool.nbytes, v_pool.nbytes), kv_heads, head_dim,
+            rotary.c() if rotary is not None else None, dtype))
+
+    def read_fp4(self, slots: DeviceBuffer, max_new: int, k_pool: DeviceBuffer, v_pool: DeviceBuffer,
+                 k_out: DeviceBuffer, v_out: DeviceBuffer, kv_heads: int, head_dim: int, dtype: int):
+        """The rows in these slots as `dtype` (fa_paged_read_slots_fp4)."""
+        check(lib().fa_paged_read_slots_fp4(
+            self.ctx.handle, self._c, slots.ptr, slots.nbytes, max_new, k_pool.ptr, v_pool.ptr,
+            min(k_pool.nbytes, v_pool.nbytes), k_out.ptr, v_out.ptr,
+            min(k_out.nbytes, v_out.nbytes), kv_heads, head_dim, dtype))
+
+    def attention_fp4(self, q: DeviceBuffer, k_pool: DeviceBuffer, v_pool: DeviceBuffer,
+                      out_and_lse: DeviceBuffer, tree_lens: DeviceBuffer, max_tokens: int,
+                      q_heads: int, kv_heads: int, head_dim: int, config: FlatAttentionConfig,
+                      rotary: Optional[RotaryEmbeddingConfig], dtype: int,
+                      positions: Optional[DeviceBuffer] = None,
+                      masks: Optional[DeviceBuffer] = None,
+                      window: Optional[AttentionWindow] = None):
+        """tree_attention, or with a window window_attention, over 4-bit pools
+        (fa_paged_attention_fp4)."""
+        check(lib().fa_paged_attention_fp4(
+            self.ctx.handle, self._c, q.ptr, q.nbytes, k_pool.ptr, v_pool.ptr,
+            min(k_pool.nbytes, v_pool.nbytes), out_and_lse.ptr, out_and_lse.nbytes, tree_lens.ptr,
+            tree_lens.nbytes, positions.ptr if positions is not None else None,
+            positions.nbytes if positions is not None else 0,
+            masks.ptr if masks is not None else None,
+            masks.nbytes if masks is not None else 0, max_tokens, q_heads, kv_heads, head_dim,
+            config.c(), window.c() if window is not None else None,
+            rotary.c() if rotary is not None else None, dtype))
+
+    def accept_fp4(self, paths: DeviceBuffer, max_accept: int, accepted: DeviceBuffer,
+                   tree_lens: DeviceBuffer, k_pool: DeviceBuffer, v_pool: DeviceBuffer, kv_heads: int,
+                   head_dim: int, ctx_lens_out: Optional[DeviceBuffer] = None):
+        """accept over 4-bit pools (fa_paged_accept_fp4)."""
+        out = self.ctx_lens if ctx_lens_out is None else ctx_lens_out
+        check(lib().fa_paged_accept_fp4(
+            self.ctx.handle, self._c, paths.ptr, paths.nbytes, max_accept, accepted.ptr,
+            accepted.nbytes, tree_lens.ptr, tree_lens.nbytes, out.ptr, out.nbytes, k_pool.ptr,
+            v_pool.ptr, min(k_pool.nbytes, v_pool.nbytes), kv_heads, head_dim))
+
+
+def fp4_row_bytes(kv_heads: int, head_dim: int) -> int:
+    """Bytes of a row of a 4-bit pool (fa_fp4_row_bytes): one token of all kv heads."""
+    out = L.U64()
+    check(lib().fa_fp4_row_bytes(kv_heads, head_dim, ctypes.byref(out)))
+    return out.value
+
+
 # ----------------------------------------------------------------------------- backward
 
 @dataclass
@@ -1315,6 +1413,16 @@ class HipGroupedBackwardRecomputePipeline:
                                         lse_ptr, dq.ptr, dk.ptr, dv.ptr,
                                         ctypes.byref(shape.c()), ctypes.byref(config.c()),
                                         self.dtype))
+
+    def encode_window(self, q, k, v, d_out, out, lse_ptr: int, dq, dk, dv,
+                      shape: GroupedAttentionShape, config: FlatAttentionConfig,
+                      window: AttentionWindow):
+        """The backward of :meth:`HipRotaryGroupedAttention.forward_window` (fa_backward_gqa_window;
+        no reference counterpart) over separate device tensors, as encode_tensors."""
+        check(lib().fa_backward_gqa_window(self.ctx.handle, q.ptr, k.ptr, v.ptr, d_out.ptr, out.ptr,
+                                           lse_ptr, dq.ptr, dk.ptr, dv.ptr,
+                                           ctypes.byref(shape.c()), ctypes.byref(config.c()),
+                                           ctypes.byref(window.c()), self.dtype))
 
     def download_gradients(self, grads: DeviceBuffer,
                            shape: GroupedAttentionShape) -> FlatAttentionBackwardOutput:

@@ -231,6 +231,23 @@ int fa_forward_gqa_rope(fa_ctx* ctx, const void* q, size_t q_bytes, const void* 
                         const fa_grouped_shape* shape, const fa_config* config,
                         const fa_rotary* rotary, int dtype);
 
+/* Causal attention with a sliding window and a few first tokens that stay visible (no counterpart in the
+ * reference): position i sees the keys j <= i with i - j < window (>= 1), and those with j < sinks (0: none).
+ * A window as long as the sequence is plain causal attention. Layouts and arguments as for
+ * fa_forward_gqa_rope; config->causal must be set (else FA_ERR_CAUSAL_VISIBILITY_MISMATCH), head_dim is a
+ * multiple of 8, every tensor starts at a multiple of 16 bytes (FA_ERR_MISALIGNED), and one (batch, head)
+ * slice takes less than 2 GiB. Only the tiles of keys that some row of a block sees are read. LSE has f32
+ * accuracy with 16-bit storage too, except that with rotary the rotated Q and K are rounded to it first, in
+ * the default manner of fa_ctx_set_prefill_precision, whose mode does not apply here. It can be captured
+ * once the context's caches are sized (rotary only). */
+typedef struct fa_window {
+    uint64_t window, sinks;
+} fa_window;
+int fa_forward_gqa_window(fa_ctx* ctx, const void* q, size_t q_bytes, const void* k, const void* v,
+                          size_t kv_bytes, void* out_lse, size_t out_bytes,
+                          const fa_grouped_shape* shape, const fa_config* config,
+                          const fa_window* window, const fa_rotary* rotary, int dtype);
+
 /* Prepared forward: PreparedGroupedForward::prepare src/wgpu_forward_grouped.rs:352 /
  * encode_prepared :496. prepare validates the buffers (Q, K, V, [O|LSE]), shape, config and
  * rotary exactly as fa_forward_gqa_rope does, resolves the kernel variant under the context's
@@ -506,6 +523,15 @@ int fa_backward_grouped(fa_ctx* ctx, const void* q, const void* k, const void* v
                         void* dv, const fa_grouped_shape* shape, const fa_config* config,
                         int dtype);
 
+/* The backward of fa_forward_gqa_window over separate tensors, as fa_backward_grouped (Q and K as they were
+ * multiplied, rotated ones included). The same requirements on causal, head_dim, alignment (LSE: 4 bytes) and
+ * size as the forward. Deterministic: every gradient element has one writer, and partial sums are added in
+ * one order. */
+int fa_backward_gqa_window(fa_ctx* ctx, const void* q, const void* k, const void* v,
+                           const void* d_out, const void* out, const float* lse, void* dq, void* dk,
+                           void* dv, const fa_grouped_shape* shape, const fa_config* config,
+                           const fa_window* window, int dtype);
+
 /* ------------------------------------------------------------ chunked prefill (paged) ---
  * Chunked prefill whose K/V live in the shared page pool: the chunk's queries
  * [batch, query_len, q_heads*head_dim] attend causally (query i at absolute position
@@ -634,6 +660,19 @@ int fa_paged_tree_attention(fa_ctx* ctx, const fa_paged_batch* batch, const void
                             uint64_t head_dim, const fa_config* config, const fa_rotary* rotary,
                             int dtype);
 
+/* Attention of new tokens q [n_seqs, max_tokens, q_heads*head_dim] over the cache with a sliding window: token
+ * t of sequence s, at row i = ctx_lens[s] + t, sees the rows j <= i with i - j < window->window or
+ * j < window->sinks (new_lens[s] rows are appended behind the live ones already; max_tokens 1: a decode step).
+ * Rows that no token sees are not read, and their pages may be gone. Everything else as for
+ * fa_paged_tree_attention without masks, rows past new_lens and lengths that do not fit included. */
+int fa_paged_window_attention(fa_ctx* ctx, const fa_paged_batch* batch, const void* q, size_t q_bytes,
+                              const void* k_pool, const void* v_pool, size_t pool_bytes,
+                              void* out_lse, size_t out_bytes, const int32_t* new_lens,
+                              size_t new_lens_bytes, const int32_t* positions,
+                              size_t positions_bytes, uint64_t max_tokens, uint64_t q_heads,
+                              uint64_t kv_heads, uint64_t head_dim, const fa_config* config,
+                              const fa_window* window, const fa_rotary* rotary, int dtype);
+
 /* Accepted tokens move into place: row ctx_lens[s] + paths[s, i] of K and V to ctx_lens[s] + i for
  * i < accepted[s], and ctx_lens_out[s] = ctx_lens[s] + accepted[s] (ctx_lens_out may be the batch's
  * ctx_lens). paths [n_seqs, max_accept] (max_accept <= 512) holds each accepted path
@@ -646,6 +685,54 @@ int fa_paged_accept(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* pat
                     size_t accepted_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
                     int32_t* ctx_lens_out, size_t ctx_lens_out_bytes, void* k_pool, void* v_pool,
                     size_t pool_bytes, uint64_t kv_heads, uint64_t head_dim, int dtype);
+
+/* ------------------------------------------------------------ 4-bit cache ----------------
+ * The pools of a device-resident batch in 4 bits a value (no counterpart in the reference), 17/64 of the bytes
+ * of 16-bit ones: [physical_pages, page_size] rows of fa_fp4_row_bytes bytes, one token of all kv heads each.
+ * head_dim is a multiple of 32, at most 128. A row holds
+ *   codes   kv_heads*head_dim/2 bytes, value i in byte i / 2, the even one low: sign * 8 + the index of
+ *           0, 0.5, 1, 1.5, 2, 3, 4, 6 (the e2m1 format)
+ *   scales  kv_heads*head_dim/32 bytes, byte g for values 32 g .. 32 g + 31: 2^(byte - 127) (e8m0), 255: NaN
+ *   zeros up to a multiple of 16 bytes.
+ * A value is code * scale. Values outside any of this are not possible: every pattern of bytes is a row. */
+int fa_fp4_row_bytes(uint64_t kv_heads, uint64_t head_dim, uint64_t* out);
+
+/* fa_paged_append_slots into 4-bit pools. K, when rotary is given, is rotated in f32 and not rounded before
+ * this. The scale of 32 values is 2^e with the least e (-127 .. 125) for which all of them are below 7 * 2^e in
+ * magnitude, and each value takes the nearest code, ties to the even one, those past 6 * 2^e the largest. 32
+ * values of which one is infinite or NaN become NaN. */
+int fa_paged_append_slots_fp4(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* slots,
+                              size_t slots_bytes, const int32_t* positions, size_t positions_bytes,
+                              uint64_t max_new, const void* k_src, const void* v_src,
+                              size_t src_bytes, void* k_pool, void* v_pool, size_t pool_bytes,
+                              uint64_t kv_heads, uint64_t head_dim, const fa_rotary* rotary, int dtype);
+
+/* The rows in slots [n_seqs, max_new] of 4-bit pools to k_out, v_out [n_seqs, max_new, kv_heads*head_dim] of
+ * `dtype` (bf16 and f32 hold every value exactly, f16 rounds); zeros for slots outside the pool. */
+int fa_paged_read_slots_fp4(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* slots,
+                            size_t slots_bytes, uint64_t max_new, const void* k_pool,
+                            const void* v_pool, size_t pool_bytes, void* k_out, void* v_out,
+                            size_t out_bytes, uint64_t kv_heads, uint64_t head_dim, int dtype);
+
+/* fa_paged_tree_attention over 4-bit pools, or, with a window (masks must be null then,
+ * FA_ERR_CAUSAL_VISIBILITY_MISMATCH), fa_paged_window_attention. dtype is that of Q and O. Scores and LSE have
+ * f32 accuracy, as the 4-bit values are exact operands; the probabilities are rounded to 16 bits for bf16, and
+ * carry 16 and 24 bits for f16 and f32. A row that sees a key with a NaN among its K or V of that head is NaN
+ * in every dim. */
+int fa_paged_attention_fp4(fa_ctx* ctx, const fa_paged_batch* batch, const void* q, size_t q_bytes,
+                           const void* k_pool, const void* v_pool, size_t pool_bytes, void* out_lse,
+                           size_t out_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                           const int32_t* positions, size_t positions_bytes, const uint64_t* masks,
+                           size_t masks_bytes, uint64_t max_tokens, uint64_t q_heads,
+                           uint64_t kv_heads, uint64_t head_dim, const fa_config* config,
+                           const fa_window* window, const fa_rotary* rotary, int dtype);
+
+/* fa_paged_accept over 4-bit pools. */
+int fa_paged_accept_fp4(fa_ctx* ctx, const fa_paged_batch* batch, const int32_t* paths,
+                        size_t paths_bytes, uint64_t max_accept, const int32_t* accepted,
+                        size_t accepted_bytes, const int32_t* tree_lens, size_t tree_lens_bytes,
+                        int32_t* ctx_lens_out, size_t ctx_lens_out_bytes, void* k_pool, void* v_pool,
+                        size_t pool_bytes, uint64_t kv_heads, uint64_t head_dim);
 
 /* ------------------------------------------------------------ telemetry ------------------
  * runtime_telemetry src/wgpu_backend.rs:374: metadata of the last logical call on `ctx`. */
