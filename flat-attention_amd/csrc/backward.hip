@@ -165,11 +165,6 @@ constexpr int kBwdKeys = 128;     // keys per bwd_dkdv workgroup (32 per wave)
 constexpr int kBwdQueries = 128;  // queries per bwd_dq workgroup (32 per wave)
 constexpr int kBwdTile = 64;      // rows per staged tile (Q/dO in bwd_dkdv, K/V in bwd_dq)
 template <bool WIN> using split_of = std::conditional_t<WIN, WindowSplit, BackwardSplit>;
-// Past the last query that sees a key of key block kb, with a window.
-__device__ __host__ __forceinline__ int window_end(const BackwardArgs& a, int kb) {
-    const int64_t end = (int64_t)(kb + 1) * kBwdKeys - 1 + a.window;
-    return kb * kBwdKeys < a.sinks || end > a.seq ? a.seq : (int)end;
-}
 constexpr uint32_t kOob = 0x7fff0000u;  // transfer offset past every buffer: writes zeros
 
 #define FA_BWD_SG(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
@@ -384,9 +379,12 @@ __global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, split_of<WIN>
     const int k0 = kb * kBwdKeys + wave * 32;
     const int64_t krow0 = (int64_t)bkv * S;
     const int qstart = a.causal ? kb * kBwdKeys : 0;  // a multiple of QT
-    const int qend = WIN ? window_end(a, kb) : S;  // past the last query that sees a key of the block
-    const int nqt = (qend - qstart + QT - 1) / QT, all_tiles = G * nqt;
-    const int tile0 = part * sp.chunk, ntiles = min(all_tiles - tile0, sp.chunk) + tile0;
+    int nqt = (S - qstart + QT - 1) / QT;
+    if constexpr (WIN) nqt = sp.tiles(a, kb);
+    const int all_tiles = G * nqt;
+    int chunk = sp.chunk;
+    if constexpr (WIN) chunk = sp.chunk_of(kb);
+    const int tile0 = part * chunk, ntiles = min(all_tiles - tile0, chunk) + tile0;
     if (WIN && tile0 >= all_tiles) return;
     const int64_t qhead0 = ((int64_t)b * a.q_heads + (int64_t)kvh * G) * S;  // first row of the group
     auto tile_hq = [&](int j) {  // head of the group and query offset qt of tile j
@@ -671,8 +669,10 @@ __global__ __launch_bounds__(256, 1) void bwd_dkdv(BackwardArgs a, split_of<WIN>
         }
     }
     // register r: key k0 + 8 (r / 4) + 4 g + r % 4, dim 32 m + c
-    if (all_tiles > sp.chunk) {  // dK then dV, kBwdKeys rows of D each
-        float* const pp = sp.part + (int64_t)blockIdx.x * 2 * kBwdKeys * D;
+    if (all_tiles > chunk) {  // dK then dV, kBwdKeys rows of D each
+        int64_t slot = blockIdx.x;
+        if constexpr (WIN) slot = (int64_t)sp.slot(kb, part) * nbk + bkv;
+        float* const pp = sp.part + slot * 2 * kBwdKeys * D;
 #pragma unroll
         for (int m = 0; m < MB; ++m) {
             const int d = 32 * m + c;
@@ -711,9 +711,8 @@ __device__ __forceinline__ void add_partials(const BackwardArgs& a, const Window
     using B = Blk<T>;
     const int S = a.seq, D = a.head_dim, units = a.batch * a.kv_heads;
     const int r0 = block % (kBwdKeys / kAddRows) * kAddRows, at = block / (kBwdKeys / kAddRows);
-    const int kb = at / units, bkv = at - kb * units;
-    const int tiles = a.group * ((window_end(a, kb) - kb * kBwdKeys + sp.tile - 1) / sp.tile);
-    const int n = (tiles + sp.chunk - 1) / sp.chunk;
+    const int k = at / units, kb = sp.split_from() + k, bkv = at - k * units;
+    const int n = (a.group * sp.tiles(a, kb) + sp.chunk_of(kb) - 1) / sp.chunk_of(kb);
     if (n < 2) return;  // written by the workgroup that has all of it
     const int64_t step = (int64_t)2 * kBwdKeys * D * units;
     const int count = min(kAddRows, S - kb * kBwdKeys - r0) * D;  // (may be negative: no rows)
@@ -800,9 +799,7 @@ __global__ __launch_bounds__(256, Blk<T>::ES == 2 ? 2 : 1) void bwd_dq(BackwardA
     // WIN: the tiles between the sinks and the first key that the block's first query sees are left out
     int before = 0, skip = 0;
     if constexpr (WIN) {
-        const int low = max(0, qb * kBwdQueries + 1 - a.window) / KT;
-        before = (min(a.sinks, low * KT) + KT - 1) / KT;
-        skip = low - before;
+        skip = WindowSplit::skip(a, qb * kBwdQueries, KT, &before);
     }
     const int ntiles = (kend + KT - 1) / KT - skip;
     auto tile_at = [&](int m) { return WIN && m >= before ? m + skip : m; };
@@ -1277,36 +1274,47 @@ void launch_backward(Dtype dt, const BackwardArgs& a, const BackwardSplit& sp, h
 }
 
 // ------------------------------------------------------------------ sliding windows
-// Key blocks without sinks have about window / 128 + 1 tiles a query head, those with sinks all queries
-// behind them, so the latter are dealt to several workgroups (and both where they leave CUs idle): a chunk
-// is an even share of the tiles for each CU, but no more than a block without sinks has.
+// Key blocks without sinks have about window / 128 + 1 tiles a query head and go to `p` workgroups each, as
+// many as end first by rounds of the chip (a workgroup costs two tiles beside its own, one with partials four);
+// the blocks with sinks, which all queries see, are dealt out in pieces of a quarter of such a workgroup behind
+// them, which fill what the others leave: B1 Hq32 Hkv8 S4096 D128 bf16, window 1024, 4 sinks, has 248 workgroups
+// of up to 36 tiles and 128 tiles for the first block.
 WindowSplit window_split(Dtype dt, const BackwardArgs& a, uint64_t limit) {
     WindowSplit sp{};
-    sp.tile = dt == Dtype::F32 ? 64 : 128;
-    const int nkb = (a.seq + kBwdKeys - 1) / kBwdKeys;
-    sp.sink_blocks = (std::min(a.sinks, a.seq) + kBwdKeys - 1) / kBwdKeys;
-    auto tiles = [&](int kb) {
-        return (int64_t)a.group * ((window_end(a, kb) - kb * kBwdKeys + sp.tile - 1) / sp.tile);
-    };
-    int64_t all = 0;
-    for (int kb = 0; kb < nkb; ++kb) all += tiles(kb);
     const int64_t units = (int64_t)a.batch * a.kv_heads, cus = device_cus();
-    const int64_t most = sp.sink_blocks < nkb ? tiles(sp.sink_blocks) : tiles(0);
-    const int64_t even = std::max<int64_t>((all * units + cus - 1) / cus, 4);
-    sp.blocks = nkb;
-    // (longer chunks where the partials would take more than `limit`: many sinks over a long sequence)
-    for (int64_t chunk = std::min(most, even);; chunk *= 2) {
-        sp.chunk = (int)std::min<int64_t>(chunk, tiles(0));
-        sp.sink_parts = (int)((tiles(0) + sp.chunk - 1) / sp.chunk);
-        sp.parts = sp.sink_blocks < nkb ? (int)((most + sp.chunk - 1) / sp.chunk) : 0;
-        // partials: of the sink blocks, and of the others where these have several parts too
-        sp.bytes = (uint64_t)(sp.parts > 1         ? sp.workgroups()
-                              : sp.sink_parts > 1 ? sp.sink_blocks * sp.sink_parts
-                                                  : 0) *
-                   units * 2 * kBwdKeys * a.head_dim * 4;
-        if (sp.bytes <= limit) break;
+    const bool small = dt == Dtype::F32 && units * ((a.seq + kBwdKeys - 1) / kBwdKeys) < cus;
+    sp.keys = small ? 32 : kBwdKeys;
+    sp.tile = small ? 32 : dt == Dtype::F32 ? 64 : 128;
+    sp.blocks = (a.seq + sp.keys - 1) / sp.keys;
+    sp.sink_blocks = (std::min(a.sinks, a.seq) + sp.keys - 1) / sp.keys;
+    const int plain = sp.blocks - sp.sink_blocks;
+    auto tiles = [&](int kb) { return (int64_t)a.group * sp.tiles(a, kb); };
+    // the f32 kernels without staging: four waves take a workgroup's tiles in turn, two fill a CU at 64 dims
+    const int64_t step = small ? 4 : 1, places = small && a.head_dim <= 64 ? 2 * cus : cus;
+    const int64_t most = plain ? tiles(sp.sink_blocks) : 0, longest = sp.sink_blocks ? tiles(0) : 0;
+    int64_t all = 0;
+    for (int kb = 0; kb < sp.blocks; ++kb) all += tiles(kb);
+    int64_t chunk = std::max<int64_t>(most, 1), best = INT64_MAX;
+    for (int64_t p = 1; p <= 16 && plain; ++p) {
+        const int64_t c = (most + p - 1) / p, rounds = (units * plain * p + places - 1) / places;
+        const int64_t time = std::max(rounds * (c + (p > 1 ? 4 : 2) * step),
+                                      (all * units + places - 1) / places + (p > 1 ? 4 : 2) * step);
+        if (time < best && (p == 1 || c >= step)) {
+            best = time;
+            chunk = c;
+        }
     }
-    return sp;
+    // (larger pieces where the partials would take more than `limit`: many sinks over a long sequence)
+    int64_t piece = plain ? std::max<int64_t>(chunk / 4, 2 * step)
+                          : std::max<int64_t>((all * units + places - 1) / places, 2 * step);
+    for (;; chunk *= 2, piece *= 2) {
+        sp.chunk = (int)std::min(chunk, std::max<int64_t>(most, 1));
+        sp.parts = plain ? (int)((most + sp.chunk - 1) / sp.chunk) : 1;
+        sp.sink_chunk = (int)std::min(piece, std::max<int64_t>(longest, 1));
+        sp.sink_parts = sp.sink_blocks ? (int)((longest + sp.sink_chunk - 1) / sp.sink_chunk) : 1;
+        sp.bytes = (uint64_t)sp.slots() * units * 2 * sp.keys * a.head_dim * 4;
+        if (sp.bytes <= limit) return sp;
+    }
 }
 
 template <typename T, int DPAD>
@@ -1315,8 +1323,7 @@ static void launch_window(const BackwardArgs& a, const WindowSplit& sp, hipStrea
     hipLaunchKernelGGL((bwd_dkdv<T, DPAD, true, false, true>), dim3(sp.workgroups() * units), dim3(256),
                        0, s, a, sp);
     const int n_dq = (a.seq + kBwdQueries - 1) / kBwdQueries * a.batch * a.q_heads;
-    const unsigned split = sp.parts > 1 ? sp.blocks : sp.sink_parts > 1 ? sp.sink_blocks : 0;
-    const unsigned n_add = split * units * (kBwdKeys / kAddRows);
+    const unsigned n_add = sp.split_blocks() * units * (kBwdKeys / kAddRows);
     hipLaunchKernelGGL((bwd_dq<T, DPAD, true, true>), dim3(n_dq + n_add), dim3(256), 0, s, a, sp, n_dq);
 }
 
@@ -1324,6 +1331,10 @@ template <typename T>
 static void launch_window_dims(const BackwardArgs& a, const WindowSplit& sp, hipStream_t s) {
     const int64_t rows = (int64_t)a.batch * a.q_heads * a.seq;
     hipLaunchKernelGGL((bwd_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a, rows);
+    if (sp.keys == 32) {
+        launch_backward_window_f32(a, sp, s);
+        return;
+    }
     if (a.head_dim <= 32) launch_window<T, 32>(a, sp, s);
     else if (a.head_dim <= 64) launch_window<T, 64>(a, sp, s);
     else launch_window<T, 128>(a, sp, s);

@@ -18,9 +18,12 @@
 #include "kernels.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fa {
 namespace {
+
+template <bool WIN> using split_of = std::conditional_t<WIN, WindowSplit, BackwardSplit>;
 
 struct Frag32 {
     float v[16];
@@ -94,9 +97,10 @@ __device__ __forceinline__ void reduce_waves(float* lds, const f32x16_t (&acc)[D
     }
 }
 
-template <int DPAD, bool FULL>
+// WIN (launch_backward_window): position i sees the keys j <= i with i - j < window or j < sinks.
+template <int DPAD, bool FULL, bool WIN = false>
 __global__ __launch_bounds__(256, DPAD == 128 ? 1 : 2) void bwd_f32_dkdv(BackwardArgs a,
-                                                                         BackwardSplit sp) {
+                                                                         split_of<WIN> sp) {
     constexpr int MB = DPAD / 32;
     __shared__ float lds[4 * 32 * DPAD];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c = lane & 31;
@@ -105,9 +109,16 @@ __global__ __launch_bounds__(256, DPAD == 128 ? 1 : 2) void bwd_f32_dkdv(Backwar
     // early key blocks first: under a causal mask they see the most queries
     const int bkv = blockIdx.x % nbk;
     int kb, part;
-    sp.coords(blockIdx.x / nbk, nq, a.group, a.causal, kb, part);
-    const int qb0 = a.causal ? kb : 0, nqv = nq - qb0, items = a.group * nqv;
-    const int first = part * sp.chunk, last = min(items, first + sp.chunk);
+    if constexpr (WIN) sp.coords(blockIdx.x / nbk, kb, part);
+    else sp.coords(blockIdx.x / nbk, nq, a.group, a.causal, kb, part);
+    const int qb0 = a.causal ? kb : 0;
+    int nqv = nq - qb0;
+    if constexpr (WIN) nqv = sp.tiles(a, kb);
+    const int items = a.group * nqv;
+    int chunk = sp.chunk;
+    if constexpr (WIN) chunk = sp.chunk_of(kb);
+    if (WIN && part * chunk >= items) return;
+    const int first = part * chunk, last = min(items, first + chunk);
     const int b = bkv / a.kv_heads, kvh = bkv - b * a.kv_heads;
     const int k0 = kb * 32;
     const int64_t krow0 = (int64_t)bkv * S;
@@ -188,7 +199,12 @@ __global__ __launch_bounds__(256, DPAD == 128 ? 1 : 2) void bwd_f32_dkdv(Backwar
         for (int i = 0; i < 16; ++i) {
             const u32x4_t l = ld[i >> 1];
             float p = fast_exp2(fmaf(s[i], c2, -__uint_as_float(l[2 * (i & 1)])));
-            if (a.causal && t.qb == kb && cc > kidx32(gg, i)) p = 0.0f;
+            if constexpr (WIN) {
+                const int back = t.qb * 32 + kidx32(gg, i) - (k0 + cc);  // from the query to the key
+                if (back < 0 || (back >= a.window && k0 + cc >= a.sinks)) p = 0.0f;
+            } else if (a.causal && t.qb == kb && cc > kidx32(gg, i)) {
+                p = 0.0f;
+            }
             pf.v[i] = p;
             df.v[i] = p * (dp[i] - __uint_as_float(l[2 * (i & 1) + 1]));
         }
@@ -207,8 +223,10 @@ __global__ __launch_bounds__(256, DPAD == 128 ? 1 : 2) void bwd_f32_dkdv(Backwar
         }
     }
     // one chunk: the gradients themselves; else this chunk's partials (dK, then dV)
-    const bool whole = items <= sp.chunk;
-    float* const pp = sp.part + (int64_t)blockIdx.x * 64 * D;
+    const bool whole = items <= chunk;
+    int64_t slot = blockIdx.x;
+    if constexpr (WIN) slot = (int64_t)sp.slot(kb, part) * nbk + bkv;
+    float* const pp = sp.part + slot * 64 * D;
     reduce_waves<DPAD, 4>(lds, dk, D, [&](int r, int d, float x) {
         if (!whole) pp[r * D + d] = x;
         else if (k0 + r < S) ((float*)a.dk)[(krow0 + k0 + r) * D + d] = x * a.scale;
@@ -259,9 +277,28 @@ __device__ __forceinline__ void add_partials(const BackwardArgs& a, const Backwa
     }
 }
 
-template <int DPAD, int NW, bool FULL>
+// The same of a window's key blocks, as those with one chunk are written already.
+__device__ __forceinline__ void add_partials(const BackwardArgs& a, const WindowSplit& sp, int block) {
+    const int S = a.seq, D = a.head_dim, units = a.batch * a.kv_heads;
+    const int which = block & 1, at = block >> 1, k = at / units, kb = sp.split_from() + k, bkv = at - k * units;
+    const int n = (a.group * sp.tiles(a, kb) + sp.chunk_of(kb) - 1) / sp.chunk_of(kb);
+    if (n < 2) return;
+    const int64_t step = (int64_t)64 * D * units;
+    const float* const base = sp.part + sp.slot(kb, 0) * step + (int64_t)bkv * 64 * D + which * 32 * D;
+    const float scale = which ? 1.0f : a.scale;
+    float* out = (float*)(which ? a.dv : a.dk) + ((int64_t)bkv * S + kb * 32) * D;
+    const int count = min(32, S - kb * 32) * D;
+    for (int e = threadIdx.x * 4; e < count; e += blockDim.x * 4) {
+        f32x4_t s = *(const f32x4_t*)(base + e);
+#pragma unroll 8
+        for (int i = 1; i < n; ++i) s += *(const f32x4_t*)(base + i * step + e);
+        *(f32x4_t*)(out + e) = s * scale;
+    }
+}
+
+template <int DPAD, int NW, bool FULL, bool WIN = false>
 __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void bwd_f32_dq(BackwardArgs a,
-                                                                           BackwardSplit sp,
+                                                                           split_of<WIN> sp,
                                                                            int n_dq) {
     constexpr int MB = DPAD / 32;
     __shared__ float lds[NW * 32 * DPAD];
@@ -290,7 +327,10 @@ __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void bwd_f32_dq(Backw
     f32x16_t dq[MB];
 #pragma unroll
     for (int m = 0; m < MB; ++m) dq[m] = (f32x16_t)0.0f;
-    const int nkb = a.causal ? qb + 1 : nq;
+    int before = 0, skip = 0;  // WIN: key blocks that no query of this one sees
+    if constexpr (WIN) skip = WindowSplit::skip(a, q0, 32, &before);
+    auto block_at = [&](int m) { return WIN && m >= before ? m + skip : m; };
+    const int nkb = (a.causal ? qb + 1 : nq) - skip;
     constexpr bool AHEAD = DPAD == 128;  // (as in bwd_f32_dkdv)
     Frag32 kr[MB], vr[MB];
     auto load_rows = [&](int kb) {
@@ -303,8 +343,9 @@ __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void bwd_f32_dq(Backw
             vr[m] = row_frag<FULL>(vt, 32 * m, D, g, c);
         }
     };
-    if (AHEAD && wave < nkb) load_rows(wave);
-    for (int kb = wave; kb < nkb; kb += NW) {
+    if (AHEAD && wave < nkb) load_rows(block_at(wave));
+    for (int m0 = wave; m0 < nkb; m0 += NW) {
+        const int kb = block_at(m0);
         const int keys = min(32, S - kb * 32);
         const Tile kt = tile_of(a.k, krow0 + kb * 32, 4 * D, keys);
         if (!AHEAD) load_rows(kb);
@@ -323,9 +364,10 @@ __global__ __launch_bounds__(64 * NW, DPAD == 128 ? 1 : 2) void bwd_f32_dq(Backw
             const int key = kidx32(g, t);
             float p = fast_exp2(fmaf(s[t], c2, -ld.x));
             if (key >= keys || (a.causal && kb == qb && key > c)) p = 0.0f;
+            if (WIN && q0 + c - (kb * 32 + key) >= a.window && kb * 32 + key >= a.sinks) p = 0.0f;
             df.v[t] = p * (dp[t] - ld.y);
         }
-        if (AHEAD && kb + NW < nkb) load_rows(kb + NW);
+        if (AHEAD && m0 + NW < nkb) load_rows(block_at(m0 + NW));
 #pragma unroll
         for (int m = 0; m < MB; ++m) {
             const Frag32 km = kc;
@@ -356,6 +398,15 @@ template <int DPAD, int NW>
 void launch_d(const BackwardArgs& a, const BackwardSplit& sp, hipStream_t s) {
     if (a.head_dim == DPAD) launch_v<DPAD, NW, true>(a, sp, s);
     else launch_v<DPAD, NW, false>(a, sp, s);
+}
+
+template <int DPAD, int NW, bool FULL>
+void launch_w(const BackwardArgs& a, const WindowSplit& sp, hipStream_t s) {
+    const int nbk = a.batch * a.kv_heads, n_dq = (a.seq + 31) / 32 * a.batch * a.q_heads;
+    hipLaunchKernelGGL((bwd_f32_dkdv<DPAD, FULL, true>), dim3((unsigned)(sp.workgroups() * nbk)), dim3(256),
+                       0, s, a, sp);
+    hipLaunchKernelGGL((bwd_f32_dq<DPAD, NW, FULL, true>),
+                       dim3((unsigned)(n_dq + 2 * sp.split_blocks() * nbk)), dim3(64 * NW), 0, s, a, sp, n_dq);
 }
 
 }  // namespace
@@ -411,6 +462,15 @@ BackwardSplit backward_f32_split(const BackwardArgs& a, uint64_t limit) {
     if (sp.bytes > limit)  // one chunk: no partials
         sp.set_chunk(longest, longest, (int)nq, a.group, a.causal, nbk, 64 * a.head_dim);
     return sp;
+}
+
+void launch_backward_window_f32(const BackwardArgs& a, const WindowSplit& sp, hipStream_t s) {
+    if (a.head_dim == 128) launch_w<128, 4, true>(a, sp, s);
+    else if (a.head_dim > 64) launch_w<128, 4, false>(a, sp, s);
+    else if (a.head_dim == 64) launch_w<64, 8, true>(a, sp, s);
+    else if (a.head_dim > 32) launch_w<64, 8, false>(a, sp, s);
+    else if (a.head_dim == 32) launch_w<32, 8, true>(a, sp, s);
+    else launch_w<32, 8, false>(a, sp, s);
 }
 
 void launch_backward_f32(const BackwardArgs& a, const BackwardSplit& sp, hipStream_t s) {

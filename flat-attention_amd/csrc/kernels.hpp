@@ -273,30 +273,57 @@ void launch_backward(Dtype dt, const BackwardArgs& a, const BackwardSplit& sp, h
                      bool* a64_out = nullptr);
 
 // The same over a sliding window (a.dma, causal; three launches, no dS). The dK/dV launch has workgroups of
-// `chunk` tiles (of `tile` queries of a head): sink_parts for each of the key blocks with sinks, which come
-// first, then `parts` for each of the others; a workgroup's index is the slot of its partials, for the blocks
-// that have several (`part`, of `bytes`; the (batch, kv head) units of an index lie side by side).
+// `chunk` tiles (of `tile` queries of a head) for key blocks of `keys`: `parts` for each block without sinks,
+// then sink_parts, of sink_chunk tiles, for each of the first sink_blocks ones, which all queries behind them
+// see. Partials of the blocks that may have several parts lie in `part` (of `bytes`), those of a workgroup
+// at its index among them, the (batch, kv head) units of an index side by side. tile = keys = 32: the f32
+// kernels without LDS staging.
 struct WindowSplit {
     float* part;
-    int tile, chunk, blocks, sink_blocks, sink_parts, parts;
+    int keys, tile, chunk, parts, sink_chunk, sink_parts, blocks, sink_blocks;
     uint64_t bytes;
-    __host__ __device__ int workgroups() const {
-        return sink_blocks * sink_parts + (blocks - sink_blocks) * parts;
+    __host__ __device__ int plain() const { return (blocks - sink_blocks) * parts; }
+    __host__ __device__ int workgroups() const { return plain() + sink_blocks * sink_parts; }
+    __host__ __device__ int slots() const {
+        return (parts > 1 ? plain() : 0) + (sink_parts > 1 ? sink_blocks * sink_parts : 0);
     }
+    // key blocks that may have several parts: from split_from() on
+    __host__ __device__ int split_from() const { return sink_parts > 1 ? 0 : sink_blocks; }
+    __host__ __device__ int split_blocks() const {
+        return (sink_parts > 1 ? sink_blocks : 0) + (parts > 1 ? blocks - sink_blocks : 0);
+    }
+    __host__ __device__ int chunk_of(int kb) const { return kb < sink_blocks ? sink_chunk : chunk; }
     __host__ __device__ int slot(int kb, int p) const {
-        return kb < sink_blocks ? kb * sink_parts + p
-                                : sink_blocks * sink_parts + (kb - sink_blocks) * parts + p;
+        return kb < sink_blocks ? (parts > 1 ? plain() : 0) + kb * sink_parts + p
+                                : (kb - sink_blocks) * parts + p;
     }
     __device__ void coords(int idx, int& kb, int& p) const {
-        const int first = sink_blocks * sink_parts, n = idx < first ? sink_parts : parts;
-        const int i = idx < first ? idx : idx - first;
-        kb = i / n + (idx < first ? 0 : sink_blocks);
+        const bool sink = idx >= plain();
+        const int i = sink ? idx - plain() : idx, n = sink ? sink_parts : parts;
+        kb = i / n + (sink ? 0 : sink_blocks);
         p = i % n;
+    }
+    // past the last query that sees a key of key block kb
+    __host__ __device__ int end(const BackwardArgs& a, int kb) const {
+        const int64_t e = (int64_t)(kb + 1) * keys - 1 + a.window;
+        return kb * keys < a.sinks || e > a.seq ? a.seq : (int)e;
+    }
+    // tiles of a query head that see it
+    __host__ __device__ int tiles(const BackwardArgs& a, int kb) const {
+        return (end(a, kb) - kb * keys + tile - 1) / tile;
+    }
+    // Of `n` tiles of keys of a block of queries from q0 on: the `skip` behind the first `before`, which hold
+    // the sinks, are not seen by any of them.
+    __device__ static int skip(const BackwardArgs& a, int q0, int kt, int* before) {
+        const int low = max(0, q0 + 1 - a.window) / kt;  // tile of the first key that q0 sees
+        *before = (min(a.sinks, low * kt) + kt - 1) / kt;
+        return low - *before;
     }
 };
 // The split whose partials take at most `limit` bytes, `part` still to be set when bytes > 0.
 WindowSplit window_split(Dtype dt, const BackwardArgs& a, uint64_t limit);
 void launch_backward_window(Dtype dt, const BackwardArgs& a, const WindowSplit& sp, hipStream_t s);
+void launch_backward_window_f32(const BackwardArgs& a, const WindowSplit& sp, hipStream_t s);
 
 // The assembly dK/dV kernel (gen_bwd_a64.py): bf16 or f16, head_dim 128, seq a multiple of 128, dS
 // stored, 16-byte aligned tensors, 32-bit offsets; its module loaded on the current device.
