@@ -167,32 +167,51 @@ void launch_read_fp4(Dtype dt, const SlotAppendArgs& a, hipStream_t s, unsigned 
 // ------------------------------------------------------------------ attention
 // What is seen, and what rows that see nothing get, as in tree.hip. A wave works by itself: 16 NB rows of a
 // (sequence, kv head), flattened as row = t * group + head, over a range of keys. Per 32 keys
-//   S^T[32 keys x 16 rows] = K . Q^T     K's codes from memory into registers, converted there (v_cvt_scalef32_pk_bf16_fp4:
+//   S^T[32 keys x 16 rows] = K . Q^T     K's codes are converted in registers (v_cvt_scalef32_pk_bf16_fp4:
 //                                        every 4-bit value is a bf16 number)
 //   P^T = exp2((S - m) scale log2 e)     two lane exchanges for a row's maximum
-//   O^T[dims x 16 rows]   += V^T . P^T   V converted, through LDS (8 KiB of the wave's own), read transposed
+//   O^T[dims x 16 rows]   += V^T . P^T   V converted, through LDS (4 KiB of the wave's own), read transposed
 // The products are 16x16x32 bf16 MFMAs with exact K and V. Q is carried as bf16 parts of its f32 value (two;
 // f32 storage three), so scores and LSE have f32 accuracy; P as one for bf16, two for f16 and three for f32.
 // Lane (r, j) = (lane & 15, lane >> 4) holds, of key r of a 16-key block, the dims from j DP / 4 on (a 16- or
 // 8-byte piece of the codes, which lies in one group of 32, one scale), and of S^T row r, keys 4 j .. 4 j + 3
 // of each block: the order of the dims and of the keys in a product is free, so Q and V are taken in these.
-// The codes of the next 32 keys, and the table entries of those behind, are on their way meanwhile.
+// Where the head count is a multiple of four, a workgroup's waves take a head each over the same keys and move
+// the rows of the four into LDS together, 16 bytes a lane in the order of the row (global_load_lds), three steps
+// deep with one barrier a step. With another count a wave loads its own codes into registers, two steps deep;
+// its loads then touch 64 bytes of a row each, and their addresses are what bounds it (64 contexts of 512 to 8192
+// tokens, 8 heads of 128, single tokens: 119 us that way, 78 together; with the eight heads in one workgroup a CU,
+// 83). More than 16 rows of up to 64 dims are the exception: what they compute bounds them, and the waves do it
+// better apart (16 contexts of up to 6000 tokens, trees of 24, 8 heads of 64: 48 us apart, 53 together; of 128:
+// 80 and 73).
 constexpr int kFp4Start = 4;  // steps that the start of a unit counts for in the split
 
-template <typename T, int DP, int NB>
+template <typename T, int DP, int NB, int HW>
 struct Fp4Cfg {
     static constexpr bool F32 = std::is_same<T, float>::value;
+    static constexpr bool COOP = HW == 4;
+    static constexpr int NW = 4;                                                       // waves
     static constexpr int NQ = F32 ? 3 : 2;                                            // parts of Q
     static constexpr int NP = F32 ? 3 : std::is_same<T, f16_t>::value ? 2 : 1;  // of P
     static constexpr int KS = DP / 32;                                                 // steps of Q.K^T
     static constexpr int DB = DP / 16;                                                 // 16-dim blocks of O^T
     static constexpr int CB = DP / 8;                // bytes of codes a lane reads of a row
-    static constexpr int CPR = DP / 8;               // 16-byte pieces of a row of V in LDS
-    static constexpr int VB = 32 * DP * 2;           // bytes of a wave's V
+    static constexpr int VB = 32 * 128;              // bytes of a wave's V: 64 dims of 32 keys
+    static constexpr int VP = DP / 64;               // such parts
+    // of them, read before the softmax, as the registers allow
+    static constexpr int VEARLY = VP == 2 && NB == 1 && !F32 ? 2 : VP == 2 && NB == 2 && !F32 && COOP ? 0 : 1;
     static constexpr int QUADS = NB * DB * 64;       // f32 quads of a partial
+    // waves a SIMD, as the registers allow
+    static constexpr int WAVES = NB == 2 && DP == 128 && (F32 || !COOP) ? 1 : 2;
+    // COOP: 16-byte pieces of a row segment in LDS (an odd number: sixteen rows of one column lie in all
+    // banks), which is also the number of transfer instructions of a step (K and V); those of a wave
+    static constexpr int RP = (HW * DP / 2 + HW * DP / 32 + 15) / 16 | 1;
+    static constexpr int NI = (RP + NW - 1) / NW;
+    static constexpr int STAGE = RP * 1024;
+    static constexpr int NST = 3;
+    static constexpr int SMEM = NW * VB + (COOP ? NST * STAGE : 0);
 };
-constexpr int kFp4Waves = 4;    // of a workgroup
-constexpr int kFp4PerCu = 2;    // workgroups
+constexpr int kFp4Pages = 256;  // block-table entries that a wave (COOP: the workgroup) holds in LDS at a time
 
 struct Fp4KArgs {
     TreeArgs a;
@@ -201,12 +220,13 @@ struct Fp4KArgs {
     int row_bytes;
 };
 
-// Which 16-byte column a piece of a V row is kept in: piece ^ fp4_swizzle(row). Sixteen rows of one piece (the
-// stores), and sixteen rows of two pieces (the transposing reads), lie in all columns alike.
-template <int CPR>
-__device__ __forceinline__ int fp4_swizzle(int row) {
-    if constexpr (CPR == 16) return ((row & 3) << 2) | ((row >> 2) & 3);
-    else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+// Which 16-byte column (of 8; two rows share the 16 of all banks) a piece of a V row is kept in: piece ^
+// fp4_swizzle(row), so that the columns hold one piece of sixteen rows (the stores), and two neighbouring
+// pieces of eight rows (half a transposing read), once each.
+__device__ __forceinline__ int fp4_swizzle(int row) { return ((row >> 1) & 3) << 1 | ((row >> 3) & 1); }
+
+__device__ __forceinline__ void fp4_to_lds16(const void* p, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(lds));
 }
 
 // Maximum (sum) over the lanes that hold the same row: lane ^ 16, lane ^ 32.
@@ -274,16 +294,22 @@ __device__ __forceinline__ int fp4_steps(const TreeArgs& a, int rows, int len) {
 }
 
 template <typename T, int DP, int NB, int HW>
-__global__ __launch_bounds__(64 * kFp4Waves, NB == 1 ? 2 : 1) void fp4_split(Fp4KArgs ka) {
-    using C = Fp4Cfg<T, DP, NB>;
+__global__ __launch_bounds__((64 * Fp4Cfg<T, DP, NB, HW>::NW), (Fp4Cfg<T, DP, NB, HW>::WAVES))
+void fp4_split(Fp4KArgs ka) {
+    using C = Fp4Cfg<T, DP, NB, HW>;
     constexpr int KS = C::KS, DB = C::DB, NQ = C::NQ, NP = C::NP;
-    constexpr int KG = kFp4Waves / HW;  // ranges of a workgroup
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kFp4Waves * C::VB];
+    constexpr bool COOP = C::COOP;
+    constexpr int NW = C::NW, KG = NW / HW;  // waves, and ranges, of a workgroup
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[C::SMEM];
+    __shared__ int bt_lds[COOP ? 1 : NW][kFp4Pages];
+    __shared__ int bad_lds[NW];
+    __shared__ uint64_t row_lds[COOP ? NW : 1][32];  // byte offset of each row of the step to come
     const TreeArgs& a = ka.a;
     const int lane = threadIdx.x & 63, r16 = lane & 15, j4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int hd = wave % HW;
     uint8_t* const vlds = smem + wave * C::VB;
+    int* const bt = bt_lds[COOP ? 0 : wave];
     const int D = a.head_dim;
     const int logical = xcd_remap(blockIdx.x, gridDim.x);
     const int wg = __builtin_amdgcn_readfirstlane((int)ka.row_blocks.div((uint32_t)logical));
@@ -335,12 +361,27 @@ __global__ __launch_bounds__(64 * kFp4Waves, NB == 1 ? 2 : 1) void fp4_split(Fp4
 
     // ---- lane constants
     const int d_lane = j4 * (DP / 4);                       // first dim of this lane's piece of a row
-    const bool d_ok = d_lane < D;
+    const bool d_ok = d_lane < D;  // (else: any codes times a Q of zeros, and dims of O that do not exist)
     const int dl = d_ok ? d_lane : 0;
     const int codes = a.kv_heads * D / 2;
     const float c2 = a.scale * kLog2e;
     typedef short v4s __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4s lds_v4s;
+    // COOP: this lane's piece in each of its wave's transfers. Pieces of a step are numbered through the rows
+    // of K, then of V; the last ones of a row may not exist (the last that does is fetched again).
+    const uint32_t stage0 = (uint32_t)(uintptr_t)(lds_void_t*)smem + NW * C::VB;
+    const int n_ins = COOP ? (C::RP - wave + NW - 1) / NW : 0;
+    uint32_t piece_of[COOP ? C::NI : 1];  // row (32 and up: V), codes or scales, and offset
+    if constexpr (COOP) {
+        // pieces of codes; of scales, whose HW D / 32 bytes (16 at most) need not begin with one
+        const int cp = HW * D / 32, sp = 16 % cp == 0 ? 1 : 2;
+#pragma unroll
+        for (int i = 0; i < C::NI; ++i) {
+            const int p = min((wave + i * NW) * 64 + lane, 64 * C::RP - 1);
+            const int r = p / C::RP, c = min(p - r * C::RP, cp + sp - 1);
+            piece_of[i] = (uint32_t)r | (c < cp ? 0u : 64u) | (uint32_t)(c < cp ? 16 * c : 16 * (c - cp)) << 7;
+        }
+    }
 
     while (pos < end) {
         while (pos >= (int64_t)first + units * length_of(rows_s, len)) {
@@ -370,6 +411,8 @@ __global__ __launch_bounds__(64 * kFp4Waves, NB == 1 ? 2 : 1) void fp4_split(Fp4
         bool row_ok[NB];
         uint64_t mask0[NB];
         u32x4_t qop[NB][KS][NQ];
+        int dq = dl;
+        asm volatile("" : "+v"(dq));  // (addresses made of it are not held, or spilled, from unit to unit)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int row = r0 + 16 * nb + r16, rq = min(row, rows_total - 1), t = ka.grp.div(rq);
@@ -383,9 +426,9 @@ __global__ __launch_bounds__(64 * kFp4Waves, NB == 1 ? 2 : 1) void fp4_split(Fp4
                 rope_pos = a.positions ? a.positions[tok[nb]] : ctx + t;
                 row_ok[nb] = row_ok[nb] && rope_pos >= 0 && rope_pos < a.rope_positions;
             }
-            const int64_t q0 = ((int64_t)tok[nb] * a.q_heads + kvh * a.group + rq - t * a.group) * D + dl;
+            const int64_t q0 = ((int64_t)tok[nb] * a.q_heads + kvh * a.group + rq - t * a.group) * D + dq;
             const float2* const cs =
-                a.rope_table + ((int64_t)(row_ok[nb] ? rope_pos : 0) + a.rope_offset) * (D >> 1) + dl / 2;
+                a.rope_table + ((int64_t)(row_ok[nb] ? rope_pos : 0) + a.rope_offset) * (D >> 1) + dq / 2;
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
                 float x[8];
@@ -412,92 +455,186 @@ __global__ __launch_bounds__(64 * kFp4Waves, NB == 1 ? 2 : 1) void fp4_split(Fp4
             for (int db = 0; db < DB; ++db) oacc[nb][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
         const int* const table = a.block_tables + (int64_t)s * a.max_pages;
-        const int head_codes = (kvh * D + dl) / 2, head_scales = codes + (kvh * D + dl) / 32;
+        // (this lane's scale is a byte of an aligned word of its row, which is a multiple of 16 bytes)
+        const int scale_byte = (kvh * D + dl) / 32, scale_at = 8 * (scale_byte & 3);
+        const int head_codes = (kvh * D + dl) / 2, head_scales = codes + (scale_byte & ~3);
 
-        auto real = [&](int step) { return a.window && step >= before ? step + skip : step; };
-        // table entries of the two keys of this lane in a step, -1 outside the pool
-        auto pages_of = [&](int step, int (&page)[2]) {
+        // (with a window, `skip` steps behind the first `before` are left out: a part of the loop ends there)
+        for (int at0 = st0; at0 < st1;) {
+        const int shift = at0 >= before ? skip : 0, c0 = at0 + shift;
+        const int part = at0 < before && skip > 0 ? min(st1, before) : st1 + shift;
+        // ---- table entries of as many steps as they cover: first pool row of each page, -1 outside the pool
+        const int p0 = ka.ps.div(c0 * 32);
+        const int64_t reach = ((int64_t)p0 + kFp4Pages) * a.page_size;  // keys below are covered
+        const int c1 = (int)min((int64_t)part, max((int64_t)c0 + 1, reach / 32));
+        const int k_end = min(c1 * 32, rows_s);
+        const int n_pages = ka.ps.div(k_end - 1) - p0 + 1;
+        bool bad = false;
+        if constexpr (COOP) __syncthreads();  // (the entries and stages before have been read)
+        for (int i = COOP ? (int)threadIdx.x : lane; i < n_pages; i += COOP ? 64 * NW : 64) {
+            const int page = table[p0 + i];
+            const bool in = (unsigned)page < (unsigned)a.physical_pages;
+            bt[i] = in ? page * a.page_size : -1;
+            bad |= !in;
+        }
+        bad = __any(bad);
+        if constexpr (COOP) {
+            if (lane == 0) bad_lds[wave] = bad;
+            __syncthreads();
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int key = min(real(step) * 32 + 16 * b + r16, rows_s - 1);
-                page[b] = table[ka.ps.div(key)];
-            }
-        };
-        // their codes and scales (those of row 0 of the pool for a page outside it)
+            for (int w = 0; w < NW; ++w) bad |= bad_lds[w] != 0;
+            bad = __builtin_amdgcn_readfirstlane(bad);
+        }
+        // codes and scales of this lane's two keys of a step (those of row 0 for a page outside the pool)
         typedef uint32_t piece_t __attribute__((ext_vector_type(C::CB / 4)));
         struct Tile {
             piece_t k[2], v[2];
-            uint32_t ks[2], vs[2];
-            uint32_t there;  // bit i: key i of the 32 is there
+            uint32_t ks[2], vs[2];  // the word that holds the scale (COOP: the scale)
         };
-        auto load_tile = [&](int step, const int (&page)[2], Tile& t) {
-            t.there = 0;
+        auto load_tile = [&](int step, Tile& t) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const int key_raw = real(step) * 32 + 16 * b + r16, key = min(key_raw, rows_s - 1);
+                const int key = min(step * 32 + 16 * b + r16, k_end - 1);
                 const int lp = ka.ps.div(key);
-                const bool in = (unsigned)page[b] < (unsigned)a.physical_pages;
-                const int64_t row = in ? (int64_t)page[b] * a.page_size + key - lp * a.page_size : 0;
-                const uint8_t* const kp = (const uint8_t*)a.k_pool + row * ka.row_bytes;
-                const uint8_t* const vp = (const uint8_t*)a.v_pool + row * ka.row_bytes;
-                t.k[b] = __builtin_nontemporal_load((const piece_t*)(kp + head_codes));
-                t.v[b] = __builtin_nontemporal_load((const piece_t*)(vp + head_codes));
-                t.ks[b] = kp[head_scales];
-                t.vs[b] = vp[head_scales];
-                t.there |= ((uint32_t)__ballot(in && key_raw < rows_s) & 0xffffu) << (16 * b);
+                const uint64_t row = (uint64_t)(uint32_t)(max(bt[lp - p0], 0) + key - lp * a.page_size) *
+                                     (uint32_t)ka.row_bytes;
+                const uint8_t* const kp = (const uint8_t*)a.k_pool + row;
+                const uint8_t* const vp = (const uint8_t*)a.v_pool + row;
+                t.k[b] = *(const piece_t*)(kp + head_codes);
+                t.v[b] = *(const piece_t*)(vp + head_codes);
+                t.ks[b] = *(const uint32_t*)(kp + head_scales);
+                t.vs[b] = *(const uint32_t*)(vp + head_scales);
+            }
+        };
+        auto scale_of = [&](uint32_t w) { return COOP ? w : (w >> scale_at) & 255u; };
+
+        // COOP: a step's rows on their way into a stage
+        auto transfer = [&](int step, int stage) {
+            if (lane < 32) {
+                const int key = min(step * 32 + lane, k_end - 1), lp = ka.ps.div(key);
+                row_lds[wave][lane] = (uint64_t)(uint32_t)(max(bt[lp - p0], 0) + key - lp * a.page_size) *
+                                      (uint32_t)ka.row_bytes;
+            }
+            const uint32_t seg_codes = unit * (HW * D / 2), seg_scales = codes + (unit * (HW * D / 32) & ~15);
+#pragma unroll
+            for (int i = 0; i < C::NI; ++i) {
+                if (i >= n_ins) break;
+                const uint32_t pc = piece_of[i];
+                // (of two pieces of scales the second may lie past the row, and is not needed then)
+                const uint32_t at = pc & 64 ? min(seg_scales + (pc >> 7), (uint32_t)ka.row_bytes - 16u)
+                                            : seg_codes + (pc >> 7);
+                const uint8_t* const p =
+                    (const uint8_t*)(pc & 32 ? a.v_pool : a.k_pool) + (row_lds[wave][pc & 31] + at);
+                fp4_to_lds16(p, stage0 + stage * C::STAGE + (wave + i * NW) * 1024);
+            }
+        };
+        // a step's codes from its stage
+        auto fetch = [&](int stage, Tile& t) {
+            const uint8_t* const at = smem + NW * C::VB + stage * C::STAGE;
+            const int cd = hd * D / 2 + dl / 2;
+            const int sb = HW * D / 2 + (unit * (HW * D / 32) & 15) + (hd * D + dl) / 32;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const uint8_t* const k = at + (16 * b + r16) * (C::RP * 16);
+                t.k[b] = *(const piece_t*)(k + cd);
+                t.ks[b] = k[sb];
+                const uint8_t* const v = k + 32 * C::RP * 16;
+                t.v[b] = *(const piece_t*)(v + cd);
+                t.vs[b] = v[sb];
             }
         };
 
-        int page[2];
-        Tile next;
-        pages_of(st0, page);
-        load_tile(st0, page, next);
-        if (st0 + 1 < st1) pages_of(st0 + 1, page);
-#pragma unroll 1
-        for (int step = st0; step < st1; ++step) {
-            const Tile cur = next;
-            if (step + 1 < st1) {
-                load_tile(step + 1, page, next);
-                if (step + 2 < st1) pages_of(step + 2, page);
-            }
-            const int rs = real(step), key0 = rs * 32;
-            // ---- V into LDS: row 16 b + r16, dims d_lane ..; without NaN (the score has it then)
-            uint32_t v_nan = 0;
+        // One step. Not COOP: its codes are used up before the softmax, and those of the step after the next
+        // take their place. (Near the end the last step's again: a branch here would have every load waited for.)
+        const auto process = [&](Tile& cur, int step) {
+            const int key0 = step * 32;
+            // ---- V into LDS, without NaN (the score has it then), 64 dims at a time: of part t the dims
+            // d_lane + 16 t .. of row 16 b + r16 in pieces 2 j4, 2 j4 + 1
+            bool nan[2];
+            float vsc[2];
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const bool nan = cur.vs[b] == 255u && d_ok;
-                const uint64_t any = __ballot(nan);
-                v_nan |= (uint32_t)((any | any >> 16 | any >> 32 | any >> 48) & 0xffffu) << (16 * b);
-                const float sc = __uint_as_float(nan ? 0u : cur.vs[b] << 23);
-                const int row = 16 * b + r16;
-#pragma unroll
-                for (int c = 0; c < C::CB / 4; ++c) {
-                    const uint32_t w = nan || !d_ok ? 0u : cur.v[b][c];
-                    const int piece = d_lane / 8 + c;
-                    *(u32x4_t*)(vlds + row * (2 * DP) + ((piece ^ fp4_swizzle<C::CPR>(row)) << 4)) =
-                        fp4_eight(w, sc);
-                }
+                const uint32_t e = scale_of(cur.vs[b]);
+                nan[b] = e == 255u && d_ok;
+                vsc[b] = __uint_as_float(e == 255u ? 0u : e << 23);
             }
-            // ---- K operands
-            u32x4_t kop[2][KS];
+            const bool any_nan = __any(nan[0] || nan[1]);
+            piece_t vc[2] = {cur.v[0], cur.v[1]};
+            auto write_v = [&](int t) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const float sc = __uint_as_float(cur.ks[b] << 23);
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int c = 0; c < KS; ++c) kop[b][c] = fp4_eight(d_ok ? cur.k[b][c] : 0u, d_ok ? sc : 1.0f);
-            }
-            const bool masked = rs < open0 || rs >= open1 || cur.there != 0xffffffffu || v_nan;
-            u32x4_t pop[NB][NP];
+                    for (int c = 0; c < 2; ++c) {
+                        const int row = 16 * b + r16;
+                        *(u32x4_t*)(vlds + row * 128 + (((2 * j4 + c) ^ fp4_swizzle(row)) << 4)) =
+                            fp4_eight(vc[b][2 * t + c], vsc[b]);
+                    }
+            };
+            // and back transposed: dims 16 g + r16 of it (of O: block VP g + t) of the keys 4 j4 .. and 16 + 4 j4 ..
+            u32x4_t vop[4 * (C::VEARLY ? C::VEARLY : 1)];
+            auto read_v = [&](int to) {
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                f32x4_t sc[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+                for (int g = 0; g < 4; ++g)
 #pragma unroll
-                for (int c = 0; c < KS; ++c)
+                    for (int b = 0; b < 2; ++b) {
+                        const int row = 16 * b + 4 * j4 + (r16 >> 2), piece = 2 * g + ((r16 & 3) >> 1);
+                        const uint8_t* const src =
+                            vlds + row * 128 + ((piece ^ fp4_swizzle(row)) << 4) + 8 * (r16 & 1);
+                        const u32x2_t x = __builtin_bit_cast(
+                            u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)src));
+                        vop[4 * to + g][2 * b] = x[0];
+                        vop[4 * to + g][2 * b + 1] = x[1];
+                    }
+            };
+            if constexpr (C::VEARLY > 0) write_v(0);
+            // ---- scores; K's operands are converted as they are multiplied
+            float ksc[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) ksc[b] = __uint_as_float(d_ok ? scale_of(cur.ks[b]) << 23 : 0x3f800000u);
+            f32x4_t sall[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) sall[nb][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KS; ++c) {
+                u32x4_t kop[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    kop[b] = fp4_eight(cur.k[b][c], ksc[b]);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int n = 0; n < NQ; ++n)
 #pragma unroll
                         for (int b = 0; b < 2; ++b)
-                            sc[b] = Half<bf16_t>::mfma16(kop[b][c], qop[nb][c][n], sc[b]);
+                            sall[nb][b] = Half<bf16_t>::mfma16(kop[b], qop[nb][c][n], sall[nb][b]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!COOP) load_tile(min(step + 2, c1 - 1), cur);
+            // V's operands are on their way while the softmax runs
+            if constexpr (C::VEARLY > 0) read_v(0);
+            if constexpr (C::VEARLY == 2) {
+                write_v(1);
+                read_v(1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const bool masked = step < open0 || step >= open1 || bad || any_nan;
+            // keys that are there, and those whose V has a NaN (masked steps only)
+            uint32_t there = 0, v_nan = 0;
+            if (masked) {
+                const int key_raw = key0 + (lane & 31), key = min(key_raw, k_end - 1);
+                there = (uint32_t)__ballot(bt[ka.ps.div(key) - p0] >= 0 && key_raw < k_end);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint64_t any = __ballot(nan[b]);
+                    v_nan |= (uint32_t)((any | any >> 16 | any >> 32 | any >> 48) & 0xffffu) << (16 * b);
+                }
+            }
+            u32x4_t pop[NB][NP];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                f32x4_t (&sc)[2] = sall[nb];
                 wait_mfma(sc[0]);
                 wait_mfma(sc[1]);
                 if (masked) {
@@ -505,12 +642,12 @@ __global__ __launch_bounds__(64 * kFp4Waves, NB == 1 ? 2 : 1) void fp4_split(Fp4
                     if (a.window) w = window_word(a, ctx + t_of[nb], key0);
                     else if (a.masks) w = mask_word(a, row_ok[nb], tok[nb], mask0[nb], key0 - ctx);
                     else w = causal_word(ctx + t_of[nb], key0);
-                    const uint32_t see = (w & cur.there) >> (4 * j4), bad = v_nan >> (4 * j4);
+                    const uint32_t see = (w & there) >> (4 * j4), odd = v_nan >> (4 * j4);
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            if ((bad >> (16 * b + i)) & 1) sc[b][i] = __uint_as_float(0x7fc00000u);
+                            if ((odd >> (16 * b + i)) & 1) sc[b][i] = __uint_as_float(0x7fc00000u);
                             if (!((see >> (16 * b + i)) & 1)) sc[b][i] = -INFINITY;
                         }
                 }
@@ -536,29 +673,61 @@ __global__ __launch_bounds__(64 * kFp4Waves, NB == 1 ? 2 : 1) void fp4_split(Fp4
                 }
                 bf16_parts<NP>(p, pop[nb]);
             }
-            // ---- O^T += V^T . P^T: dims 16 db + r16 of the keys 4 j4 .. and 16 + 4 j4 ..
+            // ---- O^T += V^T . P^T
 #pragma unroll
-            for (int db = 0; db < DB; ++db) {
-                u32x4_t vop;
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int row = 16 * b + 4 * j4 + (r16 >> 2), piece = 2 * db + ((r16 & 3) >> 1);
-                    const uint8_t* const src = vlds + row * (2 * DP) +
-                                               ((piece ^ fp4_swizzle<C::CPR>(row)) << 4) + 8 * (r16 & 1);
-                    const u32x2_t x = __builtin_bit_cast(
-                        u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)src));
-                    vop[2 * b] = x[0];
-                    vop[2 * b + 1] = x[1];
+            for (int t = 0; t < C::VP; ++t) {
+                if (t >= C::VEARLY) {
+                    write_v(t);
+                    read_v(0);
                 }
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
+                for (int g = 0; g < 4; ++g)
 #pragma unroll
-                    for (int n = 0; n < NP; ++n)
-                        oacc[nb][db] = Half<bf16_t>::mfma16(vop, pop[nb][n], oacc[nb][db]);
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int n = 0; n < NP; ++n)
+                            oacc[nb][C::VP * g + t] = Half<bf16_t>::mfma16(
+                                vop[4 * (t < C::VEARLY ? t : 0) + g], pop[nb][n], oacc[nb][C::VP * g + t]);
             }
+        };
+        if constexpr (COOP) {
+            static_assert(C::NST == 3, "two steps ahead");
+            transfer(c0, 0);
+            if (c0 + 1 < c1) transfer(c0 + 1, 1);
+            int stage = 0;
+#pragma unroll 1
+            for (int step = c0; step < c1; ++step) {
+                // (transfers complete in order: those of the next step may be on their way)
+                if (step + 1 < c1) {
+                    if (n_ins == C::NI) wait_vmcnt<C::NI>();
+                    else wait_vmcnt<C::NI - 1>();
+                } else {
+                    wait_dma();
+                }
+                __syncthreads();
+                const int ahead = stage == 0 ? 2 : stage - 1;
+                if (step + 2 < c1) transfer(step + 2, ahead);
+                Tile t;
+                fetch(stage, t);
+                process(t, step);
+                stage = stage == 2 ? 0 : stage + 1;
+            }
+        } else {
+        Tile even, odd;
+        load_tile(c0, even);
+        load_tile(min(c0 + 1, c1 - 1), odd);
+#pragma unroll 1
+        for (int step = c0; step < c1; step += 2) {
+            process(even, step);
+            if (step + 1 < c1) process(odd, step + 1);
+        }
+        }
+        at0 = c1 - shift;
         }
 
         // ---- finished rows to O and LSE, partial ones to their slot
+        int ln = lane;
+        asm volatile("" : "+v"(ln));  // (as dq)
         const bool whole = st0 == 0 && st1 == steps;
         const int64_t slot =
             ((2 * ((int64_t)range * ka.row_blocks.d + rb) + (st0 == 0 ? 1 : 0)) * HW + hd);
@@ -566,19 +735,19 @@ __global__ __launch_bounds__(64 * kFp4Waves, NB == 1 ? 2 : 1) void fp4_split(Fp4
         for (int nb = 0; nb < NB; ++nb) {
             float l = sum_rows(l_run[nb]);
             if (!row_ok[nb]) l = 0.0f;
-            const int row = r0 + 16 * nb + r16;
+            const int row = r0 + 16 * nb + (ln & 15);
             if (whole) {
                 if (row < rows_total)
 #pragma unroll
                     for (int db = 0; db < DB; ++db) {
-                        const int d = 16 * db + 4 * j4;
+                        const int d = 16 * db + 4 * (ln >> 4);
                         if (d < D) fp4_write<T>(a, s, kvh, row, d, oacc[nb][db], m_run[nb], l, ka.grp);
                     }
-            } else {
-                f32x4_t* const out = (f32x4_t*)a.part_o + slot * C::QUADS + nb * DB * 64 + lane;
+            } else if (row < rows_total) {  // (few rows: the others are a good part of the traffic)
+                f32x4_t* const out = (f32x4_t*)a.part_o + slot * C::QUADS + nb * DB * 64 + ln;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) out[db * 64] = oacc[nb][db];
-                if (j4 == 0) a.part_ml[slot * 16 * NB + 16 * nb + r16] = make_float2(m_run[nb], l);
+                if (j4 == 0) a.part_ml[slot * 16 * NB + 16 * nb + (ln & 15)] = make_float2(m_run[nb], l);
             }
         }
     }
@@ -608,6 +777,7 @@ __global__ __launch_bounds__(256) void fp4_combine(Fp4KArgs ka, int hw, int nb_r
     const uint32_t u0 = (uint32_t)a.plan[s] + (uint32_t)(kvh / hw) * (uint32_t)(steps + ov) + (uint32_t)ov;
     const int g0 = (int)(u0 / (uint32_t)share), g1 = (int)((u0 + steps - 1) / (uint32_t)share);
     if (g0 == g1) return;  // finished by the range that covers it
+    if (row >= len * a.group) return;
     const int rb = b16 / nb_rows, in = b16 - rb * nb_rows, nrb = (int)ka.row_blocks.d;
     const float c2 = a.scale * kLog2e;
     float M = -INFINITY, L = 0.0f;
@@ -635,46 +805,61 @@ __global__ __launch_bounds__(256) void fp4_combine(Fp4KArgs ka, int hw, int nb_r
             for (int e = 0; e < 4; ++e) o[e] = fmaf(x[i][e], w1, o[e] * w0);
         }
     }
-    if (row < len * a.group && d < D) fp4_write<T>(a, s, kvh, row, d, o, M, L, ka.grp);
+    if (d < D) fp4_write<T>(a, s, kvh, row, d, o, M, L, ka.grp);
 }
 
 struct Fp4Shape {
-    int nb, hw, row_blocks, ranges, workgroups;
+    int nb, hw, nw, row_blocks, ranges, workgroups;
 };
-static Fp4Shape fp4_shape(const TreeArgs& a) {
-    Fp4Shape s;
-    const int rows = a.max_tokens * a.group;
-    s.nb = rows <= 16 ? 1 : 2;
-    s.hw = a.kv_heads % 4 == 0 ? 4 : a.kv_heads % 2 == 0 ? 2 : 1;
-    s.row_blocks = (rows + 16 * s.nb - 1) / (16 * s.nb);
-    const int wgs = std::max(1, kFp4PerCu * device_cus() / s.row_blocks);
-    s.ranges = wgs * (kFp4Waves / s.hw);
-    s.workgroups = wgs * s.row_blocks;
-    return s;
+// Calls f with the 16-row blocks a wave and the heads of a launch as constants.
+template <typename T, int DP, typename F>
+static auto fp4_dispatch(const TreeArgs& a, F f) {
+    using std::integral_constant;
+    auto heads = [&](auto nb) {
+        if constexpr (DP == 128 || decltype(nb)::value == 1)
+            if (a.kv_heads % 4 == 0) return f(nb, integral_constant<int, 4>{});
+        if (a.kv_heads % 2 == 0) return f(nb, integral_constant<int, 2>{});
+        return f(nb, integral_constant<int, 1>{});
+    };
+    return a.max_tokens * a.group <= 16 ? heads(integral_constant<int, 1>{}) : heads(integral_constant<int, 2>{});
+}
+template <typename T, int DP>
+static Fp4Shape fp4_shape_t(const TreeArgs& a) {
+    return fp4_dispatch<T, DP>(a, [&](auto nb, auto hw) {
+        using C = Fp4Cfg<T, DP, decltype(nb)::value, decltype(hw)::value>;
+        Fp4Shape s;
+        s.nb = decltype(nb)::value;
+        s.hw = decltype(hw)::value;
+        s.nw = C::NW;
+        s.row_blocks = (a.max_tokens * a.group + 16 * s.nb - 1) / (16 * s.nb);
+        // one round of workgroups
+        const int wgs = std::max(1, C::WAVES * 4 / C::NW * device_cus() / s.row_blocks);
+        s.ranges = wgs * (C::NW / s.hw);
+        s.workgroups = wgs * s.row_blocks;
+        return s;
+    });
+}
+static Fp4Shape fp4_shape(Dtype dt, const TreeArgs& a) {
+    if (a.head_dim <= 64) return dt == Dtype::F32 ? fp4_shape_t<float, 64>(a) : fp4_shape_t<bf16_t, 64>(a);
+    return dt == Dtype::F32 ? fp4_shape_t<float, 128>(a) : fp4_shape_t<bf16_t, 128>(a);
 }
 
-// (one size for every shape, as tree_workspace: two partials a wave of at most 32 rows of 128 dims)
-size_t fp4_workspace(Dtype, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset) {
-    const size_t waves = std::max<size_t>((size_t)kFp4PerCu * device_cus(), fp4_shape(a).workgroups) * kFp4Waves;
-    *ml_offset = waves * 2 * 32 * 128 * 4;
-    *plan_offset = *ml_offset + waves * 2 * 32 * 8;
+// (one size for every shape, as tree_workspace: two partials a wave, at most 64 rows of 128 dims of them on a
+// CU; a single range, which more row blocks than workgroups have, leaves some with fewer than four heads)
+size_t fp4_workspace(Dtype dt, const TreeArgs& a, size_t* ml_offset, size_t* plan_offset) {
+    const size_t rows = std::max<size_t>((size_t)device_cus() * 2, (size_t)fp4_shape(dt, a).row_blocks * 2) *
+                        32 * 4 * 2;
+    *ml_offset = rows * 128 * 4;
+    *plan_offset = *ml_offset + rows * 8;
     return *plan_offset + ((size_t)a.n_seqs + 2) * 4;
 }
 
 template <typename T, int DP>
 static void fp4_launch(Fp4KArgs& ka, const Fp4Shape& sh, hipStream_t st, void (*between)(void*), void* user) {
     const TreeArgs& a = ka.a;
-    auto split = [&](auto nb, auto hw) {
-        fp4_split<T, DP, decltype(nb)::value, decltype(hw)::value>
-            <<<sh.workgroups, 64 * kFp4Waves, 0, st>>>(ka);
-    };
-    auto heads = [&](auto nb) {
-        if (sh.hw == 4) split(nb, std::integral_constant<int, 4>{});
-        else if (sh.hw == 2) split(nb, std::integral_constant<int, 2>{});
-        else split(nb, std::integral_constant<int, 1>{});
-    };
-    if (sh.nb == 1) heads(std::integral_constant<int, 1>{});
-    else heads(std::integral_constant<int, 2>{});
+    fp4_dispatch<T, DP>(a, [&](auto nb, auto hw) {
+        fp4_split<T, DP, decltype(nb)::value, decltype(hw)::value><<<sh.workgroups, 64 * sh.nw, 0, st>>>(ka);
+    });
     if (between) between(user);
     const int blocks = (a.max_tokens * a.group + 15) / 16;
     const unsigned g = (unsigned)((int64_t)a.n_seqs * a.kv_heads * blocks * (DP / 64));
@@ -683,7 +868,7 @@ static void fp4_launch(Fp4KArgs& ka, const Fp4Shape& sh, hipStream_t st, void (*
 
 void launch_fp4_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned grid[3],
                           unsigned* block, unsigned* rows, void (*between)(void*), void* user) {
-    const Fp4Shape sh = fp4_shape(a);
+    const Fp4Shape sh = fp4_shape(dt, a);
     Fp4KArgs ka;
     ka.a = a;
     ka.ps = SmallDiv((uint32_t)a.page_size);
@@ -693,7 +878,7 @@ void launch_fp4_attention(Dtype dt, const TreeArgs& a, hipStream_t s, unsigned g
     ka.row_bytes = fp4_row_bytes(a.kv_heads, a.head_dim);
     grid[0] = (unsigned)sh.workgroups;
     grid[1] = grid[2] = 1;
-    *block = 64 * kFp4Waves;
+    *block = (unsigned)(64 * sh.nw);
     *rows = (unsigned)(16 * sh.nb);
     auto go = [&](auto tag) {
         using T = decltype(tag);

@@ -235,6 +235,11 @@ SHAPES = [  # context lengths, tree lengths, most, q heads, kv heads, head dim, 
     ([40], [512], 512, 2, 2, 32, 16),
     ([2500, 11], [4, 4], 4, 12, 12, 96, 64),
     ([300, 150, 1], [3, 2, 3], 3, 40, 1, 64, 8),
+    ([260, 70], [3, 2], 3, 16, 8, 64, 16),
+    ([515, 9], [5, 20], 20, 8, 8, 96, 24),
+    ([1030, 31], [1, 1], 1, 12, 12, 32, 16),
+    ([90, 333], [1, 1], 1, 16, 4, 96, 16),
+    ([600, 5], [33, 7], 33, 8, 8, 128, 32),
 ]
 
 
