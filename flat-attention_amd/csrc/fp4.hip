@@ -201,6 +201,8 @@ struct Fp4Cfg {
     // of them, read before the softmax, as the registers allow
     static constexpr int VEARLY = VP == 2 && NB == 1 && !F32 ? 2 : VP == 2 && NB == 2 && !F32 && COOP ? 0 : 1;
     static constexpr int QUADS = NB * DB * 64;       // f32 quads of a partial
+    // the rows are loaded while the first keys are on their way, as the registers allow
+    static constexpr bool LATE = F32 || NB == 1 || DP == 64;
     // waves a SIMD, as the registers allow
     static constexpr int WAVES = NB == 2 && DP == 128 && (F32 || !COOP) ? 1 : 2;
     // COOP: 16-byte pieces of a row segment in LDS (an odd number: sixteen rows of one column lie in all
@@ -318,11 +320,18 @@ void fp4_split(Fp4KArgs ka) {
     const int units = a.kv_heads / HW;  // of a sequence
 
     // ---- this wave's range of steps [pos, end), and the sequence that holds the first (as in tree.hip)
-    auto rows_of = [&](int i) { return i < a.n_seqs ? tree_rows_of(a, i) : 0; };
-    auto len_of = [&](int i) { return a.tree_lens[min(i, a.n_seqs - 1)]; };
-    int mine = 0, count = 0;
+    auto rows_of = [&](int i, int& len) {
+        const int at = min(i, a.n_seqs - 1);
+        len = a.tree_lens[at];
+        const int rows = tree_rows_of(a, at);
+        return i < a.n_seqs ? rows : 0;
+    };
+    int mine = 0, count = 0, len0;
+    const int rows0 = rows_of(lane, len0);  // (of the first 64 sequences: not asked for again)
     for (int i = lane; i < a.n_seqs; i += 64) {
-        const int rows = rows_of(i), n = rows ? fp4_steps(a, rows, len_of(i)) : 0;
+        int rows = rows0, ln = len0;
+        if (i != lane) rows = rows_of(i, ln);
+        const int n = rows ? fp4_steps(a, rows, ln) : 0;
         mine += units * n;
         count += n ? units : 0;
     }
@@ -342,7 +351,9 @@ void fp4_split(Fp4KArgs ka) {
     int s = 0, first = 0, rows_s = 0, len = 0;
     bool found = pos >= end;
     for (int base = 0, carry = 0; base < a.n_seqs && (plans || !found); base += 64) {
-        const int rows = rows_of(base + lane), ln = len_of(base + lane), v = units * length_of(rows, ln);
+        int rows = rows0, ln = len0;
+        if (base) rows = rows_of(base + lane, ln);
+        const int v = units * length_of(rows, ln);
         const int upto = carry + wave_scan(v);
         if (plans && base + lane < a.n_seqs) a.plan[base + lane] = upto - v;
         const uint64_t past = __ballot(upto > pos);
@@ -367,21 +378,8 @@ void fp4_split(Fp4KArgs ka) {
     const float c2 = a.scale * kLog2e;
     typedef short v4s __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4s lds_v4s;
-    // COOP: this lane's piece in each of its wave's transfers. Pieces of a step are numbered through the rows
-    // of K, then of V; the last ones of a row may not exist (the last that does is fetched again).
     const uint32_t stage0 = (uint32_t)(uintptr_t)(lds_void_t*)smem + NW * C::VB;
     const int n_ins = COOP ? (C::RP - wave + NW - 1) / NW : 0;
-    uint32_t piece_of[COOP ? C::NI : 1];  // row (32 and up: V), codes or scales, and offset
-    if constexpr (COOP) {
-        // pieces of codes; of scales, whose HW D / 32 bytes (16 at most) need not begin with one
-        const int cp = HW * D / 32, sp = 16 % cp == 0 ? 1 : 2;
-#pragma unroll
-        for (int i = 0; i < C::NI; ++i) {
-            const int p = min((wave + i * NW) * 64 + lane, 64 * C::RP - 1);
-            const int r = p / C::RP, c = min(p - r * C::RP, cp + sp - 1);
-            piece_of[i] = (uint32_t)r | (c < cp ? 0u : 64u) | (uint32_t)(c < cp ? 16 * c : 16 * (c - cp)) << 7;
-        }
-    }
 
     while (pos < end) {
         while (pos >= (int64_t)first + units * length_of(rows_s, len)) {
@@ -411,40 +409,43 @@ void fp4_split(Fp4KArgs ka) {
         bool row_ok[NB];
         uint64_t mask0[NB];
         u32x4_t qop[NB][KS][NQ];
-        int dq = dl;
-        asm volatile("" : "+v"(dq));  // (addresses made of it are not held, or spilled, from unit to unit)
+        auto load_rows = [&] {
+            int dq = dl;
+            asm volatile("" : "+v"(dq));  // (addresses made of it are not held, or spilled, from unit to unit)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const int row = r0 + 16 * nb + r16, rq = min(row, rows_total - 1), t = ka.grp.div(rq);
-            row_ok[nb] = row < rows_total;
-            t_of[nb] = t;
-            tok[nb] = s * a.max_tokens + t;
-            mask0[nb] = 0;
-            if (row_ok[nb] && a.masks && a.words == 1) mask0[nb] = a.masks[tok[nb]];
-            int rope_pos = 0;
-            if (a.rope_table) {
-                rope_pos = a.positions ? a.positions[tok[nb]] : ctx + t;
-                row_ok[nb] = row_ok[nb] && rope_pos >= 0 && rope_pos < a.rope_positions;
-            }
-            const int64_t q0 = ((int64_t)tok[nb] * a.q_heads + kvh * a.group + rq - t * a.group) * D + dq;
-            const float2* const cs =
-                a.rope_table + ((int64_t)(row_ok[nb] ? rope_pos : 0) + a.rope_offset) * (D >> 1) + dq / 2;
-#pragma unroll
-            for (int c = 0; c < KS; ++c) {
-                float x[8];
-                if constexpr (C::F32) load8<T>((const float*)a.q + q0 + 8 * c, 0, x);
-                else load8<T>((const uint16_t*)a.q + q0 + 8 * c, 0, x);
+            for (int nb = 0; nb < NB; ++nb) {
+                const int row = r0 + 16 * nb + r16, rq = min(row, rows_total - 1), t = ka.grp.div(rq);
+                row_ok[nb] = row < rows_total;
+                t_of[nb] = t;
+                tok[nb] = s * a.max_tokens + t;
+                mask0[nb] = 0;
+                if (row_ok[nb] && a.masks && a.words == 1) mask0[nb] = a.masks[tok[nb]];
+                int rope_pos = 0;
                 if (a.rope_table) {
-                    const f32x4_t w0 = *(const f32x4_t*)(cs + 4 * c), w1 = *(const f32x4_t*)(cs + 4 * c + 2);
-                    const float c8[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
-                    rope4(x, c8);
+                    rope_pos = a.positions ? a.positions[tok[nb]] : ctx + t;
+                    row_ok[nb] = row_ok[nb] && rope_pos >= 0 && rope_pos < a.rope_positions;
                 }
-                const bool ok = row_ok[nb] && d_ok;
+                const int64_t q0 = ((int64_t)tok[nb] * a.q_heads + kvh * a.group + rq - t * a.group) * D + dq;
+                const float2* const cs =
+                    a.rope_table + ((int64_t)(row_ok[nb] ? rope_pos : 0) + a.rope_offset) * (D >> 1) + dq / 2;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = ok ? x[e] : 0.0f;
-                bf16_parts<NQ>(x, qop[nb][c]);
+                for (int c = 0; c < KS; ++c) {
+                    float x[8];
+                    if constexpr (C::F32) load8<T>((const float*)a.q + q0 + 8 * c, 0, x);
+                    else load8<T>((const uint16_t*)a.q + q0 + 8 * c, 0, x);
+                    if (a.rope_table) {
+                        const f32x4_t w0 = *(const f32x4_t*)(cs + 4 * c), w1 = *(const f32x4_t*)(cs + 4 * c + 2);
+                        const float c8[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
+                        rope4(x, c8);
+                    }
+                    const bool ok = row_ok[nb] && d_ok;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = ok ? x[e] : 0.0f;
+                    bf16_parts<NQ>(x, qop[nb][c]);
+                }
             }
-        }
+        };
+        if constexpr (COOP && !C::LATE) load_rows();
         f32x4_t oacc[NB][DB];
         float m_run[NB], l_run[NB];
 #pragma unroll
@@ -459,6 +460,27 @@ void fp4_split(Fp4KArgs ka) {
         const int scale_byte = (kvh * D + dl) / 32, scale_at = 8 * (scale_byte & 3);
         const int head_codes = (kvh * D + dl) / 2, head_scales = codes + (scale_byte & ~3);
 
+        // COOP: this lane's piece in each of its wave's transfers, as its address in row 0 and its row. Pieces of a
+        // step are numbered through the rows of K, then of V; the last ones of a row may not exist (the last that
+        // does is fetched again).
+        const uint8_t* piece_base[COOP ? C::NI : 1];
+        int piece_row[COOP ? C::NI : 1];
+        if constexpr (COOP) {
+            // pieces of codes; of scales, whose HW D / 32 bytes (16 at most) need not begin with one
+            const int cp = HW * D / 32, sp = 16 % cp == 0 ? 1 : 2;
+            const int seg_codes = unit * (HW * D / 2), seg_scales = codes + (unit * (HW * D / 32) & ~15);
+            int ln = lane;
+            asm volatile("" : "+v"(ln));  // (as dq)
+#pragma unroll
+            for (int i = 0; i < C::NI; ++i) {
+                const int p = min((wave + i * NW) * 64 + ln, 64 * C::RP - 1);
+                const int r = p / C::RP, c = min(p - r * C::RP, cp + sp - 1);
+                // (of two pieces of scales the second may lie past the row, and is not needed then)
+                const int at = c < cp ? seg_codes + 16 * c : min(seg_scales + 16 * (c - cp), ka.row_bytes - 16);
+                piece_row[i] = r & 31;
+                piece_base[i] = (const uint8_t*)(r < 32 ? a.k_pool : a.v_pool) + at;
+            }
+        }
         // (with a window, `skip` steps behind the first `before` are left out: a part of the loop ends there)
         for (int at0 = st0; at0 < st1;) {
         const int shift = at0 >= before ? skip : 0, c0 = at0 + shift;
@@ -515,16 +537,10 @@ void fp4_split(Fp4KArgs ka) {
                 row_lds[wave][lane] = (uint64_t)(uint32_t)(max(bt[lp - p0], 0) + key - lp * a.page_size) *
                                       (uint32_t)ka.row_bytes;
             }
-            const uint32_t seg_codes = unit * (HW * D / 2), seg_scales = codes + (unit * (HW * D / 32) & ~15);
 #pragma unroll
             for (int i = 0; i < C::NI; ++i) {
                 if (i >= n_ins) break;
-                const uint32_t pc = piece_of[i];
-                // (of two pieces of scales the second may lie past the row, and is not needed then)
-                const uint32_t at = pc & 64 ? min(seg_scales + (pc >> 7), (uint32_t)ka.row_bytes - 16u)
-                                            : seg_codes + (pc >> 7);
-                const uint8_t* const p =
-                    (const uint8_t*)(pc & 32 ? a.v_pool : a.k_pool) + (row_lds[wave][pc & 31] + at);
+                const uint8_t* const p = piece_base[i] + row_lds[wave][piece_row[i]];
                 fp4_to_lds16(p, stage0 + stage * C::STAGE + (wave + i * NW) * 1024);
             }
         };
@@ -694,6 +710,7 @@ void fp4_split(Fp4KArgs ka) {
             static_assert(C::NST == 3, "two steps ahead");
             transfer(c0, 0);
             if (c0 + 1 < c1) transfer(c0 + 1, 1);
+            if (C::LATE && at0 == st0) load_rows();  // (while the first keys are on their way)
             int stage = 0;
 #pragma unroll 1
             for (int step = c0; step < c1; ++step) {
@@ -716,6 +733,7 @@ void fp4_split(Fp4KArgs ka) {
         Tile even, odd;
         load_tile(c0, even);
         load_tile(min(c0 + 1, c1 - 1), odd);
+        if (at0 == st0) load_rows();
 #pragma unroll 1
         for (int step = c0; step < c1; step += 2) {
             process(even, step);
@@ -767,14 +785,15 @@ __global__ __launch_bounds__(256) void fp4_combine(Fp4KArgs ka, int hw, int nb_r
     const int lane = tid & 63, db = part * 4 + (tid >> 6);
     const int row = b16 * 16 + (lane & 15), d = 16 * db + 4 * (lane >> 4);
     const int rows_all = a.max_tokens * a.group;
-    const int rows_s = tree_rows_of(a, s), len = rows_s ? a.tree_lens[s] : 0;
+    // (all asked for together)
+    const int share = a.plan[a.n_seqs], ov = a.plan[a.n_seqs + 1], before = a.plan[s], len_s = a.tree_lens[s];
+    const int rows_s = tree_rows_of(a, s), len = rows_s ? len_s : 0;
     const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
     if (row < rows_all && row >= len * a.group && d < D)
         fp4_write<T>(a, s, kvh, row, d, zero, 0.0f, 0.0f, ka.grp);
     if (b16 * 16 >= len * a.group) return;
-    const int share = a.plan[a.n_seqs], ov = a.plan[a.n_seqs + 1];
     const int steps = fp4_steps(a, rows_s, len);
-    const uint32_t u0 = (uint32_t)a.plan[s] + (uint32_t)(kvh / hw) * (uint32_t)(steps + ov) + (uint32_t)ov;
+    const uint32_t u0 = (uint32_t)before + (uint32_t)(kvh / hw) * (uint32_t)(steps + ov) + (uint32_t)ov;
     const int g0 = (int)(u0 / (uint32_t)share), g1 = (int)((u0 + steps - 1) / (uint32_t)share);
     if (g0 == g1) return;  // finished by the range that covers it
     if (row >= len * a.group) return;
@@ -782,7 +801,7 @@ __global__ __launch_bounds__(256) void fp4_combine(Fp4KArgs ka, int hw, int nb_r
     const float c2 = a.scale * kLog2e;
     float M = -INFINITY, L = 0.0f;
     f32x4_t o = zero;
-    constexpr int UN = 4;
+    constexpr int UN = 8;
     for (int g = g0; g <= g1; g += UN) {
         float2 ml[UN];
         f32x4_t x[UN];
