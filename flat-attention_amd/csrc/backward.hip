@@ -1274,11 +1274,13 @@ void launch_backward(Dtype dt, const BackwardArgs& a, const BackwardSplit& sp, h
 }
 
 // ------------------------------------------------------------------ sliding windows
-// Key blocks without sinks have about window / 128 + 1 tiles a query head and go to `p` workgroups each, as
-// many as end first by rounds of the chip (a workgroup costs two tiles beside its own, one with partials four);
-// the blocks with sinks, which all queries see, are dealt out in pieces of a quarter of such a workgroup behind
-// them, which fill what the others leave: B1 Hq32 Hkv8 S4096 D128 bf16, window 1024, 4 sinks, has 248 workgroups
-// of up to 36 tiles and 128 tiles for the first block.
+// Key blocks without sinks have about window / 128 + 1 tiles a query head and go to `p` workgroups each; the
+// blocks with sinks, which all queries see, are dealt out in smaller pieces behind them, which fill what the
+// others leave. Both counts are those that end first by places of the chip, with two tiles for a workgroup's
+// start and end and four where it writes partials: B1 Hq32 Hkv8 S4096 D128 bf16, window 1024, 4 sinks, has 248
+// workgroups of up to 36 tiles and 128 tiles a unit for the first block (us, pieces of a quarter of the others / of
+// this rule: 360 / 328; S2048 184 / 171, S8192 663 / 659, B2 645 / 636, 200 sinks 374 / 367, a window of 4000 722 /
+// 744).
 WindowSplit window_split(Dtype dt, const BackwardArgs& a, uint64_t limit) {
     WindowSplit sp{};
     const int64_t units = (int64_t)a.batch * a.kv_heads, cus = device_cus();
@@ -1294,19 +1296,43 @@ WindowSplit window_split(Dtype dt, const BackwardArgs& a, uint64_t limit) {
     const int64_t most = plain ? tiles(sp.sink_blocks) : 0, longest = sp.sink_blocks ? tiles(0) : 0;
     int64_t all = 0;
     for (int kb = 0; kb < sp.blocks; ++kb) all += tiles(kb);
-    int64_t chunk = std::max<int64_t>(most, 1), best = INT64_MAX;
-    for (int64_t p = 1; p <= 16 && plain; ++p) {
-        const int64_t c = (most + p - 1) / p, rounds = (units * plain * p + places - 1) / places;
-        const int64_t time = std::max(rounds * (c + (p > 1 ? 4 : 2) * step),
-                                      (all * units + places - 1) / places + (p > 1 ? 4 : 2) * step);
-        if (time < best && (p == 1 || c >= step)) {
-            best = time;
-            chunk = c;
+    // when `n` workgroups of `d` and then `m` of `e` end: r rounds of the first leave `rest` places busy longer
+    auto ends = [&](int64_t n, int64_t d, int64_t m, int64_t e) {
+        const int64_t r = n / places, rest = n - r * places, t0 = r * d, t1 = rest ? t0 + d : t0;
+        auto done = [&](int64_t t) { return (places - rest) * ((t - t0) / e) + rest * (std::max<int64_t>(0, t - t1) / e); };
+        int64_t at0 = t0 + m / places * e, at1 = t1;
+        while (done(at0) < m) at0 += e;
+        while (at1 < at0 && done(at1) < m) at1 += e;
+        return std::max(t1, std::min(at0, at1));
+    };
+    int64_t chunk = std::max<int64_t>(most, 1), piece = std::max<int64_t>(longest, 1), best = INT64_MAX;
+    for (int64_t p = 1; p <= (plain ? 16 : 1); ++p) {
+        const int64_t c = (most + p - 1) / p, d = c + (p > 1 ? 4 : 2) * step;
+        if (p > 1 && c < step) break;
+        if (small && plain) {
+            // (many short pieces cost more than an even end gives: B2 Hq4 Hkv2 S300 D64 26.4 us so, 31 as below)
+            const int64_t time = std::max((units * plain * p + places - 1) / places * d,
+                                          (all * units + places - 1) / places + (p > 1 ? 4 : 2) * step);
+            if (time < best) {
+                best = time;
+                chunk = std::max<int64_t>(c, 1);
+                piece = std::max<int64_t>(chunk / 4, 2 * step);
+            }
+            continue;
+        }
+        for (int64_t q : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+            const int64_t l = (longest + q - 1) / q;
+            if (q > 1 && l < 2 * step) break;
+            const int64_t time =
+                ends(units * plain * p, d, longest ? units * sp.sink_blocks * q : 0, l + (q > 1 ? 4 : 2) * step);
+            if (time < best) {
+                best = time;
+                chunk = std::max<int64_t>(c, 1);
+                piece = std::max<int64_t>(l, 1);
+            }
         }
     }
     // (larger pieces where the partials would take more than `limit`: many sinks over a long sequence)
-    int64_t piece = plain ? std::max<int64_t>(chunk / 4, 2 * step)
-                          : std::max<int64_t>((all * units + places - 1) / places, 2 * step);
     for (;; chunk *= 2, piece *= 2) {
         sp.chunk = (int)std::min(chunk, std::max<int64_t>(most, 1));
         sp.parts = plain ? (int)((most + sp.chunk - 1) / sp.chunk) : 1;
