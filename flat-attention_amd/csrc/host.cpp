@@ -3328,7 +3328,7 @@ int fa_backward_gqa_window(fa_ctx* ctx, const void* q, const void* k, const void
     if (int rc = resolve_scale(cfg, sh->head_dim, &scale)) return rc;
     if (int rc = check_window_shape(sh, cfg, window, dtype)) return rc;
     for (const auto& t : ptrs)
-        if (t.p != (const void*)lse)
+        if (strcmp(t.name, "LSE"))
             if (int rc = check_aligned(t.name, t.p)) return rc;
     if (!ctx) return fail(FA_ERR_NULL_ARGUMENT, "context is null");
     begin_call(ctx);
@@ -3557,7 +3557,10 @@ int move_rows(fa_ctx* ctx, const fa_paged_batch* b, const int32_t* slots, size_t
     end_span(ctx, FA_KERNEL_PAGED_APPEND);
     HIP_TRY(hipGetLastError());
     record(ctx, FA_KERNEL_PAGED_APPEND,
-           what == Rows::kAppend ? "append_slots" : what == Rows::kAppendFp4 ? "append_fp4" : "read_fp4", 0, (uint32_t)b->page_size, grid, 256, 1, 1,
+           what == Rows::kAppend      ? "append_slots"
+           : what == Rows::kAppendFp4 ? "append_fp4"
+                                      : "read_fp4",
+           0, (uint32_t)b->page_size, grid, 256, 1, 1,
            nullptr);
     return ok();
 }

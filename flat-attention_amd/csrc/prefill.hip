@@ -1940,6 +1940,14 @@ void launch_prefill(Dtype dt, bool paged, const PrefillArgs& a, hipStream_t s, u
 }
 
 // ------------------------------------------------------------------ sliding windows
+// 4 D operations a seen pair and head over one reading of K and V: bound by the matrix cores and the softmax between
+// their products, as the kernels without a window (bf16 D 128, Hq32 Hkv8 S8192, window 1024, 4 sinks: 166 us, 778
+// TFLOP/s of seen pairs; the tiles at both edges of a block of 64 positions are a ninth more). Rows of 16-bit
+// storage per workgroup: 256 in the ping-pong schedule, 128 with two groups of keys, 64 with four, the least
+// that leave no CU without a workgroup's worth (us for 256 / 128 / 64: f16 D80 B2 Hq16 Hkv4, window 500, S500
+// 18.6 / 13.6 / 12.8, S1000 26.6 / 17.5 / 26.6, S1999 28.4 / 33.4 / 54; bf16 D128 Hq32 Hkv8, window 1024, S500 18.7 /
+// 14.2 / 12.3, S1000 27.9 / 20.6 / 24.5, S2000 37.9 / 42.5 / 60). f32: 128 rows, or 32 with groups of keys (D64 Hq2
+// Hkv2, window 32: S128 21.6 / 7.5, B4 S2000 28.7 / 14.6, B16 S2000 51.5 / 52.5).
 template <typename T, int DPAD, bool FULLD>
 static void launch_window16(const PrefillKArgs& ka, int kw, dim3 grid, hipStream_t s) {
     if (kw == 4)

@@ -236,7 +236,8 @@ int fa_forward_gqa_rope(fa_ctx* ctx, const void* q, size_t q_bytes, const void* 
  * A window as long as the sequence is plain causal attention. Layouts and arguments as for
  * fa_forward_gqa_rope; config->causal must be set (else FA_ERR_CAUSAL_VISIBILITY_MISMATCH), head_dim is a
  * multiple of 8, every tensor starts at a multiple of 16 bytes (FA_ERR_MISALIGNED), and one (batch, head)
- * slice takes less than 2 GiB. Only the tiles of keys that some row of a block sees are read. LSE has f32
+ * slice takes less than 2 GiB. Only the tiles of keys that some row of a block sees are read; an infinity or NaN
+ * in V may reach rows of the same block that do not see it, as without a window (0 times infinity). LSE has f32
  * accuracy with 16-bit storage too, except that with rotary the rotated Q and K are rounded to it first, in
  * the default manner of fa_ctx_set_prefill_precision, whose mode does not apply here. It can be captured
  * once the context's caches are sized (rotary only). */
