@@ -315,6 +315,59 @@ def test_scales_from_the_smallest_to_the_largest(hip):
     case.check()
 
 
+@pytest.mark.parametrize("dtype,most,hq,hkv,D", [(BF16, 1, 16, 8, 128), (F16, 9, 8, 8, 64), (F32, 9, 8, 4, 128),
+                                                 (F16, 3, 6, 3, 96)])
+def test_two_contexts_at_once_give_the_same_bits_each_time(hip, dtype, most, hq, hkv, D):
+    other = fa.HipContext(0)
+    try:
+        cases = [Case(c, dtype, [900, 3, 77, 2100], [most, 1, most, most], most, hq, hkv, D, 16, seed=5)
+                 for c in (hip, other)]
+        bits = []
+        for _ in range(3):
+            for c in cases:
+                c.out.fill_u32(0x7fc07fc0)
+            for _ in range(2):
+                for c in cases:
+                    c.call()
+            for c in cases:
+                bits.append(c.out.download(np.uint8, c.lay.combined_bytes))
+        assert all(np.array_equal(b, bits[0]) for b in bits)
+        for c in cases:
+            c.check()
+    finally:
+        del cases
+        other.close()
+
+
+@pytest.mark.parametrize("hkv,D,most", [(8, 128, 1), (4, 96, 6), (3, 64, 6)])
+def test_rows_past_four_gigabytes_of_a_pool(hip, hkv, D, most):
+    """The same rows at the end of pools that 32 bits do not address, and in small ones: the same bits."""
+    rng = np.random.default_rng(hkv)
+    rb, page, n, width, dtype = fa.fp4_row_bytes(hkv, D), 16, 2, 5, BF16
+    hq = 2 * hkv
+    keys = [storage(rng.standard_normal((n, width * page, hkv, D)), dtype)[1] for _ in range(2)]
+    q = storage(rng.standard_normal((n, most, hq, D)), dtype)[1]
+    order = rng.permutation(n * width).reshape(n, width)
+    results = []
+    for pages in (n * width, (1 << 32) // (rb * page) + 2 * n * width):
+        table = (pages - n * width + order).astype(np.int32)
+        pools = [fa.DeviceBuffer(hip, pages * page * rb) for _ in range(2)]
+        batch = fa.HipPagedBatch(hip, i32(hip, table), i32(hip, [width * page - most, 33]), n, width, page, pages)
+        at = np.arange(width * page)
+        slots = i32(hip, table[:, at // page] * page + at % page)
+        batch.append_fp4(slots, width * page, *(buf(hip, x) for x in keys), *pools, hkv, D, None, dtype)
+        out = [fa.DeviceBuffer(hip, x.nbytes) for x in keys]
+        batch.read_fp4(slots, width * page, *pools, *out, hkv, D, dtype)
+        lay = batch.layout(most, hq, D, dtype)
+        o = fa.DeviceBuffer(hip, lay.combined_bytes)
+        batch.attention_fp4(buf(hip, q), *pools, o, i32(hip, [most, most]), most, hq, hkv, D,
+                            fa.FlatAttentionConfig(True), None, dtype)
+        results.append([x.download(np.uint8, x_bytes) for x, x_bytes in
+                        ((out[0], keys[0].nbytes), (out[1], keys[1].nbytes), (o, lay.combined_bytes))])
+    assert all(np.array_equal(a, b) for a, b in zip(*results))
+    assert np.isfinite(fa.storage_to_f32(results[0][0].view(np.uint16), dtype)).all()
+
+
 # ------------------------------------------------------------------------------- together
 
 @pytest.mark.parametrize("windowed", [False, True])
