@@ -218,10 +218,9 @@ struct Fp4KArgs {
     int row_bytes;
 };
 
-// Which 16-byte column (of 8; two rows share the 16 of all banks) a piece of a V row is kept in: piece ^
-// fp4_swizzle(row), so that the columns hold one piece of sixteen rows (the stores), and two neighbouring
-// pieces of eight rows (half a transposing read), once each.
-__device__ __forceinline__ int fp4_swizzle(int row) { return ((row >> 1) & 3) << 1 | ((row >> 3) & 1); }
+// Which 16-byte column (of 8) a piece of a V row is kept in: piece ^ fp4_swizzle(row), so that eight rows of one
+// piece (a store's clock) and the two neighbouring pieces of eight rows (half a transposing read) lie in all banks.
+__device__ __forceinline__ int fp4_swizzle(int row) { return row & 7; }
 
 __device__ __forceinline__ void fp4_to_lds16(const void* p, uint32_t lds) {
     asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(lds));
