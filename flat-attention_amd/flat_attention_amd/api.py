@@ -122,6 +122,8 @@ class AttentionWindow:
     sinks: int = 0
 
     def c(self):
+        if self.window < 0 or self.sinks < 0:  # (as unsigned numbers they would be the longest)
+            raise ValueError("window and sinks must not be negative")
         return L.WindowC(self.window, self.sinks)
 
 

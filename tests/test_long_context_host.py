@@ -211,6 +211,12 @@ def test_model_gradient_matches_differences(S, window, sinks, hq, hkv):
             assert abs((moved[0] - moved[1]) / (2 * eps) - grads[n][at]) < 1e-5
 
 
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (4, -1)])
+def test_negative_windows_are_refused(window, sinks):
+    with pytest.raises(ValueError, match="negative"):
+        fa.AttentionWindow(window, sinks).c()
+
+
 def test_model_forward_is_the_definition():
     rng = np.random.default_rng(0)
     q, k, v = rng.standard_normal((3, 1, 7, 4))
